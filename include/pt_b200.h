@@ -430,6 +430,31 @@ int pt_rmsnorm_quantize_mx_row(const void *x, int x_dtype, const void *gamma, fl
 int pt_shuffle_e8m0_scale(const uint8_t *scale, int64_t M, int64_t N, uint8_t *out, void *stream);
 int pt_shuffle_mx_codes(const void *codes, int64_t M, int64_t row_bytes, void *out, void *stream);
 
+/* ---- per-head RMS norm and position rotation of queries and keys (csrc/qk_norm_rope.cu) -----------------------------
+ * q [B, S, Hq, D], k [B, S, Hk, D] with D contiguous; `*_strides` are host arrays of three element strides (batch, token,
+ * head), so views into a packed projection are read in place.  Outputs are contiguous.  dtype PT_BF16 / PT_F16 / PT_F32 for
+ * q, k, the gains [D] and the outputs; cos, sin fp32 [P, R / 2].
+ *   n = x * rsqrt(mean(x^2) + eps) * (gamma, or 1 + gamma when zero_centered);  the first R (even) elements of n are rotated in
+ *   pairs (i, i + R / 2), or (2 i, 2 i + 1) when interleaved, by the angle of the token's position; the rest pass through.
+ * positions: int32 / int64 [B * S] (pos_bytes 4 / 8), or null with pos_bytes 0: the token's index inside its batch entry.
+ * A position outside [0, P): that token's outputs (and gradients) are zeros and *status (optional, device or mapped host
+ * int) receives PT_ERR_INVALID.  D at most 1024.
+ * (The reference has no such operator: its models call rmsnorm of primus_turbo/pytorch/ops/normalization.py per head and
+ * rotate outside.) */
+int pt_qk_norm_rope_fwd(const void *q, const void *k, int dtype, const void *q_gamma, const void *k_gamma, const float *cos, const float *sin,
+                        const void *positions, int pos_bytes, int64_t B, int64_t S, int64_t P, int Hq, int Hk, int D, int R,
+                        const int64_t *q_strides, const int64_t *k_strides, float eps, int interleaved, int zero_centered, void *q_out,
+                        void *k_out, int *status, void *stream);
+
+/* Backward: dq, dk (strided like q, k) are the gradients of the outputs; writes the gradients of q, k (contiguous) and of the
+ * gains.  `partial` fp32 [parts, D] scratch, parts = pt_qk_norm_rope_bwd_parts(B * S, Hq, Hk).  Same bits every run. */
+int pt_qk_norm_rope_bwd_parts(int64_t tokens, int Hq, int Hk);
+int pt_qk_norm_rope_bwd(const void *dq, const void *dk, const void *q, const void *k, int dtype, const void *q_gamma, const void *k_gamma,
+                        const float *cos, const float *sin, const void *positions, int pos_bytes, int64_t B, int64_t S, int64_t P, int Hq,
+                        int Hk, int D, int R, const int64_t *dq_strides, const int64_t *dk_strides, const int64_t *q_strides,
+                        const int64_t *k_strides, float eps, int interleaved, int zero_centered, void *dq_in, void *dk_in, void *dq_gamma,
+                        void *dk_gamma, float *partial, int parts, int *status, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

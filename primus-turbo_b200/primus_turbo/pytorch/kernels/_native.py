@@ -12,6 +12,7 @@ PT_E4M3, PT_E5M2, PT_E2M1 = 0, 1, 2
 PT_TENSORWISE, PT_ROWWISE, PT_BLOCKWISE, PT_MX_BLOCKWISE = 0, 1, 2, 3
 PT_MX_ROW, PT_MX_COL, PT_MX_ROW_2D, PT_MX_COL_2D, PT_MX_ROW_RHT, PT_MX_COL_RHT = 1, 2, 4, 8, 16, 32
 PT_MX_ROW_SR, PT_MX_COL_SR = 64, 128
+PT_ERR_INVALID = -1
 
 _SRC = {torch.bfloat16: PT_BF16, torch.float16: PT_F16, torch.float32: PT_F32}
 _FMT = {torch.float8_e4m3fn: PT_E4M3, torch.float8_e5m2: PT_E5M2, torch.float4_e2m1fn_x2: PT_E2M1}
@@ -66,6 +67,7 @@ def require_cuda(*tensors):
 
 _status = {}
 _poll = {}
+_host_status = {}
 
 
 def status_word(device) -> torch.Tensor:
@@ -82,7 +84,31 @@ def status_word(device) -> torch.Tensor:
     return _status[idx]
 
 
+def host_status(device):
+    """Per-device status word in pinned host memory, which the kernels of the operators built for single calls write directly
+    (mapped, so the address is the device's too).  Reading it is one host load: a copy and an event per call, as poll_status
+    makes, would cost such an operator as much as its kernel."""
+    idx = device.index
+    w = _host_status.get(idx)
+    if w is None:
+        t = torch.zeros(1, dtype=torch.int32).pin_memory()
+        w = _host_status[idx] = (t, ctypes.c_int32.from_address(t.data_ptr()), ctypes.c_void_p(t.data_ptr()))
+    return w
+
+
+def poll_host_status(device):
+    """Raises if a kernel launched earlier has reported an error into the host status word (it is not waited for: the error
+    of a launch surfaces at a following call, or at check_status())."""
+    w = _host_status.get(device.index)
+    if w is not None and w[1].value != 0:
+        code, w[1].value = w[1].value, 0
+        _raise(code)
+
+
 def _raise(code):
+    if code == PT_ERR_INVALID:
+        raise RuntimeError("a kernel was given an index outside of its table (a position beyond the cos / sin rows); the rows of that "
+                           "launch with such an index are zeros")
     raise RuntimeError(f"a kernel gave up waiting on a barrier (status {code}); the output of that launch is invalid")
 
 
@@ -93,6 +119,7 @@ def check_status(device):
     if code != 0:
         s.zero_()
         _raise(code)
+    poll_host_status(s.device)
 
 
 def poll_status(device):

@@ -1,7 +1,10 @@
-"""rmsnorm / rmsnorm_residual with autograd; interface of primus_turbo/pytorch/ops/normalization.py of the reference."""
-from typing import Tuple
+"""rmsnorm / rmsnorm_residual with autograd; interface of primus_turbo/pytorch/ops/normalization.py of the reference.
+qk_norm_rope, which the reference lacks: the norm of every query and key head and the position rotation in one pass."""
+from typing import Optional, Tuple
 
 import torch
+
+from ..kernels.normalization.qk_norm_rope_impl import qk_norm_rope_bwd_impl, qk_norm_rope_fwd_impl
 
 from ..kernels.normalization.rmsnorm_impl import (
     rmsnorm_bwd_impl,
@@ -10,7 +13,7 @@ from ..kernels.normalization.rmsnorm_impl import (
     rmsnorm_fwd_residual_impl,
 )
 
-__all__ = ["rmsnorm", "rmsnorm_residual"]
+__all__ = ["rmsnorm", "rmsnorm_residual", "qk_norm_rope"]
 
 
 class _RMSNormFunction(torch.autograd.Function):
@@ -58,3 +61,69 @@ def rmsnorm(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, zero_center
 def rmsnorm_residual(x: torch.Tensor, residual: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
     """(rmsnorm(x + residual), x + residual) in one pass over the row."""
     return _RMSNormResidualFunction.apply(x, residual, gamma, eps)
+
+
+class _QKNormRopeFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_gamma, k_gamma, cos, sin, positions, eps, interleaved, zero_centered):
+        ctx.save_for_backward(q, k, q_gamma, k_gamma, cos, sin, positions)
+        ctx.options = (eps, interleaved, zero_centered)
+        return qk_norm_rope_fwd_impl(q, k, q_gamma, k_gamma, cos, sin, positions, eps, interleaved, zero_centered)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        q, k, q_gamma, k_gamma, cos, sin, positions = ctx.saved_tensors
+        dq, dk = (d.to(q.dtype) if d.stride(-1) == 1 else d.to(q.dtype).contiguous() for d in (dq, dk))
+        return (*qk_norm_rope_bwd_impl(dq, dk, q, k, q_gamma, k_gamma, cos, sin, positions, *ctx.options),) + (None,) * 6
+
+
+def _as_heads(x, name):
+    """x [..., heads, D] as [B, S, heads, D] with a contiguous last dimension, without a copy where its strides allow it."""
+    assert x.dim() >= 3, f"qk_norm_rope: {name} must be [..., tokens, heads, D], got {tuple(x.shape)}"
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+    if x.dim() == 4:
+        return x
+    return x.unsqueeze(0) if x.dim() == 3 else x.flatten(0, -4)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor, k_gamma: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                 positions: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                 zero_centered: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every query and key head, then the position rotation: (q_out, k_out), contiguous, in one pass.
+
+    q [..., tokens, Hq, D] and k [..., tokens, Hk, D]: bf16, fp16 or fp32, any strides with a contiguous last dimension (views
+    into a packed projection are read in place).  q_gamma, k_gamma [D] in the same dtype; cos, sin fp32 [P, R / 2].
+    n = x * rsqrt(mean(x^2, -1) + eps) * (gamma, or 1 + gamma when zero_centered); the first R elements of n are rotated in pairs
+    (i, i + R / 2), or (2 i, 2 i + 1) when interleaved, by cos / sin of the token's position; elements from R on pass through.
+    positions: int32 / int64 of the shape [..., tokens]; None: 0, 1, ... along the token dimension.  A position outside of
+    [0, P) gives zeros for its token and an error at a following call.  Differentiable in q, k and the gains."""
+    for t in (q, k, q_gamma, k_gamma, cos, sin, positions):
+        if t is not None and not t.is_cuda:
+            raise RuntimeError("primus_turbo (B200) operators take CUDA tensors only; there is no CPU path")
+    D = q.shape[-1]
+    assert q.dtype in (torch.bfloat16, torch.float16, torch.float32), f"qk_norm_rope: unsupported dtype {q.dtype}"
+    assert k.dtype == q.dtype == q_gamma.dtype == k_gamma.dtype, "qk_norm_rope: q, k and the gains must have one dtype"
+    assert k.dim() == q.dim() and k.shape[:-2] == q.shape[:-2] and k.shape[-1] == D, \
+        f"qk_norm_rope: q {tuple(q.shape)} and k {tuple(k.shape)} must agree but in their heads"
+    assert tuple(q_gamma.shape) == (D,) and tuple(k_gamma.shape) == (D,), "qk_norm_rope: the gains must be [D]"
+    assert cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape, \
+        "qk_norm_rope: cos and sin must be float32 [positions, R / 2]"
+    assert 2 * cos.shape[1] <= D, f"qk_norm_rope: the tables rotate {2 * cos.shape[1]} elements of heads of {D}"
+    assert not (cos.requires_grad or sin.requires_grad), "qk_norm_rope: the tables are not differentiated"
+    assert len({t.device for t in (q, k, q_gamma, k_gamma, cos, sin)}) == 1, "qk_norm_rope: all tensors must be on one device"
+    q4, k4 = _as_heads(q, "q"), _as_heads(k, "k")
+    if positions is not None:
+        assert positions.dtype in (torch.int32, torch.int64), "qk_norm_rope: positions must be int32 or int64"
+        assert positions.shape == q.shape[:-2], f"qk_norm_rope: positions {tuple(positions.shape)} must be [..., tokens] {tuple(q.shape[:-2])}"
+        assert positions.device == q.device, "qk_norm_rope: all tensors must be on one device"
+        positions = positions.contiguous()
+    else:
+        assert q.shape[-3] <= cos.shape[0], f"qk_norm_rope: {q.shape[-3]} tokens need as many rows of cos / sin, got {cos.shape[0]}"
+    args = (q4, k4, q_gamma.contiguous(), k_gamma.contiguous(), cos.contiguous(), sin.contiguous(), positions, float(eps), bool(interleaved),
+            bool(zero_centered))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_gamma.requires_grad or k_gamma.requires_grad):
+        q_out, k_out = _QKNormRopeFunction.apply(*args)
+    else:
+        q_out, k_out = qk_norm_rope_fwd_impl(*args)
+    return (q_out, k_out) if q.dim() == 4 else (q_out.view(q.shape), k_out.view(k.shape))

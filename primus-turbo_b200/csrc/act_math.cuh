@@ -11,10 +11,15 @@
 
 namespace ptb {
 
-enum { PT_ACT_SILU = 0, PT_ACT_GELU = 1 };
+// the first two are also the gated activations'; the rest are epilogue activations of gemm_bias_act
+enum { PT_ACT_SILU = 0, PT_ACT_GELU = 1, PT_ACT_NONE = 2, PT_ACT_RELU = 3, PT_ACT_GELU_TANH = 4 };
 
 template <int ACT> __device__ __forceinline__ float act_value(float a) {
     if constexpr (ACT == PT_ACT_SILU) return __fdividef(a, 1.0f + __expf(-a));
+    else if constexpr (ACT == PT_ACT_RELU) return a < 0.0f ? 0.0f : a;   // a NaN stays
+    // tanh form of the GELU, 0.5 a (1 + tanh u) with u = sqrt(2 / pi) (a + 0.044715 a^3), as a / (1 + exp(-2 u)): no cancellation
+    else if constexpr (ACT == PT_ACT_GELU_TANH) return __fdividef(a, 1.0f + __expf(-1.5957691216f * a * (1.0f + 0.044715f * a * a)));
+    else if constexpr (ACT == PT_ACT_NONE) return a;
     else return 0.5f * a * (1.0f + erff(a * 0.7071067811f));
 }
 // d act(a) / d a
@@ -22,11 +27,42 @@ template <int ACT> __device__ __forceinline__ float act_grad(float a) {
     if constexpr (ACT == PT_ACT_SILU) {
         const float s = __fdividef(1.0f, 1.0f + __expf(-a));
         return s * (1.0f + a * (1.0f - s));
+    } else if constexpr (ACT == PT_ACT_RELU) {
+        return a > 0.0f ? 1.0f : 0.0f;
+    } else if constexpr (ACT == PT_ACT_GELU_TANH) {
+        const float s = __fdividef(1.0f, 1.0f + __expf(-1.5957691216f * a * (1.0f + 0.044715f * a * a)));
+        return s + a * s * (1.0f - s) * 1.5957691216f * (1.0f + 0.134145f * a * a);
+    } else if constexpr (ACT == PT_ACT_NONE) {
+        return 1.0f;
     } else {
         return 0.3989422803f * a * __expf(-(0.7071067811f * a) * (0.7071067811f * a)) + 0.5f * erff(0.7071067811f * a) + 0.5f;
     }
 }
 template <int ACT> __device__ __forceinline__ float glu_value(float a, float b, float p) { return act_value<ACT>(a) * b * p; }
+
+// The activation chosen at run time (uniform over the launch), and the same for four values under one branch.
+__device__ __forceinline__ float act_any(int act, float v) {
+    switch (act) {
+    case PT_ACT_SILU: return act_value<PT_ACT_SILU>(v);
+    case PT_ACT_GELU: return act_value<PT_ACT_GELU>(v);
+    case PT_ACT_RELU: return act_value<PT_ACT_RELU>(v);
+    case PT_ACT_GELU_TANH: return act_value<PT_ACT_GELU_TANH>(v);
+    default: return v;
+    }
+}
+__device__ __forceinline__ void act_any4(int act, float (&v)[4]) {
+    auto all = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = f(v[i]);
+    };
+    switch (act) {
+    case PT_ACT_SILU: all([](float x) { return act_value<PT_ACT_SILU>(x); }); break;
+    case PT_ACT_GELU: all([](float x) { return act_value<PT_ACT_GELU>(x); }); break;
+    case PT_ACT_RELU: all([](float x) { return act_value<PT_ACT_RELU>(x); }); break;
+    case PT_ACT_GELU_TANH: all([](float x) { return act_value<PT_ACT_GELU_TANH>(x); }); break;
+    default: break;
+    }
+}
 
 __device__ __forceinline__ float rmsnorm_value(float x, float rstd, float g) { return x * rstd * g; }
 

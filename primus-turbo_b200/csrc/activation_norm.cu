@@ -488,6 +488,96 @@ __global__ void __launch_bounds__(32 * kDgLanes) rmsnorm_dgamma_kernel(const flo
     }
 }
 
+// ---------------------------------------------------------------------------------------------- backward of act(z) with z = . + bias
+// dz = dy * act'(z) in the operands' type (the next products' operand: rounded once), and the column sums of the unrounded dz for
+// the bias.  HBM-bound: dy and z read once, dz written once.  A warp walks rows of a 32 V-column strip, four rows' loads in
+// flight; the CTA's warps meet in shared memory and leave one row of partial sums per CTA, which bias_grad_kernel adds up in order.
+constexpr int kAbWarps = 8;
+template <typename T, typename DyT, int V, bool ACT>
+__global__ void __launch_bounds__(32 * kAbWarps) act_bias_bwd_kernel(const DyT *__restrict__ dy, const T *__restrict__ z, int act, int64_t M, int64_t N,
+                                                                     int64_t rows_per_cta, T *__restrict__ dz, float *__restrict__ partial) {
+    __shared__ float s_sum[kAbWarps][32 * V + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t col = ((int64_t) blockIdx.x * 32 + lane) * V;
+    const int64_t r0 = (int64_t) blockIdx.y * rows_per_cta, r1 = min(M, r0 + rows_per_cta);
+    float sum[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.f;
+    constexpr int U = 4;
+    if (col < N) {
+        for (int64_t r = r0 + warp; r < r1; r += kAbWarps * U) {
+            Vec<DyT, V> d[U];
+            Vec<T, V> zv[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t rr = r + u * kAbWarps;
+                if (rr >= r1) continue;
+                d[u] = ldv_plain<DyT, V>(dy + rr * N + col);
+                if constexpr (ACT) zv[u] = ldv_plain<T, V>(z + rr * N + col);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t rr = r + u * kAbWarps;
+                if (rr >= r1) continue;
+                float g[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[i] = an_to_f<DyT>(d[u].e[i]);
+                if constexpr (ACT) {
+                    auto scale = [&](auto f) {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) g[i] *= f(an_to_f<T>(zv[u].e[i]));
+                    };
+                    switch (act) {
+                    case PT_ACT_SILU: scale([](float x) { return act_grad<PT_ACT_SILU>(x); }); break;
+                    case PT_ACT_GELU: scale([](float x) { return act_grad<PT_ACT_GELU>(x); }); break;
+                    case PT_ACT_RELU: scale([](float x) { return act_grad<PT_ACT_RELU>(x); }); break;
+                    default: scale([](float x) { return act_grad<PT_ACT_GELU_TANH>(x); }); break;
+                    }
+                }
+                if (dz != nullptr) {
+                    Vec<T, V> o;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o.e[i] = an_from_f<T>(g[i]);
+                    stv<T, V>(dz + rr * N + col, o);
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[i] += g[i];
+            }
+        }
+    }
+    if (partial == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) s_sum[warp][lane * V + i] = sum[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * V; c += 32 * kAbWarps) {
+        const int64_t n = (int64_t) blockIdx.x * 32 * V + c;
+        if (n >= N) continue;
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < kAbWarps; ++w) t += s_sum[w][c];
+        partial[(int64_t) blockIdx.y * N + n] = t;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) bias_grad_kernel(const float *__restrict__ partial, int parts, int64_t N, T *__restrict__ dbias) {
+    __shared__ float s_sum[8][33];
+    const int c = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t n = (int64_t) blockIdx.x * 32 + c;
+    float acc = 0.f;
+    if (n < N)
+#pragma unroll 4
+        for (int p = w; p < parts; p += 8) acc += partial[(int64_t) p * N + n];
+    s_sum[w][c] = acc;
+    __syncthreads();
+    if (w == 0 && n < N) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t += s_sum[i][c];
+        dbias[n] = an_from_f<T>(t);
+    }
+}
+
 // Grid of a block-per-row kernel: no more CTAs than are resident at once, and the same number of rows for each, give or
 // take one (a fixed "SMs x 8" grid left the last of its 1.6 waves 60 % full on kernels that fit five CTAs per SM).
 template <typename Kernel> static int an_grid(Kernel kern, int64_t rows) {
@@ -598,6 +688,57 @@ int pt_rmsnorm_bwd(const void *dy, const void *dxpr, const void *x, const void *
         rmsnorm_dgamma_kernel<T><<<(unsigned) ceil_div(H, 32), 32 * kDgLanes, 0, st>>>(dg_partial, parts, H, (T *) dgamma);
     });
     PT_LAUNCH_OK();
+    return PT_OK;
+}
+
+int pt_act_bias_bwd_parts(int64_t M, int64_t N) {
+    // row chunks so that about eight CTAs per SM run over the column strips, of at least 64 rows
+    const int64_t strips = std::max<int64_t>(1, ceil_div(N, 256));
+    const int64_t want = std::max<int64_t>(1, (int64_t) sm_count() * 8 / strips);
+    return (int) std::max<int64_t>(1, std::min<int64_t>(want, ceil_div(M, 64)));
+}
+
+int pt_act_bias_bwd(const void *dy, int dy_dtype, const void *z, int dtype, int act, int64_t M, int64_t N, void *dz, void *dbias, int dbias_dtype,
+                    float *partial, int parts, void *stream) {
+    PT_REQUIRE(M >= 0 && N >= 0, "act_bias backward: bad shape");
+    PT_REQUIRE(dtype == PT_BF16 || dtype == PT_F16, "act_bias backward: bf16 or fp16 operands");
+    PT_REQUIRE(dy_dtype == PT_BF16 || dy_dtype == PT_F16 || dy_dtype == PT_F32, "act_bias backward: bad gradient dtype");
+    PT_REQUIRE(!dbias || dbias_dtype == PT_BF16 || dbias_dtype == PT_F16 || dbias_dtype == PT_F32, "act_bias backward: bad bias dtype");
+    PT_REQUIRE(act >= PT_ACT_SILU && act <= PT_ACT_GELU_TANH, "act_bias backward: bad activation %d", act);
+    PT_REQUIRE(!dbias || (partial && parts == pt_act_bias_bwd_parts(M, N)), "act_bias backward: bias buffers / part count");
+    if (N == 0) return PT_OK;
+    const bool with_act = act != PT_ACT_NONE;
+    PT_REQUIRE(M == 0 || (dy && (!with_act || z)), "act_bias backward: null pointer");
+    cudaStream_t st = (cudaStream_t) stream;
+    const int64_t rows_per_cta = ceil_div(std::max<int64_t>(M, 1), parts > 0 ? parts : pt_act_bias_bwd_parts(M, N));
+    const int64_t row_ctas = dbias ? parts : ceil_div(M, rows_per_cta);
+    float *part = dbias ? partial : nullptr;
+    if (row_ctas > 0) {
+        PT_REQUIRE(row_ctas < 65536 && ceil_div(N, 32) < (1ll << 31), "act_bias backward: grid too large");
+#define PT_AB(V_, ACT_, DY_)                                                                                                                      \
+    act_bias_bwd_kernel<T, DY_, V_, ACT_><<<dim3((unsigned) ceil_div(N, 32 * V_), (unsigned) row_ctas), 32 * kAbWarps, 0, st>>>(                  \
+        (const DY_ *) dy, (const T *) z, act, M, N, rows_per_cta, (T *) dz, part)
+#define PT_AB_DY(DY_)                                                                                                                            \
+    do {                                                                                                                                          \
+        if (N % 8 == 0 && aligned(dy, 8 * sizeof(DY_)) && aligned(z, 16) && aligned(dz, 16)) {                                                    \
+            if (with_act) PT_AB(8, true, DY_); else PT_AB(8, false, DY_);                                                                         \
+        } else {                                                                                                                                  \
+            if (with_act) PT_AB(1, true, DY_); else PT_AB(1, false, DY_);                                                                         \
+        }                                                                                                                                         \
+    } while (0)
+#define PT_AB_T(T_)                                                                                                                              \
+    do {                                                                                                                                          \
+        using T = T_;                                                                                                                             \
+        if (dy_dtype == PT_F32) PT_AB_DY(float); else PT_AB_DY(T);                                                                                \
+    } while (0)
+        PT_REQUIRE(dy_dtype == dtype || dy_dtype == PT_F32, "act_bias backward: the gradient must have the operands' type or fp32");
+        if (dtype == PT_BF16) PT_AB_T(__nv_bfloat16); else PT_AB_T(__half);
+        PT_LAUNCH_OK();
+    }
+    if (dbias) {
+        PT_SWITCH_SRC(dbias_dtype, T, (bias_grad_kernel<T><<<(unsigned) ceil_div(N, 32), 256, 0, st>>>(partial, parts, N, (T *) dbias)));
+        PT_LAUNCH_OK();
+    }
     return PT_OK;
 }
 

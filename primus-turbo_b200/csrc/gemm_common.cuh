@@ -61,6 +61,41 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
     return *reinterpret_cast<uint32_t *>(&h);
 }
 
+// One element, or four neighbouring ones (as one access: 8- or 16-byte aligned), of a tensor whose type is known at run time.
+__device__ __forceinline__ float load_as_f32(const void *p, int dtype, int64_t i) {
+    if (dtype == PT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]);
+    if (dtype == PT_F16) return __half2float(reinterpret_cast<const __half *>(p)[i]);
+    return reinterpret_cast<const float *>(p)[i];
+}
+__device__ __forceinline__ void store_from_f32(void *p, int dtype, int64_t i, float v) {
+    if (dtype == PT_BF16) reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+    else if (dtype == PT_F16) reinterpret_cast<__half *>(p)[i] = __float2half_rn(v);
+    else reinterpret_cast<float *>(p)[i] = v;
+}
+__device__ __forceinline__ void load4_as_f32(const void *p, int dtype, int64_t i, float (&v)[4]) {
+    if (dtype == PT_F32) {
+        const float4 f = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + i);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + i);
+        if (dtype == PT_BF16) {
+            v[0] = lo_f32<__nv_bfloat16>(w.x); v[1] = hi_f32<__nv_bfloat16>(w.x); v[2] = lo_f32<__nv_bfloat16>(w.y); v[3] = hi_f32<__nv_bfloat16>(w.y);
+        } else {
+            v[0] = lo_f32<__half>(w.x); v[1] = hi_f32<__half>(w.x); v[2] = lo_f32<__half>(w.y); v[3] = hi_f32<__half>(w.y);
+        }
+    }
+}
+__device__ __forceinline__ void store4_from_f32(void *p, int dtype, int64_t i, const float (&v)[4]) {
+    if (dtype == PT_F32) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+    else if (dtype == PT_BF16)
+        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p) + i) = make_uint2(pack2<__nv_bfloat16>(v[0], v[1]), pack2<__nv_bfloat16>(v[2], v[3]));
+    else *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p) + i) = make_uint2(pack2<__half>(v[0], v[1]), pack2<__half>(v[2], v[3]));
+}
+
+// few_rows.cu: y = act(a . b^T + bias) + residual for few rows of a
+int few_rows_linear(const void *a, const void *b, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
+                    void *z, int act, int64_t M, int64_t N, int64_t K, int *status, cudaStream_t st);
+
 inline int raster_rows(int64_t a_rows, int64_t k_bytes) {
     if (const char *e = getenv("PT_GEMM_RASTER_M")) {   // row blocks (of 128 rows) per band, for experiments
         const int v = atoi(e);

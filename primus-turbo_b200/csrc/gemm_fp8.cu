@@ -23,6 +23,7 @@
 #include <cstdlib>
 #include <mutex>
 
+#include "act_math.cuh"
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 #include "gemm_common.cuh"
@@ -35,8 +36,10 @@ constexpr int kGemmThreads = 32 * (2 + kNumEpiWarps);
 constexpr int kEpiWarp0 = 2;
 constexpr int kStagePitchMax = 128;  // staging row pitch (bytes) of the epilogue, fp32 worst case
 
-enum GemmMode { GEMM_TENSOR = 0, GEMM_ROW = 1, GEMM_MX = 3, GEMM_MXF4 = 4, GEMM_HP = 5 };  // HP: fp16 / bf16 operands, no scales
+// HP: fp16 / bf16 operands, no scales; HP_EPI: the same with bias, activation and residual in the epilogue
+enum GemmMode { GEMM_TENSOR = 0, GEMM_ROW = 1, GEMM_MX = 3, GEMM_MXF4 = 4, GEMM_HP = 5, GEMM_HP_EPI = 6 };
 constexpr bool mode_is_mx(int m) { return m == GEMM_MX || m == GEMM_MXF4; }
+constexpr bool mode_is_hp(int m) { return m == GEMM_HP || m == GEMM_HP_EPI; }
 
 struct GemmParams {
     int64_t M;             // rows of A / C (all groups)
@@ -61,6 +64,10 @@ struct GemmParams {
     int64_t sfb_line0;          // CTA-pair MX kernel: first 128-byte line of the re-tiled B scales in the scale buffer
     int a_mn, b_mn;             // tensorwise / rowwise, one group: the operand is stored [contraction, rows] (MN-major) and read in
                                 // place: 128-byte x 128-row boxes, described to the tensor core as in gemm_fp8_blockwise.cu
+    // HP_EPI: C = act(acc + bias[n]) + residual[m, n]; z (the operands' type) receives acc + bias.  Each may be null.
+    const void *bias, *residual;
+    void *z;
+    int bias_dtype, act;
 };
 
 // F4: packed e2m1 operands.  A 128-byte stage row then holds 256 elements = two 128-element scale blocks, so every
@@ -268,6 +275,84 @@ __device__ __forceinline__ void epilogue_store_block(const GemmParams &p, uint32
     }
 }
 
+// The same for HP_EPI.  The accumulators are staged as fp32 and everything element-wise happens on the way out, where a lane holds
+// four neighbouring columns of a row, the same columns in every row it writes: the bias is loaded once per 32-column chunk, the
+// residual, the pre-activation and the output are accessed in whole 32-byte sectors, and the result is rounded once.  The
+// residual's loads are issued before the accumulators are read, so that they return behind the tensor-memory load.
+template <int BLOCK_N, typename Release>
+__device__ __forceinline__ void epilogue_fused_block(const GemmParams &p, uint32_t taddr, bool have_acc, int64_t tile_row0, int64_t c_row_end, int n0,
+                                                     uint8_t *stg, int lane, int c_begin, int c_end, Release release) {
+    constexpr int kPasses = 8;   // 4 rows each
+    const int n_end = min(p.N, n0 + BLOCK_N);
+    const int sub = lane & 7, row_in_pass = lane >> 3;
+    const int z_dtype = p.a_fmt ? PT_BF16 : PT_F16;
+#pragma unroll 1
+    for (int c = c_begin; c < c_end; ++c) {
+        const int gcol = n0 + c * 32 + sub * 4;
+        const bool vec = p.vec_store_ok && gcol + 4 <= n_end;
+        float res[kPasses][4];
+        if (p.residual != nullptr && vec) {
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+                const int64_t grow = tile_row0 + i * 4 + row_in_pass;
+                if (grow < c_row_end) load4_as_f32(p.residual, p.c_dtype, grow * p.ldc + gcol, res[i]);
+            }
+        }
+        uint32_t r[32];
+        if (have_acc) {
+            tmem_ld32(taddr + c * 32, r);
+            tmem_ld_wait();
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = 0u;
+        }
+        if (have_acc && c == c_end - 1) {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) release();
+        }
+        uint8_t *my = stg + lane * 128;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4 *>(my + 16 * (i ^ (lane & 7))) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        if (p.bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (gcol + i < n_end) bias[i] = load_as_f32(p.bias, p.bias_dtype, gcol + i);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int rr = i * 4 + row_in_pass;
+            const int64_t grow = tile_row0 + rr;
+            if (grow >= c_row_end || gcol >= n_end) continue;
+            const float4 acc = *reinterpret_cast<const float4 *>(stg + rr * 128 + (sub ^ (rr & 7)) * 16);
+            float v[4] = {acc.x + bias[0], acc.y + bias[1], acc.z + bias[2], acc.w + bias[3]};
+            const int64_t o = grow * p.ldc + gcol;
+            if (vec) {
+                if (p.z != nullptr) store4_from_f32(p.z, z_dtype, o, v);
+                act_any4(p.act, v);
+                if (p.residual != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += res[i][e];
+                }
+                store4_from_f32(p.C, p.c_dtype, o, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (gcol + e >= n_end) continue;
+                    if (p.z != nullptr) store_from_f32(p.z, z_dtype, o + e, v[e]);
+                    float y = act_any(p.act, v[e]);
+                    if (p.residual != nullptr) y += load_as_f32(p.residual, p.c_dtype, o + e);
+                    store_from_f32(p.C, p.c_dtype, o + e, y);
+                }
+            }
+        }
+        __syncwarp();
+    }
+}
+
 template <int BLOCK_N, int MODE>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, GemmParams p) {
@@ -339,7 +424,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     bool ok = true;
     auto k_range = [&](int g, int &kb_begin, int &kb_count) {
         if (p.koffs) {  // offsets count elements; a stage holds 128 (fp8), 256 (packed fp4) or 64 (16-bit) of them
-            constexpr int kElemsPerStage = F4 ? 2 * BLOCK_K : (MODE == GEMM_HP ? BLOCK_K / 2 : BLOCK_K);
+            constexpr int kElemsPerStage = F4 ? 2 * BLOCK_K : (mode_is_hp(MODE) ? BLOCK_K / 2 : BLOCK_K);
             kb_begin = (int) (p.koffs[g] / kElemsPerStage);
             kb_count = (int) ((p.koffs[g + 1] - p.koffs[g]) / kElemsPerStage);
         } else {
@@ -397,7 +482,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (elect_one()) {
             constexpr uint32_t kIdescPlainShape = 0;
             (void) kIdescPlainShape;
-            const bool a_mn = !MX && MODE != GEMM_HP && p.a_mn, b_mn = !MX && MODE != GEMM_HP && p.b_mn;
+            const bool a_mn = !MX && !mode_is_hp(MODE) && p.a_mn, b_mn = !MX && !mode_is_hp(MODE) && p.b_mn;
             const uint32_t idesc = F4 ? idesc_block_scaled(1, 1, BLOCK_M, BLOCK_N)   // kind::mxf4: format code 1 = e2m1
                                    : MX ? idesc_block_scaled(p.a_fmt, p.b_fmt, BLOCK_M, BLOCK_N)
                                         : (idesc_f8(p.a_fmt, p.b_fmt, BLOCK_M, BLOCK_N) | ((uint32_t) a_mn << 15) | ((uint32_t) b_mn << 16));
@@ -443,7 +528,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                                      sfa_cur + (k >> 1) * Cfg::kSfColsHalf, sfb_cur + (k >> 1) * Cfg::kSfColsHalf, accumulate);
                         else if constexpr (MX)
                             mma_mxf8(d_tmem, a_desc + adv, b_desc + adv, idesc_sf_ids(idesc, k, k), sfa_cur, sfb_cur, accumulate);
-                        else if constexpr (MODE == GEMM_HP)
+                        else if constexpr (mode_is_hp(MODE))
                             mma_f16(d_tmem, a_desc + adv, b_desc + adv, idesc, accumulate);
                         else
                             mma_f8(d_tmem, a_desc + k * a_kstep, b_desc + k * b_kstep, idesc, accumulate);
@@ -472,8 +557,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             if (have_acc && !(ok = mbar_wait_warp(&tmem_full_bar[acc_stage], acc_phase, abort_flag))) break;
             tc_fence_after_sync();
             const uint32_t taddr = tmem_base + ((uint32_t) (q * 32) << 16) + acc_stage * BLOCK_N;
-            epilogue_store_block<BLOCK_N, MODE>(p, taddr, have_acc, tile_row0, c_row_end, n0, gi, stg, lane, 0, (BLOCK_N + 31) / 32,
-                                                [&]() { mbar_arrive(&tmem_empty_bar[acc_stage]); });
+            auto release = [&]() { mbar_arrive(&tmem_empty_bar[acc_stage]); };
+            if constexpr (MODE == GEMM_HP_EPI)
+                epilogue_fused_block<BLOCK_N>(p, taddr, have_acc, tile_row0, c_row_end, n0, stg, lane, 0, (BLOCK_N + 31) / 32, release);
+            else
+                epilogue_store_block<BLOCK_N, MODE>(p, taddr, have_acc, tile_row0, c_row_end, n0, gi, stg, lane, 0, (BLOCK_N + 31) / 32, release);
             if (have_acc && ++acc_stage == kAccStages) { acc_stage = 0; acc_phase ^= 1; }
         }
     }
@@ -759,11 +847,44 @@ int gemm_hp_host(const void *a, const void *b, int ab_dtype, void *c, int c_dtyp
     return dispatch_block_n<GEMM_HP>(0, a, a_rows_total, b, b_rows, p, mx, max_ctas, (cudaStream_t) stream);
 }
 
+// Up to this many rows the product runs on the weight-streaming kernels of few_rows.cu, from there on on the tiles above.
+static bool few_rows_better(int64_t M, int64_t N, int64_t K) { return M <= 128; }
+
+static int gemm_bias_act_host(const void *a, const void *b, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
+                              void *z, int act, int64_t M, int64_t N, int64_t K, int *status, cudaStream_t st) {
+    PT_REQUIRE(M >= 0 && N >= 0 && K >= 0, "gemm_bias_act: bad shape (M=%lld N=%lld K=%lld)", (long long) M, (long long) N, (long long) K);
+    PT_REQUIRE(ab_dtype == PT_BF16 || ab_dtype == PT_F16, "gemm_bias_act: operands must be bf16 or fp16");
+    PT_REQUIRE(c_dtype == PT_BF16 || c_dtype == PT_F16 || c_dtype == PT_F32, "gemm_bias_act: bad output dtype");
+    PT_REQUIRE(!bias || bias_dtype == PT_BF16 || bias_dtype == PT_F16 || bias_dtype == PT_F32, "gemm_bias_act: bad bias dtype");
+    PT_REQUIRE(act >= PT_ACT_SILU && act <= PT_ACT_GELU_TANH, "gemm_bias_act: bad activation %d", act);
+    if (M == 0 || N == 0) return PT_OK;
+    PT_REQUIRE(K > 0 && K % 8 == 0, "gemm_bias_act: K must be a positive multiple of 8 (got %lld)", (long long) K);
+    PT_REQUIRE(a && b && c, "gemm_bias_act: null pointer");
+    PT_REQUIRE(N < (1 << 30) && K < (1 << 29) && M < (1ll << 31), "gemm_bias_act: extent exceeds 32-bit tile coordinates");
+    if (few_rows_better(M, N, K)) return few_rows_linear(a, b, ab_dtype, bias, bias_dtype, residual, c, c_dtype, z, act, M, N, K, status, st);
+    GemmParams p{};
+    p.M = M; p.N = (int) N; p.K = (int) (2 * K); p.C = c; p.ldc = N; p.c_dtype = c_dtype;
+    p.bias = bias; p.bias_dtype = bias_dtype; p.residual = residual; p.z = z; p.act = act;
+    const int esize = c_dtype == PT_F32 ? 4 : 2;
+    p.vec_store_ok = N % 4 == 0 && aligned(c, 4 * esize) && aligned(residual, 4 * esize) && aligned(z, 8);
+    p.a_fmt = p.b_fmt = ab_dtype == PT_BF16 ? 1 : 0;
+    p.G = 1; p.b_group_rows = N; p.status = status;
+    p.raster_m = raster_rows(M, 2 * K);
+    return dispatch_block_n<GEMM_HP_EPI>(0, a, M, b, N, p, MxScales{nullptr, nullptr, 0, nullptr, 0}, 0, st);
+}
+
 }  // namespace ptb
 
 using namespace ptb;
 
 extern "C" {
+
+int pt_gemm_bias_act_few_rows(int64_t M, int64_t N, int64_t K) { return few_rows_better(M, N, K) ? 1 : 0; }
+
+int pt_gemm_bias_act(const void *a, const void *b, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype, void *z,
+                     int act, int64_t M, int64_t N, int64_t K, int *status, void *stream) {
+    return gemm_bias_act_host(a, b, ab_dtype, bias, bias_dtype, residual, c, c_dtype, z, act, M, N, K, status, (cudaStream_t) stream);
+}
 
 int pt_gemm(const void *a, const void *b, int ab_dtype, void *c, int c_dtype, int64_t M, int64_t N, int64_t K, float beta, int *status,
             void *stream) {

@@ -130,7 +130,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BLOCK_N, mo
     int gi, m_blk, n_blk;
     auto k_range = [&](int g, int &kb_begin, int &kb_count) {
         if (p.koffs) {  // offsets count elements; a stage holds 128 (fp8), 256 (packed fp4) or 64 (16-bit) of them
-            constexpr int kElemsPerStage = F4 ? 2 * BLOCK_K : (MODE == GEMM_HP ? BLOCK_K / 2 : BLOCK_K);
+            constexpr int kElemsPerStage = F4 ? 2 * BLOCK_K : (mode_is_hp(MODE) ? BLOCK_K / 2 : BLOCK_K);
             kb_begin = (int) (p.koffs[g] / kElemsPerStage);
             kb_count = (int) ((p.koffs[g + 1] - p.koffs[g]) / kElemsPerStage);
         } else {
@@ -185,7 +185,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BLOCK_N, mo
             const uint32_t idesc = F4 ? idesc_block_scaled(1, 1, kTileM, BLOCK_N)  // kind::mxf4: format code 1 = e2m1
                                    : MX ? idesc_block_scaled(p.a_fmt, p.b_fmt, kTileM, BLOCK_N)
                                         : (idesc_f8(p.a_fmt, p.b_fmt, kTileM, BLOCK_N) | ((uint32_t) (p.a_mn != 0) << 15) | ((uint32_t) (p.b_mn != 0) << 16));
-            const bool a_mn = !MX && MODE != GEMM_HP && p.a_mn, b_mn = !MX && MODE != GEMM_HP && p.b_mn;
+            const bool a_mn = !MX && !mode_is_hp(MODE) && p.a_mn, b_mn = !MX && !mode_is_hp(MODE) && p.b_mn;
             const uint64_t a_kstep = a_mn ? (uint64_t) ((UMMA_K * 128) >> 4) : (uint64_t) (UMMA_K >> 4);
             const uint64_t b_kstep = b_mn ? (uint64_t) ((UMMA_K * 128) >> 4) : (uint64_t) (UMMA_K >> 4);
             uint32_t stage = 0, phase = 0, acc_stage = 0, acc_phase = 0, sf_buf = 0;
@@ -223,7 +223,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BLOCK_N, mo
                             mma_mxf4_pair(d_tmem, a_desc + adv, b_desc + adv, idesc_sf_ids(idesc, (k & 1) * 2, (k & 1) * 2),
                                           sfa_cur + (k >> 1) * Cfg::kSfColsHalf, sfb_cur + (k >> 1) * Cfg::kSfColsHalf, accumulate);
                         else if constexpr (MX) mma_mxf8_pair(d_tmem, a_desc + adv, b_desc + adv, idesc_sf_ids(idesc, k, k), sfa_cur, sfb_cur, accumulate);
-                        else if constexpr (MODE == GEMM_HP) mma_f16_pair(d_tmem, a_desc + adv, b_desc + adv, idesc, accumulate);
+                        else if constexpr (mode_is_hp(MODE)) mma_f16_pair(d_tmem, a_desc + adv, b_desc + adv, idesc, accumulate);
                         else mma_f8_pair(d_tmem, a_desc + k * a_kstep, b_desc + k * b_kstep, idesc, accumulate);
                     }
                     tc_commit_pair(&empty_bar[stage], 3);  // frees the ring slot in both CTAs
@@ -255,8 +255,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BLOCK_N, mo
             tc_fence_after_sync();
             const uint32_t taddr = tmem_base + ((uint32_t) (q * 32) << 16) + acc_stage * BLOCK_N;
             const uint32_t release_addr = map_to_rank(&tmem_empty_bar[acc_stage], 0);
-            epilogue_store_block<BLOCK_N, MODE>(p, taddr, have_acc, tile_row0, c_row_end, n0, gi, stg, lane, c_begin, c_end,
-                                                [&]() { mbar_arrive_cluster(release_addr); });
+            auto release = [&]() { mbar_arrive_cluster(release_addr); };
+            if constexpr (MODE == GEMM_HP_EPI)
+                epilogue_fused_block<BLOCK_N>(p, taddr, have_acc, tile_row0, c_row_end, n0, stg, lane, c_begin, c_end, release);
+            else
+                epilogue_store_block<BLOCK_N, MODE>(p, taddr, have_acc, tile_row0, c_row_end, n0, gi, stg, lane, c_begin, c_end, release);
             if (have_acc && ++acc_stage == kAccStages) { acc_stage = 0; acc_phase ^= 1; }
         }
     }

@@ -324,6 +324,25 @@ __device__ __forceinline__ void tma_load_2d_pair_hint(void *smem_dst, const CUte
         ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster_addr), "r"(c0), "r"(c1), "l"(policy)
         : "memory");
 }
+// Four rows r0 .. r3 of a 2-D tensor (box one row high), 128 bytes each at column c0, as consecutive rows of the swizzled tile.
+__device__ __forceinline__ void tma_gather4(void *smem_dst, const CUtensorMap *m, uint64_t *bar, int c0, int r0, int r1, int r2, int r3,
+                                            uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "l"(policy)
+        : "memory");
+}
+// shared::cluster address of a shared::cta address in the CTA of cluster rank `rank`
+__device__ __forceinline__ uint32_t map_addr_to_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+// two floats from shared memory: of another CTA of the cluster (address from map_addr_to_rank), or this one's own
+__device__ __forceinline__ void ld_cluster_f32x2(uint32_t addr, bool remote, float &x, float &y) {
+    if (remote) asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x), "=f"(y) : "r"(addr) : "memory");
+    else asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(x), "=f"(y) : "r"(addr) : "memory");
+}
 // executed by the same warp of both CTAs of the pair
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t *smem_result, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)), "r"(ncols) : "memory");

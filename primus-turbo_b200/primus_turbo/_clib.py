@@ -68,6 +68,15 @@ SIGNATURES = {
     "pt_transpose_batched": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
     "pt_grouped_transpose_pad": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p]),
     "pt_zero_rows_from": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
+    "pt_moe_few_tokens_scratch_bytes": (c_size_t, [c_int64, c_int, c_int64]),
+    "pt_moe_few_tokens": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int64, c_int64,
+                                  c_int, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p]),
+    "pt_gemm_bias_act_few_rows": (c_int, [c_int64, c_int64, c_int64]),
+    "pt_gemm_bias_act": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64,
+                                 c_int64, c_void_p, c_void_p]),
+    "pt_act_bias_bwd_parts": (c_int, [c_int64, c_int64]),
+    "pt_act_bias_bwd": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                c_void_p]),
     "pt_qk_norm_rope_fwd": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64,
                                     c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_void_p, c_void_p,
                                     c_void_p, c_void_p]),

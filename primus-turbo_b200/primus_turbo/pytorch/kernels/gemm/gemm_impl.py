@@ -5,6 +5,8 @@ Same call shape as primus_turbo::gemm_impl / gemm_accum_impl of the reference
 C = A . B^T with both operands K-major; the other (trans_a, trans_b, trans_c) combinations swap the operands
 (trans_c) or transpose the 16-bit elements first.
 """
+from typing import Optional, Tuple
+
 import torch
 
 from .. import _native as nv
@@ -60,3 +62,62 @@ def gemm_accum_impl(a: torch.Tensor, trans_a: bool, b: torch.Tensor, trans_b: bo
                     out: torch.Tensor, default_backend: int = 0) -> torch.Tensor:
     """out += op(a) . op(b) in place (the fused main_grad accumulation of the wgrad)."""
     return _gemm(a, trans_a, b, trans_b, out.dtype, trans_c, out=out)
+
+
+EPILOGUE_ACTS = {"silu": 0, "gelu": 1, None: 2, "relu": 3, "gelu_tanh": 4}
+
+
+def gemm_bias_act_impl(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Optional[torch.Tensor], act: Optional[str],
+                       residual: Optional[torch.Tensor], out_dtype: torch.dtype, want_z: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(act(a . op(b) + bias) + residual, the pre-activation in a's type or None) in one kernel."""
+    nv.require_cuda(a, b, bias, residual)
+    a_km = _k_major16(a, False)          # [M, K]
+    b_km = _k_major16(b, not trans_b)    # [N, K]
+    if a_km.data_ptr() % 16:             # a view into a larger buffer; TMA reads from 16-byte boundaries
+        a_km = a_km.clone()
+    (M, K), N = a_km.shape, b_km.shape[0]
+    out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    z = torch.empty((M, N), dtype=a.dtype, device=a.device) if want_z else None
+    bias = None if bias is None else bias.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    lib = nv.lib()
+    few = lib.pt_gemm_bias_act_few_rows(M, N, K)
+    if few:
+        nv.poll_host_status(a.device)
+        st = nv.host_status(a.device)[2]
+    else:
+        st = nv.ptr(nv.status_word(a.device))
+    with nv.on_device(a.device):
+        nv.check(lib.pt_gemm_bias_act(nv.ptr(a_km), nv.ptr(b_km), nv.src_code(a.dtype), nv.ptr(bias), 0 if bias is None else nv.src_code(bias.dtype),
+                                      nv.ptr(residual), nv.ptr(out), nv.src_code(out_dtype), nv.ptr(z), EPILOGUE_ACTS[act], M, N, K, st,
+                                      nv.stream(a.device)), "gemm_bias_act")
+    if not few:
+        nv.poll_status(a.device)
+    return out, z
+
+
+def act_bias_bwd_impl(grad_out: torch.Tensor, z: Optional[torch.Tensor], act: Optional[str], dtype: torch.dtype,
+                      bias_dtype: Optional[torch.dtype], want_dz: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(grad_out * act'(z) in the operands' type, its column sums in bias_dtype or None) in one pass.  Without an activation the
+    first is grad_out itself where the types agree."""
+    nv.require_cuda(grad_out, z)
+    grad_out = grad_out.contiguous()
+    if grad_out.dtype not in (dtype, torch.float32):
+        grad_out = grad_out.to(torch.float32)
+    M, N = grad_out.shape
+    same = act is None and grad_out.dtype == dtype
+    dz = torch.empty((M, N), dtype=dtype, device=grad_out.device) if want_dz and not same else None
+    if dz is None and bias_dtype is None:
+        return (grad_out if same else None), None
+    lib = nv.lib()
+    with nv.on_device(grad_out.device):
+        dbias = partial = None
+        parts = 0
+        if bias_dtype is not None:
+            parts = lib.pt_act_bias_bwd_parts(M, N)
+            dbias = torch.empty((N,), dtype=bias_dtype, device=grad_out.device)
+            partial = torch.empty((parts, N), dtype=torch.float32, device=grad_out.device)
+        nv.check(lib.pt_act_bias_bwd(nv.ptr(grad_out), nv.src_code(grad_out.dtype), nv.ptr(z), nv.src_code(dtype), EPILOGUE_ACTS[act], M, N,
+                                     nv.ptr(dz), nv.ptr(dbias), 0 if dbias is None else nv.src_code(bias_dtype), nv.ptr(partial), parts,
+                                     nv.stream(grad_out.device)), "act_bias_bwd")
+    return (grad_out if same else dz), dbias

@@ -1,15 +1,16 @@
 """gemm: BF16 / FP16 GEMM with autograd, on the tcgen05 kernels of the FP8 path run with 16-bit operands.
 
-Operator surface and data flow follow primus_turbo/pytorch/ops/gemm.py of the reference (GemmFunction, gemm).
+Operator surface and data flow follow primus_turbo/pytorch/ops/gemm.py of the reference (GemmFunction, gemm).  gemm_bias_act, which
+the reference lacks, adds bias, activation and residual in the product's epilogue and serves single tokens as well as prompts.
 """
 from typing import Optional, Union
 
 import torch
 
-from ..kernels.gemm.gemm_impl import gemm_accum_impl, gemm_impl
+from ..kernels.gemm.gemm_impl import EPILOGUE_ACTS, act_bias_bwd_impl, gemm_accum_impl, gemm_bias_act_impl, gemm_impl
 from .utils import _get_dummy_wgrad, _setup_fused_grad_accum
 
-__all__ = ["gemm"]
+__all__ = ["gemm", "gemm_bias_act"]
 
 
 class GemmFunction(torch.autograd.Function):
@@ -43,3 +44,59 @@ def gemm(a: torch.Tensor, b: torch.Tensor, trans_a: bool = False, trans_b: bool 
     if out_dtype is None:
         out_dtype = torch.result_type(a, b)
     return GemmFunction.apply(a, b, trans_a, trans_b, out_dtype, fuse_bgrad_accum_pattern)
+
+
+class GemmBiasActFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, b, bias, residual, trans_b, act, out_dtype, fuse_bgrad_accum_pattern):
+        fuse, main_grad = _setup_fused_grad_accum(b, fuse_bgrad_accum_pattern)
+        out, z = gemm_bias_act_impl(a, b, trans_b, bias, act, residual, out_dtype, act is not None and any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(a, b, z)
+        ctx.trans_b, ctx.act, ctx.fuse, ctx.main_grad = trans_b, act, fuse, main_grad
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return out
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        a, b, z = ctx.saved_tensors
+        need_a, need_b, need_bias, need_residual = ctx.needs_input_grad[:4]
+        grad_a = grad_b = grad_bias = None
+        if need_a or need_b or need_bias:
+            dz, grad_bias = act_bias_bwd_impl(grad_out, z, ctx.act, a.dtype, ctx.bias_dtype if need_bias else None, need_a or need_b)
+        # an empty contraction (no columns for grad_a, no rows for grad_b) is a sum of nothing
+        if need_a:                                                                         # dz . op(b)^T
+            grad_a = gemm_impl(dz, False, b, not ctx.trans_b, a.dtype, False) if dz.shape[1] else torch.zeros_like(a)
+        if need_b and ctx.fuse:
+            if a.shape[0]:
+                gemm_accum_impl(a, True, dz, False, b.dtype, ctx.trans_b, out=ctx.main_grad)
+            grad_b = _get_dummy_wgrad(b.shape, b.dtype, device=b.device)
+        elif need_b:                                                                       # a^T . dz
+            grad_b = gemm_impl(a, True, dz, False, b.dtype, ctx.trans_b) if a.shape[0] else torch.zeros_like(b)
+        return grad_a, grad_b, grad_bias, (grad_out if need_residual else None), None, None, None, None
+
+
+def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+                  residual: Optional[torch.Tensor] = None, trans_b: bool = False, out_dtype: Optional[torch.dtype] = None,
+                  fuse_bgrad_accum_pattern: Union[None, str] = None) -> torch.Tensor:
+    """out = act(a . op(b) + bias) + residual for 2-D bf16 / fp16 tensors in one kernel; fp32 accumulate, rounded once.
+
+    activation: None, "relu", "silu", "gelu" (erf form) or "gelu_tanh".  bias [N] in a's dtype or fp32; residual [M, N] in out_dtype
+    (a's dtype by default).  Few rows (a decoding batch) run on a kernel that streams the weight over all SMs.  Differentiable in
+    a, b, bias and residual; the pre-activation is kept in a's dtype for the backward when an activation needs it."""
+    assert a.dim() == 2 and b.dim() == 2, "Only 2D GEMM is supported"
+    assert a.dtype == b.dtype and a.dtype in (torch.bfloat16, torch.float16), "a and b must both be bf16 or fp16"
+    assert activation in EPILOGUE_ACTS, f"Unsupported activation: {activation}. Supported: {list(EPILOGUE_ACTS)}"
+    M, N = a.shape[0], b.shape[0] if trans_b else b.shape[1]
+    assert a.shape[1] == b.shape[1 if trans_b else 0], f"contraction mismatch: {tuple(a.shape)} vs {tuple(b.shape)} (trans_b={trans_b})"
+    assert a.shape[1] > 0, "gemm_bias_act: the contraction must not be empty"
+    out_dtype = a.dtype if out_dtype is None else out_dtype
+    assert out_dtype in (torch.bfloat16, torch.float16, torch.float32), f"gemm_bias_act: unsupported out_dtype {out_dtype}"
+    if bias is not None:
+        assert tuple(bias.shape) == (N,) and bias.dtype in (a.dtype, torch.float32), f"gemm_bias_act: bias must be [{N}] in a's dtype or float32"
+    if residual is not None:
+        assert tuple(residual.shape) == (M, N) and residual.dtype == out_dtype, f"gemm_bias_act: residual must be [{M}, {N}] in {out_dtype}"
+    tensors = [t for t in (a, b, bias, residual) if t is not None]
+    assert len({t.device for t in tensors}) == 1, "gemm_bias_act: all tensors must be on one device"
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return GemmBiasActFunction.apply(a, b, bias, residual, trans_b, activation, out_dtype, fuse_bgrad_accum_pattern)
+    return gemm_bias_act_impl(a, b, trans_b, bias, activation, residual, out_dtype, False)[0]

@@ -261,6 +261,8 @@ int pt_grouped_gemm_fp8_variable_k(const void *a, const void *a_scale, int a_fmt
 
 /* fp16 / bf16 GEMMs on the same tcgen05 kernels (kind::f16, fp32 accumulate, no scales): C [M, N] = A [M, K] . B [N, K]^T,
  * both operands K-major with K a multiple of 8; ab_dtype PT_BF16 or PT_F16; c_dtype any PT_* output type; beta 0 or 1.
+ * pt_gemm_mn: either operand may be stored contraction-major ([K, M] / [K, N], flag a_mn / b_mn; its row count a multiple of 8) and
+ * is read in place, the same sums as after a transposition; K a multiple of 8 unless both are.
  * Grouped: A [a_rows, K] split by group_offs int64 [G+1] (device), B [G, N, K], rows of C past group_offs[G] are not
  * written.  Variable-K: A [M, K_total], B [N, K_total], C [G, M, N], k_offs int64 [G+1] multiples of 64 elements.
  * Replace primus_turbo::gemm_impl / gemm_accum_impl (primus_turbo/pytorch/kernels/gemm/gemm_impl.py) and
@@ -268,6 +270,8 @@ int pt_grouped_gemm_fp8_variable_k(const void *a, const void *a_scale, int a_fmt
  * (primus_turbo/pytorch/kernels/grouped_gemm/grouped_gemm_impl.py). */
 int pt_gemm(const void *a, const void *b, int ab_dtype, void *c, int c_dtype, int64_t M, int64_t N, int64_t K, float beta, int *status,
             void *stream);
+int pt_gemm_mn(const void *a, int a_mn, const void *b, int b_mn, int ab_dtype, void *c, int c_dtype, int64_t M, int64_t N, int64_t K, float beta,
+               int *status, void *stream);
 int pt_grouped_gemm(const void *a, const void *b, int ab_dtype, void *c, int c_dtype, int64_t a_rows, int64_t N, int64_t K,
                     const int64_t *group_offs, int G, float beta, int max_ctas, int *status, void *stream);
 int pt_grouped_gemm_variable_k(const void *a, const void *b, int ab_dtype, void *c, int c_dtype, int64_t M, int64_t N, int64_t K_total,
@@ -470,14 +474,14 @@ int pt_moe_few_tokens(const void *x, const void *gate_up, const void *down, int 
                       int E, int top_k, int64_t H, int64_t I, int act, void *scratch, size_t scratch_bytes, void *out, int *status, void *stream);
 
 /* ---- matrix product with bias, activation and residual in its epilogue (csrc/gemm_fp8.cu, csrc/few_rows.cu) ----------
- * c [M, N] = act(a . b^T + bias) + residual, fp32 accumulate, rounded once: a [M, K], b [N, K] (PT_BF16 / PT_F16, K a multiple of 8,
- * 16-byte aligned bases), bias [N] of any of the three types or null, residual [M, N] of c's type or null.  act 0 = SiLU, 1 = GELU
+ * c [M, N] = act(a . b^T + bias) + residual, fp32 accumulate, rounded once: a [M, K], b [N, K], or [K, N] with b_mn (N a multiple of
+ * 8 then); PT_BF16 / PT_F16, K a multiple of 8, 16-byte aligned bases; bias [N] of any of the three types or null, residual [M, N] of c's type or null.  act 0 = SiLU, 1 = GELU
  * (erf), 2 = none, 3 = ReLU, 4 = GELU (tanh).  z: null, or [M, N] in the operands' type, receives a . b^T + bias (the backward's
  * input).  residual may be c itself.  status as in pt_gemm; calls for which pt_gemm_bias_act_few_rows is 1 may also be given a
  * mapped host word.  (The reference runs gemm and leaves bias, activation and residual to separate torch kernels:
  * primus_turbo/pytorch/ops/gemm.py.) */
 int pt_gemm_bias_act_few_rows(int64_t M, int64_t N, int64_t K);
-int pt_gemm_bias_act(const void *a, const void *b, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype, void *z,
+int pt_gemm_bias_act(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype, void *z,
                      int act, int64_t M, int64_t N, int64_t K, int *status, void *stream);
 /* Its element-wise backward: dz [M, N] = dy * act'(z) in the operands' type `dtype` (null: not written), dbias [N] = column sums of
  * the unrounded dz (null: none).  dy of type `dtype` or fp32; z may be null with act 2.  partial fp32 [parts, N] with

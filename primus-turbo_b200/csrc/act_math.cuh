@@ -40,7 +40,7 @@ template <int ACT> __device__ __forceinline__ float act_grad(float a) {
 }
 template <int ACT> __device__ __forceinline__ float glu_value(float a, float b, float p) { return act_value<ACT>(a) * b * p; }
 
-// The activation chosen at run time (uniform over the launch), and the same for four values under one branch.
+// The activation chosen at run time (uniform over the launch), and the same for a lane's values under one branch.
 __device__ __forceinline__ float act_any(int act, float v) {
     switch (act) {
     case PT_ACT_SILU: return act_value<PT_ACT_SILU>(v);
@@ -50,10 +50,12 @@ __device__ __forceinline__ float act_any(int act, float v) {
     default: return v;
     }
 }
-__device__ __forceinline__ void act_any4(int act, float (&v)[4]) {
+template <int ROWS> __device__ __forceinline__ void act_any_all(int act, float (&v)[ROWS][4]) {
     auto all = [&](auto f) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = f(v[i]);
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[r][i] = f(v[r][i]);
     };
     switch (act) {
     case PT_ACT_SILU: all([](float x) { return act_value<PT_ACT_SILU>(x); }); break;

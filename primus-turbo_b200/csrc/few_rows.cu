@@ -41,6 +41,7 @@ constexpr int kFrFeat = 128;              // features (weight rows) of a CTA
 constexpr int kFrABytes = kFrFeat * 128;  // a weight block: 128 rows of 64 16-bit elements
 constexpr int kFrMaxSlots = 2048;         // tokens x experts per token
 constexpr int kFrMaxTopK = 32;
+constexpr int kFrMaxSplit = 8;            // CTAs of a cluster
 
 enum FewRowsKind { FR_LINEAR = 0, FR_GATE_UP = 1, FR_DOWN = 2 };
 
@@ -53,6 +54,7 @@ struct FewRowsArgs {
     int out_dtype;
     int act;
     // LINEAR
+    int w_mn;                // the weight is stored [k, n]: two boxes of 64 features x 64 contraction rows, read in place
     const void *bias, *residual;
     int bias_dtype;
     void *z;                 // pre-activation in the operands' type, or null
@@ -109,6 +111,10 @@ __global__ void __launch_bounds__(kFrThreads, 2)
         prefetch_tmap(&tmap_w);
         prefetch_tmap(&tmap_x);
     }
+    if (warp == 1) {
+        tmem_alloc(&s_tmem, Cfg::kTmemCols);
+        tmem_relinquish();
+    }
     if (KIND != FR_DOWN) {   // DOWN waits later: what it reads up to there is not written by the kernel before it
         grid_dep_wait();
         grid_dep_launch();
@@ -138,7 +144,10 @@ __global__ void __launch_bounds__(kFrThreads, 2)
         const int excl = incl - __popc(bits);
         if constexpr (KIND == FR_GATE_UP) {
             const int want = (int) blockIdx.y;
-            if (want >= n_active) return;   // the same for every CTA of the cluster
+            if (want >= n_active) {   // the same for every CTA of the cluster
+                if (warp == 1) tmem_dealloc(s_tmem, Cfg::kTmemCols);
+                return;
+            }
             const bool here = want >= excl && want < incl;
             uint32_t b = bits;
             for (int i = here ? want - excl : 0; i > 0; --i) b &= b - 1;
@@ -174,10 +183,6 @@ __global__ void __launch_bounds__(kFrThreads, 2)
             }
         }
     }
-    if (warp == 1) {
-        tmem_alloc(&s_tmem, Cfg::kTmemCols);
-        tmem_relinquish();
-    }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
@@ -205,7 +210,12 @@ __global__ void __launch_bounds__(kFrThreads, 2)
                     uint8_t *A = ring + stage * Cfg::kStageBytes, *B = A + kFrABytes;
                     mbar_arrive_expect_tx(&full_bar[stage], bytes);
                     if constexpr (KIND == FR_LINEAR) {
-                        tma_load_2d_hint(A, &tmap_w, &full_bar[stage], l * 128, tile * kFrFeat, stream_pol);
+                        if (a.w_mn) {
+                            tma_load_2d_hint(A, &tmap_w, &full_bar[stage], tile * kFrFeat * 2, l * 64, stream_pol);
+                            tma_load_2d_hint(A + kFrABytes / 2, &tmap_w, &full_bar[stage], tile * kFrFeat * 2 + 128, l * 64, stream_pol);
+                        } else {
+                            tma_load_2d_hint(A, &tmap_w, &full_bar[stage], l * 128, tile * kFrFeat, stream_pol);
+                        }
                         tma_load_2d_hint(B, &tmap_x, &full_bar[stage], l * 128, (int) blockIdx.y * TOK, keep_pol);
                     } else {
                         const int row = expert * 2 * a.n + tile * 64;
@@ -281,7 +291,9 @@ __global__ void __launch_bounds__(kFrThreads, 2)
     } else if (warp == 1) {
         // ================================================================ MMA issuer
         if (elect_one()) {
-            const uint32_t idesc0 = idesc_f8(a.fmt, a.fmt, kFrFeat, 0);
+            const bool w_mn = KIND == FR_LINEAR && a.w_mn;
+            const uint32_t idesc0 = idesc_f8(a.fmt, a.fmt, kFrFeat, 0) | ((uint32_t) w_mn << 15);
+            const uint64_t w_step = w_mn ? (16 * 128) >> 4 : 32 >> 4;   // 16 contraction rows, or 32 bytes along a row
             uint32_t touched = 0;   // 16-token blocks that hold sums
             const uint32_t all = (1u << ((cnt + 15) / 16)) - 1;
             uint32_t stage = 0, phase = 0;
@@ -289,7 +301,7 @@ __global__ void __launch_bounds__(kFrThreads, 2)
                 if (!(ok = mbar_wait(&full_bar[stage], phase, abort_flag))) break;
                 tc_fence_after_sync();
                 const uint32_t A = smem_u32(ring + stage * Cfg::kStageBytes);
-                const uint64_t a_desc = smem_desc_sw128(A);
+                const uint64_t a_desc = w_mn ? smem_desc_sw128_mn(A, kFrABytes / 2) : smem_desc_sw128(A);
                 uint32_t m = KIND == FR_DOWN ? s_mask[stage] : all;
                 const uint32_t used = m;
                 while (m != 0) {   // runs of blocks that all hold sums, or none of which does
@@ -302,7 +314,7 @@ __global__ void __launch_bounds__(kFrThreads, 2)
                     const uint32_t acc0 = touched >> b0 & 1;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16(tmem + 16 * b0, a_desc + 2 * k, b_desc + 2 * k, idesc, acc0 | (uint32_t) (k > 0));
+                        mma_f16(tmem + 16 * b0, a_desc + k * w_step, b_desc + 2 * k, idesc, acc0 | (uint32_t) (k > 0));
                     m &= ~(((1u << len) - 1) << b0);
                 }
                 touched |= used;
@@ -361,22 +373,29 @@ __global__ void __launch_bounds__(kFrThreads, 2)
     }
     const uint32_t part_addr = smem_u32(part);
     for (int t = rank + a.split * warp; t < cnt; t += a.split * (kFrThreads / 32)) {
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint32_t at = part_addr + (uint32_t) t * (kFrFeat * 4);
+        float vv[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+        float(&v)[4] = vv[0];
         // GATE_UP: features 2 lane, 2 lane + 1 of the gate half and of the up half
-        for (int s = 0; s < a.split; ++s) {
-            float w[4];
-            if constexpr (KIND == FR_GATE_UP) {
-                const uint32_t src = a.split > 1 ? map_addr_to_rank(at + lane * 8, s) : at + lane * 8;
-                ld_cluster_f32x2(src, a.split > 1, w[0], w[1]);
-                ld_cluster_f32x2(src + 256, a.split > 1, w[2], w[3]);
-            } else {
-                const uint32_t src = a.split > 1 ? map_addr_to_rank(at + lane * 16, s) : at + lane * 16;
-                ld_cluster_f32x2(src, a.split > 1, w[0], w[1]);
-                ld_cluster_f32x2(src + 8, a.split > 1, w[2], w[3]);
+        constexpr uint32_t kSecond = KIND == FR_GATE_UP ? 256 : 8;
+        const uint32_t at = part_addr + (uint32_t) t * (kFrFeat * 4) + lane * (KIND == FR_GATE_UP ? 8 : 16);
+        if (a.split == 1) {
+            ld_cluster_f32x2(at, false, v[0], v[1]);
+            ld_cluster_f32x2(at + kSecond, false, v[2], v[3]);
+        } else {
+            float w[kFrMaxSplit][4];   // all loads on their way before the first addition: one remote round trip, not one per CTA
+#pragma unroll
+            for (int s = 0; s < kFrMaxSplit; ++s) {
+                if (s >= a.split) continue;
+                const uint32_t src = map_addr_to_rank(at, s);
+                ld_cluster_f32x2(src, true, w[s][0], w[s][1]);
+                ld_cluster_f32x2(src + kSecond, true, w[s][2], w[s][3]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += w[i];
+            for (int s = 0; s < kFrMaxSplit; ++s)
+                if (s < a.split) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] += w[s][i];
+                }
         }
         if constexpr (KIND == FR_GATE_UP) {
             const int f = tile * 64 + 2 * lane;
@@ -399,7 +418,7 @@ __global__ void __launch_bounds__(kFrThreads, 2)
                         for (int i = 0; i < 4; ++i) v[i] += x[i];
                     }
                     if (a.z != nullptr) store4_from_f32(a.z, zt, o, v);
-                    act_any4(a.act, v);
+                    act_any_all<1>(a.act, vv);
                     if (a.residual != nullptr) {
                         load4_as_f32(a.residual, a.out_dtype, o, x);
 #pragma unroll
@@ -460,7 +479,7 @@ static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRows
 // blocks.
 static int fr_split(int64_t tiles, int64_t chunks) {
     int s = 1;
-    while (s < 8 && tiles * s * 2 <= 2 * (int64_t) sm_count() && chunks / (s * 2) >= 4) s *= 2;
+    while (s < kFrMaxSplit && tiles * s * 2 <= 2 * (int64_t) sm_count() && chunks / (s * 2) >= 4) s *= 2;
     return s;
 }
 
@@ -476,15 +495,15 @@ static int fr_dispatch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRo
 static int fr_tokens(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 // y = act(a . b^T + bias) + residual for few rows of a
-int few_rows_linear(const void *a, const void *b, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
+int few_rows_linear(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
                     void *z, int act, int64_t M, int64_t N, int64_t K, int *status, cudaStream_t st) {
     const int tok = fr_tokens(M);
     CUtensorMap tw, tx;
     int rc;
-    if ((rc = make_tmap_bytes(&tw, b, N, 2 * K, 2 * K, kFrFeat)) != PT_OK) return rc;
+    if ((rc = b_mn ? make_tmap_bytes(&tw, b, K, 2 * N, 2 * N, 64) : make_tmap_bytes(&tw, b, N, 2 * K, 2 * K, kFrFeat)) != PT_OK) return rc;
     if ((rc = make_tmap_bytes(&tx, a, M, 2 * K, 2 * K, tok)) != PT_OK) return rc;
     FewRowsArgs r{};
-    r.rows = (int) M; r.n = (int) N; r.k = (int) K; r.fmt = ab_dtype == PT_BF16 ? 1 : 0;
+    r.w_mn = b_mn; r.rows = (int) M; r.n = (int) N; r.k = (int) K; r.fmt = ab_dtype == PT_BF16 ? 1 : 0;
     r.out = c; r.out_dtype = c_dtype; r.act = act; r.bias = bias; r.bias_dtype = bias_dtype; r.residual = residual; r.z = z; r.status = status;
     const int esize = c_dtype == PT_F32 ? 4 : 2;
     r.vec_ok = N % 4 == 0 && aligned(c, 4 * esize) && aligned(residual, 4 * esize) && aligned(z, 8) && aligned(bias, bias_dtype == PT_F32 ? 16 : 8);

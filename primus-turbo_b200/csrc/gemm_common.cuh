@@ -72,18 +72,25 @@ __device__ __forceinline__ void store_from_f32(void *p, int dtype, int64_t i, fl
     else if (dtype == PT_F16) reinterpret_cast<__half *>(p)[i] = __float2half_rn(v);
     else reinterpret_cast<float *>(p)[i] = v;
 }
-__device__ __forceinline__ void load4_as_f32(const void *p, int dtype, int64_t i, float (&v)[4]) {
+// four elements held as they lie in memory (16-bit types: .x and .y)
+__device__ __forceinline__ void raw4_as_f32(const uint4 &w, int dtype, float (&v)[4]) {
     if (dtype == PT_F32) {
-        const float4 f = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + i);
-        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+    } else if (dtype == PT_BF16) {
+        v[0] = lo_f32<__nv_bfloat16>(w.x); v[1] = hi_f32<__nv_bfloat16>(w.x); v[2] = lo_f32<__nv_bfloat16>(w.y); v[3] = hi_f32<__nv_bfloat16>(w.y);
     } else {
-        const uint2 w = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + i);
-        if (dtype == PT_BF16) {
-            v[0] = lo_f32<__nv_bfloat16>(w.x); v[1] = hi_f32<__nv_bfloat16>(w.x); v[2] = lo_f32<__nv_bfloat16>(w.y); v[3] = hi_f32<__nv_bfloat16>(w.y);
-        } else {
-            v[0] = lo_f32<__half>(w.x); v[1] = hi_f32<__half>(w.x); v[2] = lo_f32<__half>(w.y); v[3] = hi_f32<__half>(w.y);
-        }
+        v[0] = lo_f32<__half>(w.x); v[1] = hi_f32<__half>(w.x); v[2] = lo_f32<__half>(w.y); v[3] = hi_f32<__half>(w.y);
     }
+}
+__device__ __forceinline__ void load4_as_f32(const void *p, int dtype, int64_t i, float (&v)[4]) {
+    uint4 w = {};
+    if (dtype == PT_F32) {
+        w = *reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(p) + i);
+    } else {
+        const uint2 h = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + i);
+        w.x = h.x; w.y = h.y;
+    }
+    raw4_as_f32(w, dtype, v);
 }
 __device__ __forceinline__ void store4_from_f32(void *p, int dtype, int64_t i, const float (&v)[4]) {
     if (dtype == PT_F32) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
@@ -93,7 +100,7 @@ __device__ __forceinline__ void store4_from_f32(void *p, int dtype, int64_t i, c
 }
 
 // few_rows.cu: y = act(a . b^T + bias) + residual for few rows of a
-int few_rows_linear(const void *a, const void *b, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
+int few_rows_linear(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
                     void *z, int act, int64_t M, int64_t N, int64_t K, int *status, cudaStream_t st);
 
 inline int raster_rows(int64_t a_rows, int64_t k_bytes) {

@@ -62,12 +62,22 @@ struct GemmParams {
     int *status;                // device int: set to a PT_ERR_* code on a bounded-wait expiry
     int raster_m;               // row blocks per raster band
     int64_t sfb_line0;          // CTA-pair MX kernel: first 128-byte line of the re-tiled B scales in the scale buffer
-    int a_mn, b_mn;             // tensorwise / rowwise, one group: the operand is stored [contraction, rows] (MN-major) and read in
-                                // place: 128-byte x 128-row boxes, described to the tensor core as in gemm_fp8_blockwise.cu
+    int a_mn, b_mn;             // one group, no block scales: the operand is stored [contraction, rows] (MN-major) and read in place
+                                // (MnBox), described to the tensor core as in gemm_fp8_blockwise.cu
     // HP_EPI: C = act(acc + bias[n]) + residual[m, n]; z (the operands' type) receives acc + bias.  Each may be null.
     const void *bias, *residual;
     void *z;
     int bias_dtype, act;
+};
+
+// How a stage of an MN-major operand arrives: boxes of 128 bytes of row indices x the stage's contraction rows, one after the
+// other.  8-bit operands: 128 indices x 128 rows; 16-bit: 64 x 64.
+template <int MODE> struct MnBox {
+    static constexpr int kEsize = mode_is_hp(MODE) ? 2 : 1;
+    static constexpr int kIdx = 128 / kEsize;                  // row indices of a box
+    static constexpr int kRows = BLOCK_K / kEsize;             // contraction rows of a stage
+    static constexpr int kBytes = 128 * kRows;
+    static constexpr int kStep = (UMMA_K / kEsize) * 128;      // bytes between the contraction rows of consecutive MMAs
 };
 
 // F4: packed e2m1 operands.  A 128-byte stage row then holds 256 elements = two 128-element scale blocks, so every
@@ -276,78 +286,108 @@ __device__ __forceinline__ void epilogue_store_block(const GemmParams &p, uint32
 }
 
 // The same for HP_EPI.  The accumulators are staged as fp32 and everything element-wise happens on the way out, where a lane holds
-// four neighbouring columns of a row, the same columns in every row it writes: the bias is loaded once per 32-column chunk, the
+// four neighbouring columns of a row, the same columns in each of its eight rows: the bias is loaded once per 32-column chunk, the
 // residual, the pre-activation and the output are accessed in whole 32-byte sectors, and the result is rounded once.  The
-// residual's loads are issued before the accumulators are read, so that they return behind the tensor-memory load.
+// residual's loads are issued before the accumulators are read, so that they return behind the tensor-memory load.  The lane's 32
+// values pass the activation together, under one branch: its exponentials and divisions then overlap each other.
 template <int BLOCK_N, typename Release>
 __device__ __forceinline__ void epilogue_fused_block(const GemmParams &p, uint32_t taddr, bool have_acc, int64_t tile_row0, int64_t c_row_end, int n0,
                                                      uint8_t *stg, int lane, int c_begin, int c_end, Release release) {
-    constexpr int kPasses = 8;   // 4 rows each
+    constexpr int kRows = 8;   // a lane's rows of a chunk: row_in_pass, + 4, + 8, ...
     const int n_end = min(p.N, n0 + BLOCK_N);
     const int sub = lane & 7, row_in_pass = lane >> 3;
     const int z_dtype = p.a_fmt ? PT_BF16 : PT_F16;
+    const int rows = (int) min((int64_t) 32, c_row_end - tile_row0);   // rows of this warp inside the matrix (may be negative)
 #pragma unroll 1
     for (int c = c_begin; c < c_end; ++c) {
         const int gcol = n0 + c * 32 + sub * 4;
         const bool vec = p.vec_store_ok && gcol + 4 <= n_end;
-        float res[kPasses][4];
+        const int64_t o0 = (tile_row0 + row_in_pass) * p.ldc + gcol;
+        uint4 res[kRows];   // raw: converting here would wait for every load in turn
         if (p.residual != nullptr && vec) {
+            if (p.c_dtype == PT_F32) {
+                const float *src = reinterpret_cast<const float *>(p.residual) + o0;
 #pragma unroll
-            for (int i = 0; i < kPasses; ++i) {
-                const int64_t grow = tile_row0 + i * 4 + row_in_pass;
-                if (grow < c_row_end) load4_as_f32(p.residual, p.c_dtype, grow * p.ldc + gcol, res[i]);
+                for (int i = 0; i < kRows; ++i)
+                    if (i * 4 + row_in_pass < rows) res[i] = *reinterpret_cast<const uint4 *>(src + (int64_t) (4 * i) * p.ldc);
+            } else {
+                const uint16_t *src = reinterpret_cast<const uint16_t *>(p.residual) + o0;
+#pragma unroll
+                for (int i = 0; i < kRows; ++i)
+                    if (i * 4 + row_in_pass < rows) {
+                        const uint2 w = *reinterpret_cast<const uint2 *>(src + (int64_t) (4 * i) * p.ldc);
+                        res[i].x = w.x; res[i].y = w.y;
+                    }
             }
         }
-        uint32_t r[32];
-        if (have_acc) {
-            tmem_ld32(taddr + c * 32, r);
-            tmem_ld_wait();
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = 0u;
-        }
-        if (have_acc && c == c_end - 1) {
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) release();
-        }
-        uint8_t *my = stg + lane * 128;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4 *>(my + 16 * (i ^ (lane & 7))) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
         float bias[4] = {0.f, 0.f, 0.f, 0.f};
         if (p.bias != nullptr) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (gcol + i < n_end) bias[i] = load_as_f32(p.bias, p.bias_dtype, gcol + i);
         }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const int rr = i * 4 + row_in_pass;
-            const int64_t grow = tile_row0 + rr;
-            if (grow >= c_row_end || gcol >= n_end) continue;
-            const float4 acc = *reinterpret_cast<const float4 *>(stg + rr * 128 + (sub ^ (rr & 7)) * 16);
-            float v[4] = {acc.x + bias[0], acc.y + bias[1], acc.z + bias[2], acc.w + bias[3]};
-            const int64_t o = grow * p.ldc + gcol;
-            if (vec) {
-                if (p.z != nullptr) store4_from_f32(p.z, z_dtype, o, v);
-                act_any4(p.act, v);
-                if (p.residual != nullptr) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += res[i][e];
-                }
-                store4_from_f32(p.C, p.c_dtype, o, v);
+        {
+            uint32_t r[32];
+            if (have_acc) {
+                tmem_ld32(taddr + c * 32, r);
+                tmem_ld_wait();
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (gcol + e >= n_end) continue;
-                    if (p.z != nullptr) store_from_f32(p.z, z_dtype, o + e, v[e]);
-                    float y = act_any(p.act, v[e]);
-                    if (p.residual != nullptr) y += load_as_f32(p.residual, p.c_dtype, o + e);
-                    store_from_f32(p.C, p.c_dtype, o + e, y);
-                }
+                for (int i = 0; i < 32; ++i) r[i] = 0u;
             }
+            if (have_acc && c == c_end - 1) {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) release();
+            }
+            uint8_t *my = stg + lane * 128;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<uint4 *>(my + 16 * (i ^ (lane & 7))) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+        }
+        __syncwarp();
+        float v[kRows][4];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int rr = i * 4 + row_in_pass;
+            const float4 acc = *reinterpret_cast<const float4 *>(stg + rr * 128 + (sub ^ (rr & 7)) * 16);
+            v[i][0] = acc.x + bias[0]; v[i][1] = acc.y + bias[1]; v[i][2] = acc.z + bias[2]; v[i][3] = acc.w + bias[3];
+        }
+        if (p.z != nullptr && vec) {
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+                if (i * 4 + row_in_pass < rows) store4_from_f32(p.z, z_dtype, o0 + (int64_t) (4 * i) * p.ldc, v[i]);
+        } else if (p.z != nullptr) {
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i * 4 + row_in_pass < rows && gcol + e < n_end) store_from_f32(p.z, z_dtype, o0 + (int64_t) (4 * i) * p.ldc + e, v[i][e]);
+        }
+        act_any_all<kRows>(p.act, v);
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                if (i * 4 + row_in_pass >= rows) continue;
+                if (p.residual != nullptr) {
+                    float x[4];
+                    raw4_as_f32(res[i], p.c_dtype, x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[i][e] += x[e];
+                }
+                store4_from_f32(p.C, p.c_dtype, o0 + (int64_t) (4 * i) * p.ldc, v[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (i * 4 + row_in_pass >= rows || gcol + e >= n_end) continue;
+                    const int64_t o = o0 + (int64_t) (4 * i) * p.ldc + e;
+                    float y = v[i][e];
+                    if (p.residual != nullptr) y += load_as_f32(p.residual, p.c_dtype, o);
+                    store_from_f32(p.C, p.c_dtype, o, y);
+                }
         }
         __syncwarp();
     }
@@ -359,6 +399,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     constexpr bool MX = mode_is_mx(MODE);
     constexpr bool F4 = MODE == GEMM_MXF4;
     using Cfg = GemmCfg<BLOCK_N, MX, F4>;
+    using Mn = MnBox<MODE>;
     constexpr int kSfP = Cfg::kSfPerStage;
     constexpr int kStages = Cfg::kStages;
     constexpr int kAccStages = Cfg::kAccStages;
@@ -455,12 +496,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     if (!(ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag))) break;
                     mbar_arrive_expect_tx(&full_bar[stage], Cfg::kABytes + Cfg::kBBytes + Cfg::kSfBytes);
                     const int k0 = (kb_begin + kb) * BLOCK_K;
-                    if (!MX && p.a_mn) tma_load_2d_hint(smem_a + stage * Cfg::kABytes, &tmap_a, &full_bar[stage], (int) a_row0, k0, keep);
-                    else tma_load_2d_hint(smem_a + stage * Cfg::kABytes, &tmap_a, &full_bar[stage], k0, (int) a_row0, keep);
-                    if (!MX && p.b_mn) {   // one 128-wide box per 128 columns of the tile, 16 KiB apart
+                    if (!MX && p.a_mn) {
 #pragma unroll
-                        for (int j = 0; j < (BLOCK_N + 127) / 128; ++j)
-                            tma_load_2d_hint(smem_b + stage * Cfg::kBBytes + j * 16384, &tmap_b, &full_bar[stage], (int) b_row0 + 128 * j, k0, keep);
+                        for (int j = 0; j < BLOCK_M / Mn::kIdx; ++j)
+                            tma_load_2d_hint(smem_a + stage * Cfg::kABytes + j * Mn::kBytes, &tmap_a, &full_bar[stage], ((int) a_row0 + j * Mn::kIdx) * Mn::kEsize,
+                                             k0 / Mn::kEsize, keep);
+                    } else tma_load_2d_hint(smem_a + stage * Cfg::kABytes, &tmap_a, &full_bar[stage], k0, (int) a_row0, keep);
+                    if (!MX && p.b_mn) {
+#pragma unroll
+                        for (int j = 0; j < (BLOCK_N + Mn::kIdx - 1) / Mn::kIdx; ++j)
+                            tma_load_2d_hint(smem_b + stage * Cfg::kBBytes + j * Mn::kBytes, &tmap_b, &full_bar[stage], ((int) b_row0 + j * Mn::kIdx) * Mn::kEsize,
+                                             k0 / Mn::kEsize, keep);
                     } else {
                         tma_load_2d_hint(smem_b + stage * Cfg::kBBytes, &tmap_b, &full_bar[stage], k0, (int) b_row0, keep);
                     }
@@ -482,14 +528,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (elect_one()) {
             constexpr uint32_t kIdescPlainShape = 0;
             (void) kIdescPlainShape;
-            const bool a_mn = !MX && !mode_is_hp(MODE) && p.a_mn, b_mn = !MX && !mode_is_hp(MODE) && p.b_mn;
+            const bool a_mn = !MX && p.a_mn, b_mn = !MX && p.b_mn;
             const uint32_t idesc = F4 ? idesc_block_scaled(1, 1, BLOCK_M, BLOCK_N)   // kind::mxf4: format code 1 = e2m1
                                    : MX ? idesc_block_scaled(p.a_fmt, p.b_fmt, BLOCK_M, BLOCK_N)
                                         : (idesc_f8(p.a_fmt, p.b_fmt, BLOCK_M, BLOCK_N) | ((uint32_t) a_mn << 15) | ((uint32_t) b_mn << 16));
             // one instruction consumes 32 contraction indices: 32 bytes along a K-major row, or 32 rows of 128 bytes of an
             // MN-major tile
-            const uint64_t a_kstep = a_mn ? (uint64_t) ((UMMA_K * 128) >> 4) : (uint64_t) (UMMA_K >> 4);
-            const uint64_t b_kstep = b_mn ? (uint64_t) ((UMMA_K * 128) >> 4) : (uint64_t) (UMMA_K >> 4);
+            const uint64_t a_kstep = a_mn ? (uint64_t) (Mn::kStep >> 4) : (uint64_t) (UMMA_K >> 4);
+            const uint64_t b_kstep = b_mn ? (uint64_t) (Mn::kStep >> 4) : (uint64_t) (UMMA_K >> 4);
             uint32_t stage = 0, phase = 0, acc_stage = 0, acc_phase = 0, sf_buf = 0;
             for (int t = blockIdx.x; ok && walk.locate(t, gi, m_blk, n_blk); t += gridDim.x) {
                 int kb_begin, kb_count;
@@ -517,8 +563,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                         if constexpr (!F4) sf_buf ^= 1;
                     }
                     const uint32_t a_addr = smem_u32(smem_a + stage * Cfg::kABytes), b_addr = smem_u32(smem_b + stage * Cfg::kBBytes);
-                    const uint64_t a_desc = a_mn ? smem_desc_sw128_mn(a_addr, 16384) : smem_desc_sw128(a_addr);
-                    const uint64_t b_desc = b_mn ? smem_desc_sw128_mn(b_addr, 16384) : smem_desc_sw128(b_addr);
+                    const uint64_t a_desc = a_mn ? smem_desc_sw128_mn(a_addr, Mn::kBytes) : smem_desc_sw128(a_addr);
+                    const uint64_t b_desc = b_mn ? smem_desc_sw128_mn(b_addr, Mn::kBytes) : smem_desc_sw128(b_addr);
 #pragma unroll
                     for (int k = 0; k < BLOCK_K / UMMA_K; ++k) {
                         const uint64_t adv = (uint64_t) ((k * UMMA_K) >> 4);
@@ -529,7 +575,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                         else if constexpr (MX)
                             mma_mxf8(d_tmem, a_desc + adv, b_desc + adv, idesc_sf_ids(idesc, k, k), sfa_cur, sfb_cur, accumulate);
                         else if constexpr (mode_is_hp(MODE))
-                            mma_f16(d_tmem, a_desc + adv, b_desc + adv, idesc, accumulate);
+                            mma_f16(d_tmem, a_desc + k * a_kstep, b_desc + k * b_kstep, idesc, accumulate);
                         else
                             mma_f8(d_tmem, a_desc + k * a_kstep, b_desc + k * b_kstep, idesc, accumulate);
                     }
@@ -630,6 +676,12 @@ static int prepare_mx_scales(GemmParams &p, const MxScales &mx, int64_t a_rows, 
     return PT_OK;
 }
 
+// MN-major operand [contraction, rows]; k_bytes counts the contraction as the kernels do (elements x their size)
+template <int MODE> static int make_tmap_mn(CUtensorMap *m, const void *base, int64_t k_bytes, int64_t rows) {
+    using Mn = MnBox<MODE>;
+    return make_tmap_bytes(m, base, k_bytes / Mn::kEsize, rows * Mn::kEsize, rows * Mn::kEsize, Mn::kRows);
+}
+
 template <int BLOCK_N, int MODE>
 static int launch_gemm(const void *a, int64_t a_rows, const void *b, int64_t b_rows, GemmParams p, const MxScales &mx,
                        int max_ctas, int64_t max_tiles, cudaStream_t st) {
@@ -640,9 +692,9 @@ static int launch_gemm(const void *a, int64_t a_rows, const void *b, int64_t b_r
     }
     CUtensorMap ta, tb;
     int rc;
-    // K-major: box = 128 contraction bytes x tile rows; MN-major: box = 128 row indices x 128 contraction rows
-    if ((rc = p.a_mn ? make_tmap_bytes(&ta, a, p.K, a_rows, a_rows, BLOCK_K) : make_tmap_bytes(&ta, a, a_rows, p.K, p.K, BLOCK_M)) != PT_OK) return rc;
-    if ((rc = p.b_mn ? make_tmap_bytes(&tb, b, p.K, b_rows, b_rows, BLOCK_K) : make_tmap_bytes(&tb, b, b_rows, p.K, p.K, BLOCK_N)) != PT_OK) return rc;
+    // K-major: box = 128 contraction bytes x tile rows; MN-major: MnBox
+    if ((rc = p.a_mn ? make_tmap_mn<MODE>(&ta, a, p.K, a_rows) : make_tmap_bytes(&ta, a, a_rows, p.K, p.K, BLOCK_M)) != PT_OK) return rc;
+    if ((rc = p.b_mn ? make_tmap_mn<MODE>(&tb, b, p.K, b_rows) : make_tmap_bytes(&tb, b, b_rows, p.K, p.K, BLOCK_N)) != PT_OK) return rc;
     auto kern = gemm_fp8_kernel<BLOCK_N, MODE>;
     static bool attr_set[64] = {};  // per instantiation and device
     const int dev = current_device_slot();
@@ -665,7 +717,7 @@ static bool g_pair_refused[64] = {};
 template <int BLOCK_N, int MODE>
 static int launch_gemm_pair(const void *a, int64_t a_rows, const void *b, int64_t b_rows, GemmParams p, const MxScales &mx,
                             cudaStream_t st) {
-    using Cfg = PairCfg<BLOCK_N, mode_is_mx(MODE), MODE == GEMM_MXF4>;
+    using Cfg = PairCfg<BLOCK_N, mode_is_mx(MODE), MODE == GEMM_MXF4, MODE == GEMM_HP_EPI>;
     CUtensorMap ta, tb, tsf;
     int rc;
     if constexpr (mode_is_mx(MODE)) {
@@ -674,8 +726,8 @@ static int launch_gemm_pair(const void *a, int64_t a_rows, const void *b, int64_
         const int64_t lines = (int64_t) mx_workspace_bytes(p.M, p.N, p.K, p.koffs ? 1 : p.G, grouped, BLOCK_N) * Cfg::kSfPerStage / 128;
         if ((rc = make_tmap_lines(&tsf, p.sfa_tiled, lines, 4 * Cfg::kSfPerStage)) != PT_OK) return rc;
     }
-    if ((rc = p.a_mn ? make_tmap_bytes(&ta, a, p.K, a_rows, a_rows, BLOCK_K) : make_tmap_bytes(&ta, a, a_rows, p.K, p.K, BLOCK_M)) != PT_OK) return rc;
-    if ((rc = p.b_mn ? make_tmap_bytes(&tb, b, p.K, b_rows, b_rows, BLOCK_K) : make_tmap_bytes(&tb, b, b_rows, p.K, p.K, Cfg::kHalfN)) != PT_OK) return rc;
+    if ((rc = p.a_mn ? make_tmap_mn<MODE>(&ta, a, p.K, a_rows) : make_tmap_bytes(&ta, a, a_rows, p.K, p.K, BLOCK_M)) != PT_OK) return rc;
+    if ((rc = p.b_mn ? make_tmap_mn<MODE>(&tb, b, p.K, b_rows) : make_tmap_bytes(&tb, b, b_rows, p.K, p.K, Cfg::kHalfN)) != PT_OK) return rc;
     if constexpr (!mode_is_mx(MODE)) tsf = ta;
     auto kern = gemm_fp8_pair_kernel<BLOCK_N, MODE>;
     PT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes));
@@ -821,19 +873,23 @@ int gemm_fp8_host(const void *a, const void *a_scale, int a_fmt, const void *b, 
 
 // fp16 / bf16 operands on the same kernels (kind::f16, no scales): the kernels count the contraction in bytes
 int gemm_hp_host(const void *a, const void *b, int ab_dtype, void *c, int c_dtype, int64_t M, int64_t N, int64_t K, float beta,
-                 const int64_t *offs, const int64_t *k_offs, int G, int64_t a_rows_total, int max_ctas, int *status, void *stream) {
+                 const int64_t *offs, const int64_t *k_offs, int G, int64_t a_rows_total, int max_ctas, int *status, void *stream, int a_mn = 0,
+                 int b_mn = 0) {
     PT_REQUIRE(M >= 0 && N >= 0 && K >= 0 && G >= 1 && G <= kMaxGroups, "GEMM: bad shape (M=%lld N=%lld K=%lld G=%d)",
                (long long) M, (long long) N, (long long) K, G);
     PT_REQUIRE(ab_dtype == PT_BF16 || ab_dtype == PT_F16, "GEMM: operands must be bf16 or fp16");
     PT_REQUIRE(c_dtype == PT_BF16 || c_dtype == PT_F16 || c_dtype == PT_F32, "GEMM: bad output dtype");
     PT_REQUIRE(beta == 0.f || beta == 1.f, "GEMM: beta must be 0 or 1");
     PT_REQUIRE(!k_offs || !offs, "GEMM: the variable-K form takes no row offsets");
+    PT_REQUIRE(!(a_mn || b_mn) || (G == 1 && !offs && !k_offs), "GEMM: MN-major operands are taken by the dense form");
+    PT_REQUIRE((!a_mn || M % 8 == 0) && (!b_mn || N % 8 == 0), "GEMM: an MN-major operand needs a row count that is a multiple of 8");
     if (M == 0 || N == 0) return PT_OK;
-    PT_REQUIRE(K > 0 && K % 8 == 0, "GEMM: K must be a positive multiple of 8 for 16-bit operands (got %lld)", (long long) K);
+    PT_REQUIRE(K > 0 && (K % 8 == 0 || (a_mn && b_mn)), "GEMM: K must be a positive multiple of 8 for 16-bit operands (got %lld)", (long long) K);
     PT_REQUIRE(a && b && c, "GEMM: null pointer");
     PT_REQUIRE(N < (1 << 30) && K < (1 << 29) && a_rows_total < (1ll << 31) && (int64_t) G * N < (1ll << 31),
                "GEMM: extent exceeds 32-bit tile coordinates");
     GemmParams p{};
+    p.a_mn = a_mn; p.b_mn = b_mn;
     p.M = M; p.N = (int) N; p.K = (int) (2 * K); p.C = c; p.ldc = N; p.c_dtype = c_dtype; p.beta = beta;
     const int esize = c_dtype == PT_F32 ? 4 : 2;
     p.vec_store_ok = aligned(c, 16) && (N * esize) % 16 == 0;
@@ -850,7 +906,7 @@ int gemm_hp_host(const void *a, const void *b, int ab_dtype, void *c, int c_dtyp
 // Up to this many rows the product runs on the weight-streaming kernels of few_rows.cu, from there on on the tiles above.
 static bool few_rows_better(int64_t M, int64_t N, int64_t K) { return M <= 128; }
 
-static int gemm_bias_act_host(const void *a, const void *b, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
+static int gemm_bias_act_host(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
                               void *z, int act, int64_t M, int64_t N, int64_t K, int *status, cudaStream_t st) {
     PT_REQUIRE(M >= 0 && N >= 0 && K >= 0, "gemm_bias_act: bad shape (M=%lld N=%lld K=%lld)", (long long) M, (long long) N, (long long) K);
     PT_REQUIRE(ab_dtype == PT_BF16 || ab_dtype == PT_F16, "gemm_bias_act: operands must be bf16 or fp16");
@@ -858,13 +914,14 @@ static int gemm_bias_act_host(const void *a, const void *b, int ab_dtype, const 
     PT_REQUIRE(!bias || bias_dtype == PT_BF16 || bias_dtype == PT_F16 || bias_dtype == PT_F32, "gemm_bias_act: bad bias dtype");
     PT_REQUIRE(act >= PT_ACT_SILU && act <= PT_ACT_GELU_TANH, "gemm_bias_act: bad activation %d", act);
     if (M == 0 || N == 0) return PT_OK;
+    PT_REQUIRE(!b_mn || N % 8 == 0, "gemm_bias_act: a contraction-major b needs a row count that is a multiple of 8");
     PT_REQUIRE(K > 0 && K % 8 == 0, "gemm_bias_act: K must be a positive multiple of 8 (got %lld)", (long long) K);
     PT_REQUIRE(a && b && c, "gemm_bias_act: null pointer");
     PT_REQUIRE(N < (1 << 30) && K < (1 << 29) && M < (1ll << 31), "gemm_bias_act: extent exceeds 32-bit tile coordinates");
-    if (few_rows_better(M, N, K)) return few_rows_linear(a, b, ab_dtype, bias, bias_dtype, residual, c, c_dtype, z, act, M, N, K, status, st);
+    if (few_rows_better(M, N, K)) return few_rows_linear(a, b, b_mn, ab_dtype, bias, bias_dtype, residual, c, c_dtype, z, act, M, N, K, status, st);
     GemmParams p{};
     p.M = M; p.N = (int) N; p.K = (int) (2 * K); p.C = c; p.ldc = N; p.c_dtype = c_dtype;
-    p.bias = bias; p.bias_dtype = bias_dtype; p.residual = residual; p.z = z; p.act = act;
+    p.b_mn = b_mn; p.bias = bias; p.bias_dtype = bias_dtype; p.residual = residual; p.z = z; p.act = act;
     const int esize = c_dtype == PT_F32 ? 4 : 2;
     p.vec_store_ok = N % 4 == 0 && aligned(c, 4 * esize) && aligned(residual, 4 * esize) && aligned(z, 8);
     p.a_fmt = p.b_fmt = ab_dtype == PT_BF16 ? 1 : 0;
@@ -881,14 +938,19 @@ extern "C" {
 
 int pt_gemm_bias_act_few_rows(int64_t M, int64_t N, int64_t K) { return few_rows_better(M, N, K) ? 1 : 0; }
 
-int pt_gemm_bias_act(const void *a, const void *b, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype, void *z,
+int pt_gemm_bias_act(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype, void *z,
                      int act, int64_t M, int64_t N, int64_t K, int *status, void *stream) {
-    return gemm_bias_act_host(a, b, ab_dtype, bias, bias_dtype, residual, c, c_dtype, z, act, M, N, K, status, (cudaStream_t) stream);
+    return gemm_bias_act_host(a, b, b_mn, ab_dtype, bias, bias_dtype, residual, c, c_dtype, z, act, M, N, K, status, (cudaStream_t) stream);
 }
 
 int pt_gemm(const void *a, const void *b, int ab_dtype, void *c, int c_dtype, int64_t M, int64_t N, int64_t K, float beta, int *status,
             void *stream) {
     return gemm_hp_host(a, b, ab_dtype, c, c_dtype, M, N, K, beta, nullptr, nullptr, 1, M, 0, status, stream);
+}
+
+int pt_gemm_mn(const void *a, int a_mn, const void *b, int b_mn, int ab_dtype, void *c, int c_dtype, int64_t M, int64_t N, int64_t K, float beta,
+               int *status, void *stream) {
+    return gemm_hp_host(a, b, ab_dtype, c, c_dtype, M, N, K, beta, nullptr, nullptr, 1, M, 0, status, stream, a_mn, b_mn);
 }
 
 int pt_grouped_gemm(const void *a, const void *b, int ab_dtype, void *c, int c_dtype, int64_t a_rows, int64_t N, int64_t K,

@@ -21,8 +21,8 @@
 namespace ptb {
 
 // F4: packed e2m1 operands, 256 elements per 128-byte stage row = two 128-element scale blocks per stage (kSfPerStage)
-template <int BLOCK_N, bool MX, bool F4 = false> struct PairCfg {
-    static constexpr int kEpiWarps = F4 ? 8 : 4;
+template <int BLOCK_N, bool MX, bool F4 = false, bool EPI = false> struct PairCfg {
+    static constexpr int kEpiWarps = F4 || EPI ? 8 : 4;
     static constexpr int kThreads = 32 * (2 + kEpiWarps);
     static constexpr int kHalfN = BLOCK_N / 2;
     static constexpr int kSfbBlocks = (BLOCK_N + 127) / 128;
@@ -48,12 +48,13 @@ template <int BLOCK_N, bool MX, bool F4 = false> struct PairCfg {
 };
 
 template <int BLOCK_N, int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BLOCK_N, mode_is_mx(MODE), MODE == GEMM_MXF4>::kThreads), 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BLOCK_N, mode_is_mx(MODE), MODE == GEMM_MXF4, MODE == GEMM_HP_EPI>::kThreads), 1)
     gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                          const __grid_constant__ CUtensorMap tmap_sf, GemmParams p) {
     constexpr bool MX = mode_is_mx(MODE);
     constexpr bool F4 = MODE == GEMM_MXF4;
-    using Cfg = PairCfg<BLOCK_N, MX, F4>;
+    using Cfg = PairCfg<BLOCK_N, MX, F4, MODE == GEMM_HP_EPI>;
+    using Mn = MnBox<MODE>;
     constexpr int kSfP = Cfg::kSfPerStage;
     constexpr int kStages = Cfg::kStages;
     constexpr int kAccStages = Cfg::kAccStages;
@@ -162,11 +163,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BLOCK_N, mo
                     const uint32_t full_leader = map_to_rank(&full_bar[stage], 0);
                     if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::kStageBytes);
                     const int k0 = (kb_begin + kb) * BLOCK_K;
-                    // MN-major operands (dense tensorwise / rowwise): 128 row indices x 128 contraction rows per CTA
-                    if (!MX && p.a_mn) tma_load_2d_pair_hint(smem_a + stage * Cfg::kABytes, &tmap_a, full_leader, a_row0, k0, keep);
-                    else tma_load_2d_pair_hint(smem_a + stage * Cfg::kABytes, &tmap_a, full_leader, k0, a_row0, keep);
-                    if (!MX && p.b_mn) tma_load_2d_pair_hint(smem_b + stage * Cfg::kBBytes, &tmap_b, full_leader, b_row0, k0, keep);
-                    else tma_load_2d_pair_hint(smem_b + stage * Cfg::kBBytes, &tmap_b, full_leader, k0, b_row0, keep);
+                    // MN-major operands (one group, no block scales): 128 row indices x the stage's contraction rows per CTA
+                    if (!MX && p.a_mn) {
+#pragma unroll
+                        for (int j = 0; j < BLOCK_M / Mn::kIdx; ++j)
+                            tma_load_2d_pair_hint(smem_a + stage * Cfg::kABytes + j * Mn::kBytes, &tmap_a, full_leader, (a_row0 + j * Mn::kIdx) * Mn::kEsize,
+                                                  k0 / Mn::kEsize, keep);
+                    } else tma_load_2d_pair_hint(smem_a + stage * Cfg::kABytes, &tmap_a, full_leader, k0, a_row0, keep);
+                    if (!MX && p.b_mn) {
+#pragma unroll
+                        for (int j = 0; j < (Cfg::kHalfN + Mn::kIdx - 1) / Mn::kIdx; ++j)
+                            tma_load_2d_pair_hint(smem_b + stage * Cfg::kBBytes + j * Mn::kBytes, &tmap_b, full_leader, (b_row0 + j * Mn::kIdx) * Mn::kEsize,
+                                                  k0 / Mn::kEsize, keep);
+                    } else tma_load_2d_pair_hint(smem_b + stage * Cfg::kBBytes, &tmap_b, full_leader, k0, b_row0, keep);
                     if constexpr (MX) {
                         uint8_t *sf = smem_sf + stage * Cfg::kSfBytes;
                         tma_load_2d_pair(sf, &tmap_sf, full_leader, 0, (int) (sfa_line0 + 4 * kSfP * kb));
@@ -185,9 +194,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BLOCK_N, mo
             const uint32_t idesc = F4 ? idesc_block_scaled(1, 1, kTileM, BLOCK_N)  // kind::mxf4: format code 1 = e2m1
                                    : MX ? idesc_block_scaled(p.a_fmt, p.b_fmt, kTileM, BLOCK_N)
                                         : (idesc_f8(p.a_fmt, p.b_fmt, kTileM, BLOCK_N) | ((uint32_t) (p.a_mn != 0) << 15) | ((uint32_t) (p.b_mn != 0) << 16));
-            const bool a_mn = !MX && !mode_is_hp(MODE) && p.a_mn, b_mn = !MX && !mode_is_hp(MODE) && p.b_mn;
-            const uint64_t a_kstep = a_mn ? (uint64_t) ((UMMA_K * 128) >> 4) : (uint64_t) (UMMA_K >> 4);
-            const uint64_t b_kstep = b_mn ? (uint64_t) ((UMMA_K * 128) >> 4) : (uint64_t) (UMMA_K >> 4);
+            const bool a_mn = !MX && p.a_mn, b_mn = !MX && p.b_mn;
+            const uint64_t a_kstep = a_mn ? (uint64_t) (Mn::kStep >> 4) : (uint64_t) (UMMA_K >> 4);
+            const uint64_t b_kstep = b_mn ? (uint64_t) (Mn::kStep >> 4) : (uint64_t) (UMMA_K >> 4);
             uint32_t stage = 0, phase = 0, acc_stage = 0, acc_phase = 0, sf_buf = 0;
             for (int t = pair; ok && walk.locate(t, gi, m_blk, n_blk); t += num_pairs) {
                 int kb_begin, kb_count;
@@ -213,8 +222,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BLOCK_N, mo
                         sf_buf ^= 1;
                     }
                     const uint32_t a_addr = smem_u32(smem_a + stage * Cfg::kABytes), b_addr = smem_u32(smem_b + stage * Cfg::kBBytes);
-                    const uint64_t a_desc = a_mn ? smem_desc_sw128_mn(a_addr, 16384) : smem_desc_sw128(a_addr);
-                    const uint64_t b_desc = b_mn ? smem_desc_sw128_mn(b_addr, 16384) : smem_desc_sw128(b_addr);
+                    const uint64_t a_desc = a_mn ? smem_desc_sw128_mn(a_addr, Mn::kBytes) : smem_desc_sw128(a_addr);
+                    const uint64_t b_desc = b_mn ? smem_desc_sw128_mn(b_addr, Mn::kBytes) : smem_desc_sw128(b_addr);
 #pragma unroll
                     for (int k = 0; k < BLOCK_K / UMMA_K; ++k) {
                         const uint64_t adv = (uint64_t) ((k * UMMA_K) >> 4);
@@ -223,7 +232,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BLOCK_N, mo
                             mma_mxf4_pair(d_tmem, a_desc + adv, b_desc + adv, idesc_sf_ids(idesc, (k & 1) * 2, (k & 1) * 2),
                                           sfa_cur + (k >> 1) * Cfg::kSfColsHalf, sfb_cur + (k >> 1) * Cfg::kSfColsHalf, accumulate);
                         else if constexpr (MX) mma_mxf8_pair(d_tmem, a_desc + adv, b_desc + adv, idesc_sf_ids(idesc, k, k), sfa_cur, sfb_cur, accumulate);
-                        else if constexpr (mode_is_hp(MODE)) mma_f16_pair(d_tmem, a_desc + adv, b_desc + adv, idesc, accumulate);
+                        else if constexpr (mode_is_hp(MODE)) mma_f16_pair(d_tmem, a_desc + k * a_kstep, b_desc + k * b_kstep, idesc, accumulate);
                         else mma_f8_pair(d_tmem, a_desc + k * a_kstep, b_desc + k * b_kstep, idesc, accumulate);
                     }
                     tc_commit_pair(&empty_bar[stage], 3);  // frees the ring slot in both CTAs

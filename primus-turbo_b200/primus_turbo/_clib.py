@@ -72,7 +72,7 @@ SIGNATURES = {
     "pt_moe_few_tokens": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int64, c_int64,
                                   c_int, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p]),
     "pt_gemm_bias_act_few_rows": (c_int, [c_int64, c_int64, c_int64]),
-    "pt_gemm_bias_act": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64,
+    "pt_gemm_bias_act": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64,
                                  c_int64, c_void_p, c_void_p]),
     "pt_act_bias_bwd_parts": (c_int, [c_int64, c_int64]),
     "pt_act_bias_bwd": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int,
@@ -85,6 +85,8 @@ SIGNATURES = {
                                     c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_float,
                                     c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "pt_gemm": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_float, c_void_p, c_void_p]),
+    "pt_gemm_mn": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_float, c_void_p,
+                           c_void_p]),
     "pt_grouped_gemm": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_float,
                                 c_int, c_void_p, c_void_p]),
     "pt_grouped_gemm_variable_k": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int,

@@ -2,8 +2,9 @@
 
 Same call shape as primus_turbo::gemm_impl / gemm_accum_impl of the reference
 (primus_turbo/pytorch/kernels/gemm/gemm_impl.py).  The CUDA kernel is the FP8 one run with kind::f16 instructions:
-C = A . B^T with both operands K-major; the other (trans_a, trans_b, trans_c) combinations swap the operands
-(trans_c) or transpose the 16-bit elements first.
+C = A . B^T; an operand is read as it is stored, K-major ([rows, K]) or contraction-major ([K, rows]), and the operands swap for
+trans_c.  Rows that are not a multiple of 8 elements cannot be read contraction-major in place (a TMA row is a multiple of 16
+bytes): those operands are transposed first.
 """
 from typing import Optional, Tuple
 
@@ -25,14 +26,22 @@ def _k_major16(x, trans):
     return z
 
 
-def _launch(a_km, b_km, out, beta):
-    M, K = a_km.shape
-    N = b_km.shape[0]
-    assert b_km.shape[1] == K, f"contraction mismatch: {tuple(a_km.shape)} vs {tuple(b_km.shape)}"
+def _in_place(x, trans, other, other_trans):
+    """Whether x, needed as [rows, K] and stored [K, rows] (trans), is read where it lies: see the note above.  A contraction that
+    is not a multiple of 8 must be contraction-major on both sides (a K-major operand would be padded)."""
+    def fits(t):
+        return t.shape[1] % 8 == 0 and t.data_ptr() % 16 == 0
+    return trans and x.is_contiguous() and fits(x) and (x.shape[0] % 8 == 0 or (other_trans and other.is_contiguous() and fits(other)))
+
+
+def _launch(a, a_mn, b, b_mn, out, beta):
+    (M, K) = a.shape[::-1] if a_mn else a.shape
+    (N, Kb) = b.shape[::-1] if b_mn else b.shape
+    assert Kb == K, f"contraction mismatch: {tuple(a.shape)} vs {tuple(b.shape)}"
     st = nv.status_word(out.device)
     with nv.on_device(out.device):
-        nv.check(nv.lib().pt_gemm(nv.ptr(a_km), nv.ptr(b_km), nv.src_code(a_km.dtype), nv.ptr(out), nv.src_code(out.dtype), M, N, K,
-                                   float(beta), nv.ptr(st), nv.stream(out.device)), "gemm")
+        nv.check(nv.lib().pt_gemm_mn(nv.ptr(a), int(a_mn), nv.ptr(b), int(b_mn), nv.src_code(a.dtype), nv.ptr(out), nv.src_code(out.dtype), M, N, K,
+                                     float(beta), nv.ptr(st), nv.stream(out.device)), "gemm")
     nv.poll_status(out.device)
     return out
 
@@ -41,15 +50,18 @@ def _gemm(a, trans_a, b, trans_b, out_dtype, trans_c, out=None):
     nv.require_cuda(a, b)
     assert a.dim() == 2 and b.dim() == 2, "Only 2D tensors are supported"
     assert a.dtype == b.dtype and a.dtype in (torch.bfloat16, torch.float16), "a and b must both be bf16 or fp16"
-    a_km = _k_major16(a, trans_a)        # [M, K]
-    b_km = _k_major16(b, not trans_b)    # [N, K]
-    M, N = a_km.shape[0], b_km.shape[0]
+    a_mn, b_mn = _in_place(a, trans_a, b, not trans_b), _in_place(b, not trans_b, a, trans_a)
+    if not a_mn:
+        a = _k_major16(a, trans_a)        # [M, K]
+    if not b_mn:
+        b = _k_major16(b, not trans_b)    # [N, K]
+    M, N = a.shape[1 if a_mn else 0], b.shape[1 if b_mn else 0]
     beta = 0.0 if out is None else 1.0
     if out is None:
         out = torch.empty((N, M) if trans_c else (M, N), dtype=out_dtype, device=a.device)
     else:
         assert out.is_contiguous() and tuple(out.shape) == ((N, M) if trans_c else (M, N))
-    return _launch(b_km, a_km, out, beta) if trans_c else _launch(a_km, b_km, out, beta)
+    return _launch(b, b_mn, a, a_mn, out, beta) if trans_c else _launch(a, a_mn, b, b_mn, out, beta)
 
 
 def gemm_impl(a: torch.Tensor, trans_a: bool, b: torch.Tensor, trans_b: bool, out_dtype: torch.dtype, trans_c: bool,
@@ -71,11 +83,12 @@ def gemm_bias_act_impl(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Op
                        residual: Optional[torch.Tensor], out_dtype: torch.dtype, want_z: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(act(a . op(b) + bias) + residual, the pre-activation in a's type or None) in one kernel."""
     nv.require_cuda(a, b, bias, residual)
-    a_km = _k_major16(a, False)          # [M, K]
-    b_km = _k_major16(b, not trans_b)    # [N, K]
+    b_mn = _in_place(b, not trans_b, a, False)
+    a_km = _k_major16(a, False)                          # [M, K]
+    b_km = b if b_mn else _k_major16(b, not trans_b)     # [N, K]
     if a_km.data_ptr() % 16:             # a view into a larger buffer; TMA reads from 16-byte boundaries
         a_km = a_km.clone()
-    (M, K), N = a_km.shape, b_km.shape[0]
+    (M, K), N = a_km.shape, b_km.shape[1 if b_mn else 0]
     out = torch.empty((M, N), dtype=out_dtype, device=a.device)
     z = torch.empty((M, N), dtype=a.dtype, device=a.device) if want_z else None
     bias = None if bias is None else bias.contiguous()
@@ -88,7 +101,7 @@ def gemm_bias_act_impl(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Op
     else:
         st = nv.ptr(nv.status_word(a.device))
     with nv.on_device(a.device):
-        nv.check(lib.pt_gemm_bias_act(nv.ptr(a_km), nv.ptr(b_km), nv.src_code(a.dtype), nv.ptr(bias), 0 if bias is None else nv.src_code(bias.dtype),
+        nv.check(lib.pt_gemm_bias_act(nv.ptr(a_km), nv.ptr(b_km), int(b_mn), nv.src_code(a.dtype), nv.ptr(bias), 0 if bias is None else nv.src_code(bias.dtype),
                                       nv.ptr(residual), nv.ptr(out), nv.src_code(out_dtype), nv.ptr(z), EPILOGUE_ACTS[act], M, N, K, st,
                                       nv.stream(a.device)), "gemm_bias_act")
     if not few:

@@ -247,3 +247,33 @@ def test_same_bits_on_streams_and_in_graphs(M):
                 g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(h, t) for h, t in zip(held, want))
+
+
+@pytest.mark.parametrize("M,N,K", [(128, 128, 64), (200, 264, 72), (1032, 520, 1000), (4096, 4104, 200), (64, 8, 16), (2048, 4096, 33), (8, 16, 130)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_operands_read_contraction_major_give_the_bits_of_transposed_ones(M, N, K, dt):
+    """pt_gemm_mn on operands stored [K, rows] against the same call on their transposed copies: the tensor core sees the same
+    products in the same order."""
+    from primus_turbo.pytorch.kernels.gemm import gemm_impl as g
+    a, b = _make((M, K), dt, 1), _make((N, K), dt, 2)
+    want = torch.empty(M, N, dtype=torch.float32, device="cuda")
+    ak, bk = g._k_major16(a, False), g._k_major16(b, False)      # padded where K is not a multiple of 8
+    g._launch(ak, False, bk, False, want, 0.0)
+    _assert_within(want, a.double() @ b.double().t(), _mm_bound(a.double(), b.double().t(), K) + U * want.double().abs() + 1e-30, "product")
+    for a_mn, b_mn in ((True, True), (True, False), (False, True)):
+        if K % 8 and not (a_mn and b_mn):
+            continue
+        got = torch.empty_like(want)
+        g._launch(a.t().contiguous() if a_mn else a, a_mn, b.t().contiguous() if b_mn else b, b_mn, got, 0.0)
+        assert torch.equal(got, want), (a_mn, b_mn)
+
+
+@pytest.mark.parametrize("M", [1, 20, 100, 300, 4200])
+def test_weight_read_contraction_major(M):
+    """trans_b=False reads a [K, N] weight in place, with the bits of the transposed call."""
+    from primus_turbo.pytorch.ops import gemm_bias_act
+    for N, K in ((4200, 264), (136, 1000)):
+        a, b, bias = _make((M, K), torch.bfloat16, 1), _make((K, N), torch.bfloat16, 2, K ** -0.5), _make((N,), torch.bfloat16, 3)
+        y = _check(M, N, K, torch.bfloat16, "silu", True, True, trans_b=False)
+        assert y.shape == (M, N)
+        assert torch.equal(gemm_bias_act(a, b, bias=bias, activation="gelu"), gemm_bias_act(a, b.t().contiguous(), bias=bias, activation="gelu", trans_b=True))

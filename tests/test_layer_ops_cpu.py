@@ -101,13 +101,17 @@ def test_gemm_bias_act_abi_refusals():
     from primus_turbo import _clib
     lib = _clib.load()
 
-    def call(ab=0, bias=None, bias_dt=0, cd=0, act=2, M=4, N=8, K=64):
-        return lib.pt_gemm_bias_act(None, None, ab, bias, bias_dt, None, None, cd, None, act, M, N, K, None, None)
+    def call(ab=0, bias=None, bias_dt=0, cd=0, act=2, M=4, N=8, K=64, b_mn=0):
+        return lib.pt_gemm_bias_act(None, None, b_mn, ab, bias, bias_dt, None, None, cd, None, act, M, N, K, None, None)
     for kw, msg in ((dict(ab=2), b"operands"), (dict(cd=7), b"output dtype"), (dict(act=5), b"activation"), (dict(act=-1), b"activation"),
-                    (dict(M=-1), b"bad shape"), (dict(K=12), b"multiple of 8"), (dict(K=0), b"multiple of 8"), (dict(), b"null"),
+                    (dict(M=-1), b"bad shape"), (dict(K=12), b"multiple of 8"), (dict(K=0), b"multiple of 8"), (dict(), b"null"), (dict(b_mn=1, N=12), b"row count"),
                     (dict(bias=ctypes.c_void_p(16), bias_dt=9), b"bias dtype")):
         assert call(**kw) == -1 and msg in lib.pt_last_error(), kw
     assert call(M=0) == 0 and call(N=0) == 0
+    mn = lambda a_mn=1, b_mn=0, M=8, N=8, K=64: lib.pt_gemm_mn(None, a_mn, None, b_mn, 0, None, 0, M, N, K, 0.0, None, None)
+    for kw, msg in ((dict(M=12), b"row count"), (dict(b_mn=1, N=12), b"row count"), (dict(K=12), b"multiple of 8"), (dict(), b"null"),
+                    (dict(b_mn=1, K=12), b"null")):
+        assert mn(**kw) == -1 and msg in lib.pt_last_error(), kw
     bwd = lambda dt=0, act=0, dy=0, dbias=None, parts=0: lib.pt_act_bias_bwd(None, dy, None, dt, act, 4, 8, None, dbias, 0, None, parts, None)
     for kw, msg in ((dict(dt=2), b"operands"), (dict(act=9), b"activation"), (dict(dy=4), b"gradient dtype"), (dict(), b"null"),
                     (dict(dbias=ctypes.c_void_p(16)), b"bias buffers")):

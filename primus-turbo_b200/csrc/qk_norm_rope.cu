@@ -12,8 +12,10 @@
 // rotation needs no exchange and the norm one shuffle reduction.  A warp takes heads of one token only: the token's cosines and
 // sines and the gains are converted once for all of them.  Arithmetic in fp32, one rounding at the end.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
+#include "gemm_common.cuh"
 #include "sm100_ptx.cuh"
 
 namespace ptb {
@@ -21,6 +23,10 @@ using namespace sm100;
 
 constexpr int kQkThreads = 128;
 constexpr int kQkBwdThreads = 256;
+// CTAs per SM the registers are cut to.  Measured on 8192 x 72 heads of 128, bf16 (forward) and 8191 x 40 heads, fp16 (forward and
+// backward): 8 and 3 CTAs 64.5 / 104.7 us; 6 and 3 69.3 / 125; 10 and 4 66.1 / 138; 8 and 2 65.4 / 142.  A few spilled registers
+// cost less than the loads in flight that they buy.
+constexpr int kQkFwdCtas = 8, kQkBwdCtas = 3;
 constexpr int kQkMaxD = 1024;
 
 struct QkArgs {
@@ -35,7 +41,7 @@ struct QkArgs {
     int pos_bytes;
     int64_t T, S, P;                       // tokens, tokens per batch entry, rows of the tables
     int D, R;
-    float eps;
+    float eps, inv_d;                      // 1 / D
     float g0;                              // added to gamma: 1 when zero centred
     float *partial;                        // backward: [parts, D] sums of dn * xhat of every CTA (query CTAs first)
     int parts_q, parts;
@@ -48,13 +54,70 @@ template <> __device__ __forceinline__ float qk_from_f<float>(float v) { return 
 template <> __device__ __forceinline__ __nv_bfloat16 qk_from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half qk_from_f<__half>(float v) { return __float2half_rn(v); }
 
-template <typename T, int V> struct alignas(sizeof(T) * V) QkVec { T e[V]; };
+// ---------------------------------------------------------------- two fp32 values in one instruction
+// The kernels are bound by instruction issue before they are bound by memory (29 instructions per element in scalar form), so
+// the arithmetic runs on register pairs.
+struct F2 { uint64_t v; };
+__device__ __forceinline__ F2 f2(float x, float y) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void f2_split(F2 a, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ F2 f2_swap(F2 a) {
+    float x, y;
+    f2_split(a, x, y);
+    return f2(y, x);
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ float f2_sum(F2 a) {
+    float x, y;
+    f2_split(a, x, y);
+    return x + y;
+}
 
-// Row of the tables of token t, or -1 (reported) when its position lies outside of them.
-__device__ __forceinline__ int64_t qk_position(const QkArgs &a, int64_t t) {
-    int64_t p = t % a.S;
-    if (a.positions != nullptr)
-        p = a.pos_bytes == 8 ? reinterpret_cast<const int64_t *>(a.positions)[t] : (int64_t) reinterpret_cast<const int *>(a.positions)[t];
+// V (2 or 4) elements of a head as they lie in memory, and as V / 2 pairs
+template <typename T, int V> struct QkWords { uint32_t w[V * sizeof(T) / 4]; };
+template <typename T, int V> __device__ __forceinline__ QkWords<T, V> qk_load(const T *p) {
+    QkWords<T, V> r;
+    if constexpr (sizeof(r) == 4) r.w[0] = *reinterpret_cast<const uint32_t *>(p);
+    else if constexpr (sizeof(r) == 8) { const uint2 u = *reinterpret_cast<const uint2 *>(p); r.w[0] = u.x; r.w[1] = u.y; }
+    else { const uint4 u = *reinterpret_cast<const uint4 *>(p); r.w[0] = u.x; r.w[1] = u.y; r.w[2] = u.z; r.w[3] = u.w; }
+    return r;
+}
+template <typename T, int V> __device__ __forceinline__ F2 qk_pair(const QkWords<T, V> &r, int j) {
+    if constexpr (sizeof(T) == 4) return f2(__uint_as_float(r.w[2 * j]), __uint_as_float(r.w[2 * j + 1]));
+    else return f2(lo_f32<T>(r.w[j]), hi_f32<T>(r.w[j]));
+}
+template <typename T> __device__ __forceinline__ uint32_t qk_pack(F2 a) {
+    float x, y;
+    f2_split(a, x, y);
+    return pack2<T>(x, y);
+}
+template <typename T, int V> __device__ __forceinline__ void qk_store(T *p, const F2 (&y)[V / 2]) {
+    if constexpr (sizeof(T) == 4) {
+        if constexpr (V == 2) *reinterpret_cast<uint64_t *>(p) = y[0].v;
+        else *reinterpret_cast<ulonglong2 *>(p) = make_ulonglong2(y[0].v, y[1].v);
+    } else {
+        if constexpr (V == 2) *reinterpret_cast<uint32_t *>(p) = qk_pack<T>(y[0]);
+        else *reinterpret_cast<uint2 *>(p) = make_uint2(qk_pack<T>(y[0]), qk_pack<T>(y[1]));
+    }
+}
+
+// Row of the tables of token t (ti: its index inside its batch entry), or -1 (reported) when its position lies outside of them.
+__device__ __forceinline__ int64_t qk_position(const QkArgs &a, uint32_t t, uint32_t ti) {
+    int64_t p = ti;
+    if (a.pos_bytes == 8) p = reinterpret_cast<const int64_t *>(a.positions)[t];
+    else if (a.pos_bytes == 4) p = reinterpret_cast<const int *>(a.positions)[t];
     if (p < 0 || p >= a.P) {
         if (a.status != nullptr) *reinterpret_cast<volatile int *>(a.status) = PT_ERR_INVALID;
         return -1;
@@ -62,11 +125,13 @@ __device__ __forceinline__ int64_t qk_position(const QkArgs &a, int64_t t) {
     return p;
 }
 
-// What a lane owns of a head: ITEMS items of two vectors.  Neighbours half a rotation apart form an item in the half-split
-// form (indices below NP), else the item just holds two vectors.
-template <int V, int G, int ITEMS, bool IL> struct QkLane {
-    int off[ITEMS][2];      // element offset of each vector; -1: none
-    bool rot[ITEMS][2];     // the vector lies in the rotated part (half-split: both or none)
+// What a lane owns of a head: ITEMS items of two vectors of V elements.  Half-split form: the vectors at i and at i + R / 2 form
+// an item, so that both elements of every pair are the lane's own; what is not rotated is paired up anyhow.  Interleaved form: the
+// pairs lie inside a vector.
+template <typename T, int V, int G, int ITEMS, bool IL> struct QkLane {
+    static constexpr int P = V / 2;   // register pairs of a vector
+    int off[ITEMS][2];                // element offset of each vector; -1: none
+    bool rot[ITEMS][2];               // the vector lies in the rotated part (half-split: both or none)
     __device__ __forceinline__ void init(int lane, int D, int R) {
         const int n_items = IL ? (D / V + 1) / 2 : R / 2 / V + ((D - R) / V + 1) / 2;
 #pragma unroll
@@ -87,40 +152,64 @@ template <int V, int G, int ITEMS, bool IL> struct QkLane {
             rot[i][1] = off[i][1] >= 0 && o1 < R;
         }
     }
-    // half-split: cs[i][e] belongs to pair e of the item; interleaved: cs[i][0 .. V/2) to the first vector, the rest to the second
-    __device__ __forceinline__ void load_table(const float *row, float (&c)[ITEMS][V]) const {
+    // cosines and signed sines of every register pair: the pair becomes x * c + partner(x) * s (turned by -sign)
+    __device__ __forceinline__ void load_table(const float *cos_row, const float *sin_row, float sign, F2 (&c)[ITEMS][2][P], F2 (&s)[ITEMS][2][P]) const {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             if constexpr (IL) {
 #pragma unroll
                 for (int v = 0; v < 2; ++v)
 #pragma unroll
-                    for (int e = 0; e < V / 2; ++e) c[i][v * (V / 2) + e] = rot[i][v] ? row[off[i][v] / 2 + e] : 0.f;
+                    for (int j = 0; j < P; ++j) {
+                        const float ce = rot[i][v] ? cos_row[off[i][v] / 2 + j] : 1.f, se = rot[i][v] ? sign * sin_row[off[i][v] / 2 + j] : 0.f;
+                        c[i][v][j] = f2(ce, ce);
+                        s[i][v][j] = f2(-se, se);
+                    }
             } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e) c[i][e] = rot[i][0] ? row[off[i][0] + e] : 0.f;
+                for (int j = 0; j < P; ++j) {
+                    float2 ce = {1.f, 1.f}, se = {0.f, 0.f};
+                    if (rot[i][0]) {
+                        ce = *reinterpret_cast<const float2 *>(cos_row + off[i][0] + 2 * j);
+                        se = *reinterpret_cast<const float2 *>(sin_row + off[i][0] + 2 * j);
+                    }
+                    c[i][0][j] = c[i][1][j] = f2(ce.x, ce.y);
+                    s[i][0][j] = f2(-sign * se.x, -sign * se.y);
+                    s[i][1][j] = f2(sign * se.x, sign * se.y);
+                }
             }
         }
     }
-    // rotation of the item's two vectors (sign = -1: back)
-    __device__ __forceinline__ void rotate(int i, float (&a)[V], float (&b)[V], const float (&c)[ITEMS][V], const float (&s)[ITEMS][V], float sign) const {
-        if constexpr (IL) {
+    __device__ __forceinline__ void load_gains(const T *gamma, float g0, F2 (&g)[ITEMS][2][P]) const {
 #pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                const float ca = c[i][e / 2], sa = sign * s[i][e / 2], cb = c[i][V / 2 + e / 2], sb = sign * s[i][V / 2 + e / 2];
-                const float a0 = a[e] * ca - a[e + 1] * sa, a1 = a[e + 1] * ca + a[e] * sa;
-                const float b0 = b[e] * cb - b[e + 1] * sb, b1 = b[e + 1] * cb + b[e] * sb;
-                if (rot[i][0]) { a[e] = a0; a[e + 1] = a1; }
-                if (rot[i][1]) { b[e] = b0; b[e + 1] = b1; }
-            }
-        } else {
+        for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float ce = c[i][e], se = sign * s[i][e];
-                const float a0 = a[e] * ce - b[e] * se, b0 = b[e] * ce + a[e] * se;
-                if (rot[i][0]) { a[e] = a0; b[e] = b0; }
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int j = 0; j < P; ++j) {
+                    g[i][v][j] = f2(0.f, 0.f);
+                    if (off[i][v] >= 0) g[i][v][j] = f2(qk_to_f<T>(gamma[off[i][v] + 2 * j]) + g0, qk_to_f<T>(gamma[off[i][v] + 2 * j + 1]) + g0);
+                }
+    }
+    __device__ __forceinline__ void store_zeros(T *head, bool inside) const {
+        const F2 zero[P] = {};
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+                if (inside && off[i][v] >= 0) qk_store<T, V>(head + off[i][v], zero);
+    }
+    // x * m + partner * n for the lane's item i; an element that is not rotated takes nothing of its partner (which may be infinite)
+    __device__ __forceinline__ void turn(int i, const F2 (&x)[2][P], const F2 (&m)[2][P], const F2 (&n)[2][P], bool full, F2 (&y)[2][P]) const {
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                const F2 other = IL ? f2_swap(x[v][j]) : x[1 - v][j];
+                const F2 own = f2_mul(x[v][j], m[v][j]);
+                if (full) y[v][j] = f2_fma(other, n[v][j], own);
+                else y[v][j] = rot[i][v] ? f2_fma(other, n[v][j], own) : own;
             }
-        }
     }
 };
 
@@ -132,82 +221,81 @@ template <int G> __device__ __forceinline__ float qk_group_sum(float v) {
 
 // A warp takes 32 / G * U heads of one token, U per lane group, their loads all in flight together.
 template <typename T, int V, int G, int ITEMS, bool IL, int U>
-__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_fwd_kernel(QkArgs a) {
-    constexpr int kRows = 32 / G;
-    using Vt = QkVec<T, V>;
+__global__ void __launch_bounds__(kQkThreads, kQkFwdCtas) qk_norm_rope_fwd_kernel(QkArgs a) {
+    constexpr int kRows = 32 / G, P = V / 2;
     grid_dep_wait();
     grid_dep_launch();
     const int lane = threadIdx.x & 31;
-    const int per_token = a.chunks[0] + a.chunks[1];
-    const int64_t unit = (int64_t) blockIdx.x * (kQkThreads / 32) + (threadIdx.x >> 5);
-    const int64_t t = unit / per_token;
+    const uint32_t per_token = a.chunks[0] + a.chunks[1];
+    const uint32_t unit = blockIdx.x * (kQkThreads / 32) + (threadIdx.x >> 5);
+    const uint32_t t = unit / per_token;
     if (t >= a.T) return;
     int chunk = (int) (unit - t * per_token);
     const int r = chunk >= a.chunks[0];
     chunk -= r ? a.chunks[0] : 0;
-    const int h0 = chunk * kRows * U + lane / G;
-    const int64_t b = t / a.S, ti = t - b * a.S;
-    const T *x = reinterpret_cast<const T *>(a.x[r]) + b * a.xb[r] + ti * a.xt[r];
-    QkLane<V, G, ITEMS, IL> ln;
+    const uint32_t b = a.S == a.T ? 0 : t / (uint32_t) a.S, ti = t - b * (uint32_t) a.S;
+    const int heads = a.heads[r], h0 = chunk * kRows * U + lane / G;
+    const int64_t xh = a.xh[r];
+    const T *x = reinterpret_cast<const T *>(a.x[r]) + b * a.xb[r] + ti * a.xt[r] + h0 * xh;
+    QkLane<T, V, G, ITEMS, IL> ln;
     ln.init(lane, a.D, a.R);
 
-    Vt raw[U][ITEMS][2];
+    QkWords<T, V> raw[U][ITEMS][2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int h = h0 + u * kRows;
+    for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
-                raw[u][i][v] = Vt{};
-                if (h < a.heads[r] && ln.off[i][v] >= 0) raw[u][i][v] = *reinterpret_cast<const Vt *>(x + (int64_t) h * a.xh[r] + ln.off[i][v]);
+                raw[u][i][v] = QkWords<T, V>{};
+                if (h0 + u * kRows < heads && ln.off[i][v] >= 0) raw[u][i][v] = qk_load<T, V>(x + u * kRows * xh + ln.off[i][v]);
             }
+    T *out = reinterpret_cast<T *>(a.out[r]) + ((int64_t) t * heads + h0) * a.D;
+    const int64_t pos = qk_position(a, t, ti);
+    if (pos < 0) {   // the same for the whole warp
+        for (int u = 0; u < U; ++u) ln.store_zeros(out + u * kRows * a.D, h0 + u * kRows < heads);
+        return;
     }
-    const int64_t pos = qk_position(a, t);
-    float c[ITEMS][V], s[ITEMS][V], g[ITEMS][2][V];
-    ln.load_table(a.cos + (pos < 0 ? 0 : pos) * (a.R / 2), c);
-    ln.load_table(a.sin + (pos < 0 ? 0 : pos) * (a.R / 2), s);
-    const T *gamma = reinterpret_cast<const T *>(a.gamma[r]);
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            Vt gr = {};
-            if (ln.off[i][v] >= 0) gr = *reinterpret_cast<const Vt *>(gamma + ln.off[i][v]);
-#pragma unroll
-            for (int e = 0; e < V; ++e) g[i][v][e] = qk_to_f<T>(gr.e[e]) + a.g0;
-        }
-
-    T *out = reinterpret_cast<T *>(a.out[r]) + t * a.heads[r] * a.D;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        float ss = 0.f;
+    const bool full = a.R == a.D;
+    F2 m[ITEMS][2][P], n[ITEMS][2][P];   // gain times cosine; the partner's gain times the signed sine
+    {
+        F2 c[ITEMS][2][P], s[ITEMS][2][P], g[ITEMS][2][P];
+        const int64_t row = pos * (a.R / 2);
+        ln.load_table(a.cos + row, a.sin + row, 1.f, c, s);
+        ln.load_gains(reinterpret_cast<const T *>(a.gamma[r]), a.g0, g);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
             for (int v = 0; v < 2; ++v)
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float f = qk_to_f<T>(raw[u][i][v].e[e]);
-                    ss += f * f;
+                for (int j = 0; j < P; ++j) {
+                    m[i][v][j] = f2_mul(g[i][v][j], c[i][v][j]);
+                    n[i][v][j] = f2_mul(IL ? f2_swap(g[i][v][j]) : g[i][1 - v][j], s[i][v][j]);
                 }
-        const float rstd = rsqrtf(qk_group_sum<G>(ss) / (float) a.D + a.eps);
-        const int h = h0 + u * kRows;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        F2 xs[ITEMS][2][P], ss2 = f2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int j = 0; j < P; ++j) {
+                    xs[i][v][j] = qk_pair<T, V>(raw[u][i][v], j);
+                    ss2 = f2_fma(xs[i][v][j], xs[i][v][j], ss2);
+                }
+        float rstd = rsqrtf(qk_group_sum<G>(f2_sum(ss2)) * a.inv_d + a.eps);
+        const F2 scale = f2(rstd, rstd);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            float n[2][V];
-#pragma unroll
-            for (int v = 0; v < 2; ++v)
-#pragma unroll
-                for (int e = 0; e < V; ++e) n[v][e] = qk_to_f<T>(raw[u][i][v].e[e]) * rstd * g[i][v][e];
-            ln.rotate(i, n[0], n[1], c, s, 1.f);
+            F2 y[2][P];
+            ln.turn(i, xs[i], m[i], n[i], full, y);
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
-                if (h >= a.heads[r] || ln.off[i][v] < 0) continue;
-                Vt o;
 #pragma unroll
-                for (int e = 0; e < V; ++e) o.e[e] = qk_from_f<T>(pos < 0 ? 0.f : n[v][e]);
-                *reinterpret_cast<Vt *>(out + (int64_t) h * a.D + ln.off[i][v]) = o;
+                for (int j = 0; j < P; ++j) y[v][j] = f2_mul(y[v][j], scale);
+                if (h0 + u * kRows < heads && ln.off[i][v] >= 0) qk_store<T, V>(out + u * kRows * a.D + ln.off[i][v], y[v]);
             }
         }
     }
@@ -216,97 +304,93 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_fwd_kernel(QkArgs a) 
 // Persistent CTAs: the first parts_q work on queries, the rest on keys, so that a lane's share of dgamma stays in registers over
 // all its heads.  Per CTA one row of partial sums (fixed order: lanes, then warps); qk_dgamma_kernel adds the rows.
 template <typename T, int V, int G, int ITEMS, bool IL, int U>
-__global__ void __launch_bounds__(kQkBwdThreads) qk_norm_rope_bwd_kernel(QkArgs a) {
-    constexpr int kRows = 32 / G;
+__global__ void __launch_bounds__(kQkBwdThreads, kQkBwdCtas) qk_norm_rope_bwd_kernel(QkArgs a) {
+    constexpr int kRows = 32 / G, P = V / 2;
     constexpr int kWarps = kQkBwdThreads / 32;
-    using Vt = QkVec<T, V>;
     extern __shared__ float s_part[];   // [warps][D]
     grid_dep_wait();
     grid_dep_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int r = (int) blockIdx.x >= a.parts_q;
-    const int cta = (int) blockIdx.x - (r ? a.parts_q : 0), ctas = r ? a.parts - a.parts_q : a.parts_q;
-    const int64_t units = a.T * a.chunks[r];
-    QkLane<V, G, ITEMS, IL> ln;
+    const uint32_t cta = blockIdx.x - (r ? a.parts_q : 0), ctas = r ? a.parts - a.parts_q : a.parts_q;
+    const uint32_t chunks = a.chunks[r], units = (uint32_t) a.T * chunks;
+    const int heads = a.heads[r];
+    const int64_t xh = a.xh[r], gh = a.gh[r];
+    const bool full = a.R == a.D;
+    QkLane<T, V, G, ITEMS, IL> ln;
     ln.init(lane, a.D, a.R);
-    float g[ITEMS][2][V], dg[ITEMS][2][V];
-    const T *gamma = reinterpret_cast<const T *>(a.gamma[r]);
+    F2 g[ITEMS][2][P], dg[ITEMS][2][P];
+    ln.load_gains(reinterpret_cast<const T *>(a.gamma[r]), a.g0, g);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            Vt gr = {};
-            if (ln.off[i][v] >= 0) gr = *reinterpret_cast<const Vt *>(gamma + ln.off[i][v]);
+        for (int v = 0; v < 2; ++v)
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                g[i][v][e] = qk_to_f<T>(gr.e[e]) + a.g0;
-                dg[i][v][e] = 0.f;
-            }
-        }
-    for (int64_t unit = (int64_t) cta * kWarps + warp; unit < units; unit += (int64_t) ctas * kWarps) {
-        const int64_t t = unit / a.chunks[r];
-        const int h0 = (int) (unit - t * a.chunks[r]) * kRows * U + lane / G;
-        const int64_t b = t / a.S, ti = t - b * a.S;
-        const T *x = reinterpret_cast<const T *>(a.x[r]) + b * a.xb[r] + ti * a.xt[r];
-        const T *dy = reinterpret_cast<const T *>(a.dy[r]) + b * a.gb[r] + ti * a.gt[r];
-        Vt rx[U][ITEMS][2], rd[U][ITEMS][2];
+            for (int j = 0; j < P; ++j) dg[i][v][j] = f2(0.f, 0.f);
+    for (uint32_t unit = cta * kWarps + warp; unit < units; unit += ctas * kWarps) {
+        const uint32_t t = unit / chunks, b = a.S == a.T ? 0 : t / (uint32_t) a.S, ti = t - b * (uint32_t) a.S;
+        const int h0 = (int) (unit - t * chunks) * kRows * U + lane / G;
+        const T *x = reinterpret_cast<const T *>(a.x[r]) + b * a.xb[r] + ti * a.xt[r] + h0 * xh;
+        const T *dy = reinterpret_cast<const T *>(a.dy[r]) + b * a.gb[r] + ti * a.gt[r] + h0 * gh;
+        QkWords<T, V> rx[U][ITEMS][2], rd[U][ITEMS][2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = h0 + u * kRows;
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
-                    rx[u][i][v] = Vt{};
-                    rd[u][i][v] = Vt{};
-                    if (h < a.heads[r] && ln.off[i][v] >= 0) {
-                        rx[u][i][v] = *reinterpret_cast<const Vt *>(x + (int64_t) h * a.xh[r] + ln.off[i][v]);
-                        rd[u][i][v] = *reinterpret_cast<const Vt *>(dy + (int64_t) h * a.gh[r] + ln.off[i][v]);
+                    rx[u][i][v] = QkWords<T, V>{};
+                    rd[u][i][v] = QkWords<T, V>{};
+                    if (h0 + u * kRows < heads && ln.off[i][v] >= 0) {
+                        rx[u][i][v] = qk_load<T, V>(x + u * kRows * xh + ln.off[i][v]);
+                        rd[u][i][v] = qk_load<T, V>(dy + u * kRows * gh + ln.off[i][v]);
                     }
                 }
+        T *dx = reinterpret_cast<T *>(a.out[r]) + ((int64_t) t * heads + h0) * a.D;
+        const int64_t pos = qk_position(a, t, ti);
+        if (pos < 0) {   // the same for the whole warp; nothing for dgamma either
+            for (int u = 0; u < U; ++u) ln.store_zeros(dx + u * kRows * a.D, h0 + u * kRows < heads);
+            continue;
         }
-        const int64_t pos = qk_position(a, t);
-        float c[ITEMS][V], s[ITEMS][V];
-        ln.load_table(a.cos + (pos < 0 ? 0 : pos) * (a.R / 2), c);
-        ln.load_table(a.sin + (pos < 0 ? 0 : pos) * (a.R / 2), s);
-        T *dx = reinterpret_cast<T *>(a.out[r]) + t * a.heads[r] * a.D;
+        const int64_t row = pos * (a.R / 2);
+        F2 c[ITEMS][2][P], s[ITEMS][2][P];
+        ln.load_table(a.cos + row, a.sin + row, -1.f, c, s);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int h = h0 + u * kRows;
-            float ss = 0.f, dot = 0.f;
-            float dn[ITEMS][2][V];
+            F2 xs[ITEMS][2][P], dn[ITEMS][2][P], ss2 = f2(0.f, 0.f), dot2 = f2(0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
+                F2 d[2][P];
 #pragma unroll
                 for (int v = 0; v < 2; ++v)
 #pragma unroll
-                    for (int e = 0; e < V; ++e) dn[i][v][e] = qk_to_f<T>(rd[u][i][v].e[e]);
-                ln.rotate(i, dn[i][0], dn[i][1], c, s, -1.f);
-#pragma unroll
-                for (int v = 0; v < 2; ++v)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const float f = qk_to_f<T>(rx[u][i][v].e[e]);
-                        ss += f * f;
-                        dot += dn[i][v][e] * g[i][v][e] * f;
+                    for (int j = 0; j < P; ++j) {
+                        xs[i][v][j] = qk_pair<T, V>(rx[u][i][v], j);
+                        d[v][j] = qk_pair<T, V>(rd[u][i][v], j);
+                        ss2 = f2_fma(xs[i][v][j], xs[i][v][j], ss2);
                     }
+                ln.turn(i, d, c[i], s[i], full, dn[i]);
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int j = 0; j < P; ++j) dot2 = f2_fma(f2_mul(dn[i][v][j], g[i][v][j]), xs[i][v][j], dot2);
             }
-            const float rstd = rsqrtf(qk_group_sum<G>(ss) / (float) a.D + a.eps);
-            const float m = qk_group_sum<G>(dot) * rstd / (float) a.D;   // mean(dn * g * xhat)
-            if (h >= a.heads[r]) continue;
+            const float rstd = rsqrtf(qk_group_sum<G>(f2_sum(ss2)) * a.inv_d + a.eps);
+            const float mean = qk_group_sum<G>(f2_sum(dot2)) * rstd * a.inv_d;   // mean(dn * g * xhat)
+            if (h0 + u * kRows >= heads) continue;
+            const F2 r2 = f2(rstd, rstd), m2 = f2(-mean * rstd, -mean * rstd);
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
-                    if (ln.off[i][v] < 0) continue;
-                    Vt o;
+                    F2 o[P];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const float xh = qk_to_f<T>(rx[u][i][v].e[e]) * rstd;
-                        o.e[e] = qk_from_f<T>(pos < 0 ? 0.f : (dn[i][v][e] * g[i][v][e] - xh * m) * rstd);
-                        if (pos >= 0) dg[i][v][e] += dn[i][v][e] * xh;
+                    for (int j = 0; j < P; ++j) {
+                        const F2 xhat = f2_mul(xs[i][v][j], r2);
+                        o[j] = f2_fma(xhat, m2, f2_mul(f2_mul(dn[i][v][j], g[i][v][j]), r2));
+                        dg[i][v][j] = f2_fma(dn[i][v][j], xhat, dg[i][v][j]);
                     }
-                    *reinterpret_cast<Vt *>(dx + (int64_t) h * a.D + ln.off[i][v]) = o;
+                    if (ln.off[i][v] >= 0) qk_store<T, V>(dx + u * kRows * a.D + ln.off[i][v], o);
                 }
         }
     }
@@ -315,11 +399,15 @@ __global__ void __launch_bounds__(kQkBwdThreads) qk_norm_rope_bwd_kernel(QkArgs 
 #pragma unroll
         for (int v = 0; v < 2; ++v)
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                float d = dg[i][v][e];
+            for (int j = 0; j < P; ++j) {
+                float d[2];
+                f2_split(dg[i][v][j], d[0], d[1]);
 #pragma unroll
-                for (int o = G; o < 32; o <<= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-                if (lane < G && ln.off[i][v] >= 0) s_part[warp * a.D + ln.off[i][v] + e] = d;
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int o = G; o < 32; o <<= 1) d[e] += __shfl_xor_sync(0xffffffffu, d[e], o);
+                    if (lane < G && ln.off[i][v] >= 0) s_part[warp * a.D + ln.off[i][v] + 2 * j + e] = d[e];
+                }
             }
     __syncthreads();
     for (int d = threadIdx.x; d < a.D; d += kQkBwdThreads) {
@@ -355,7 +443,7 @@ __global__ void __launch_bounds__(kQkBwdThreads) qk_norm_rope_any_kernel(QkArgs 
         int h = (int) (unit - t * per_token);
         const int r = BWD ? r_cta : h >= a.heads[0];
         if (!BWD && r) h -= a.heads[0];
-        const int64_t b = t / a.S, ti = t - b * a.S, pos = qk_position(a, t);
+        const int64_t b = t / a.S, ti = t - b * a.S, pos = qk_position(a, (uint32_t) t, (uint32_t) ti);
         const T *x = reinterpret_cast<const T *>(a.x[r]) + b * a.xb[r] + ti * a.xt[r] + (int64_t) h * a.xh[r];
         const T *dy = BWD ? reinterpret_cast<const T *>(a.dy[r]) + b * a.gb[r] + ti * a.gt[r] + (int64_t) h * a.gh[r] : nullptr;
         const T *gamma = reinterpret_cast<const T *>(a.gamma[r]);
@@ -447,44 +535,45 @@ __global__ void __launch_bounds__(512) qk_dgamma_kernel(const float *__restrict_
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-// How a head is laid over lanes.  vec elements per access: a full 16 bytes when the head, both halves of the rotation and every
-// stride are whole vectors; else two elements; 0: the element-wise kernel.
+// How a head is laid over lanes: elements per access, four when the head, both halves of the rotation and every stride are whole
+// vectors of them, else two; 0: the element-wise kernel.
 static int qk_vec(const QkArgs &a, int esize, bool il, bool bwd) {
-    for (int v : {16 / esize, 2}) {
-        bool ok = a.D % v == 0 && (il ? a.R : a.R / 2) % v == 0 && a.R % v == 0;
+    for (int v : {4, 2}) {
+        bool ok = aligned(a.cos, 8) && aligned(a.sin, 8) && a.D % v == 0 && (il ? a.R : a.R / 2) % v == 0 && a.R % v == 0;
         for (int r = 0; r < 2; ++r) {
             ok = ok && aligned(a.x[r], v * esize) && aligned(a.gamma[r], v * esize) && aligned(a.out[r], v * esize) &&
                  (a.xb[r] | a.xt[r] | a.xh[r]) % v == 0;
             if (bwd) ok = ok && aligned(a.dy[r], v * esize) && (a.gb[r] | a.gt[r] | a.gh[r]) % v == 0;
         }
         const int items = il ? (a.D / v + 1) / 2 : a.R / 2 / v + ((a.D - a.R) / v + 1) / 2;
-        if (ok && items <= (v == 2 ? 64 : 32)) return v;
+        if (ok && items <= 64) return v;
     }
     return 0;
 }
 
 template <typename T, int V, int G, int ITEMS, bool IL> static int qk_launch(QkArgs a, bool bwd, cudaStream_t st) {
-    // heads per lane group and warp: four while a token has that many (their loads overlap), one otherwise
-    constexpr int kRows = 32 / G;
+    // heads per lane group and warp, their loads in flight together; one where a token has fewer
+    constexpr int kRows = 32 / G, kMost = (ITEMS == 1 ? 4 : 2) / (sizeof(T) == 4 ? 2 : 1);
+    const int most = std::max(a.heads[0], a.heads[1]);
+    auto set_chunks = [&](int U) { for (int r = 0; r < 2; ++r) a.chunks[r] = (int) ceil_div(a.heads[r], kRows * U); };
     if (!bwd) {
-        const int most = std::max(a.heads[0], a.heads[1]);
-        const int U = most >= 2 * kRows && ITEMS == 1 ? 4 : 1;
-        for (int r = 0; r < 2; ++r) a.chunks[r] = (int) ceil_div(a.heads[r], kRows * U);
-        const int64_t grid = ceil_div(a.T * (a.chunks[0] + a.chunks[1]), kQkThreads / 32);
-        PT_REQUIRE(grid < (1ll << 31), "qk_norm_rope: too many tokens");
-        if (U == 4) PT_CUDA_OK(launch_overlapped(qk_norm_rope_fwd_kernel<T, V, G, ITEMS, IL, ITEMS == 1 ? 4 : 1>, dim3((unsigned) grid), dim3(kQkThreads), 0, st, a));
-        else PT_CUDA_OK(launch_overlapped(qk_norm_rope_fwd_kernel<T, V, G, ITEMS, IL, 1>, dim3((unsigned) grid), dim3(kQkThreads), 0, st, a));
-        return PT_OK;
+        auto go = [&](auto u) {
+            constexpr int U = decltype(u)::value;
+            set_chunks(U);
+            const int64_t grid = ceil_div(a.T * (a.chunks[0] + a.chunks[1]), kQkThreads / 32);
+            PT_CUDA_OK(launch_overlapped(qk_norm_rope_fwd_kernel<T, V, G, ITEMS, IL, U>, dim3((unsigned) grid), dim3(kQkThreads), 0, st, a));
+            return (int) PT_OK;
+        };
+        return most >= 2 * kRows ? go(std::integral_constant<int, kMost>{}) : go(std::integral_constant<int, 1>{});
     }
-    constexpr int U = ITEMS == 1 ? 2 : 1;
-    for (int r = 0; r < 2; ++r) a.chunks[r] = (int) ceil_div(a.heads[r], kRows * U);
+    constexpr int U = ITEMS == 1 && sizeof(T) == 2 ? 2 : 1;
+    set_chunks(U);
     PT_CUDA_OK(launch_overlapped(qk_norm_rope_bwd_kernel<T, V, G, ITEMS, IL, U>, dim3(a.parts), dim3(kQkBwdThreads),
                                  (size_t) (kQkBwdThreads / 32) * a.D * 4, st, a));
     return PT_OK;
 }
 
 template <typename T, bool IL> static int qk_dispatch(const QkArgs &a, bool bwd, cudaStream_t st) {
-    constexpr int V16 = 16 / (int) sizeof(T);
     const int v = qk_vec(a, sizeof(T), IL, bwd);
     if (v == 0) {
         const size_t smem = bwd ? (size_t) (kQkBwdThreads / 32) * a.D * 4 : 0;
@@ -494,11 +583,11 @@ template <typename T, bool IL> static int qk_dispatch(const QkArgs &a, bool bwd,
         return PT_OK;
     }
     const int items = IL ? (a.D / v + 1) / 2 : a.R / 2 / v + ((a.D - a.R) / v + 1) / 2;
-    if (v == V16) {
-        if (items <= 4) return qk_launch<T, V16, 4, 1, IL>(a, bwd, st);
-        if (items <= 8) return qk_launch<T, V16, 8, 1, IL>(a, bwd, st);
-        if (items <= 16) return qk_launch<T, V16, 16, 1, IL>(a, bwd, st);
-        return qk_launch<T, V16, 32, 1, IL>(a, bwd, st);
+    if (v == 4) {
+        if (items <= 8) return qk_launch<T, 4, 8, 1, IL>(a, bwd, st);
+        if (items <= 16) return qk_launch<T, 4, 16, 1, IL>(a, bwd, st);
+        if (items <= 32) return qk_launch<T, 4, 32, 1, IL>(a, bwd, st);
+        return qk_launch<T, 4, 32, 2, IL>(a, bwd, st);
     }
     if (items <= 16) return qk_launch<T, 2, 16, 1, IL>(a, bwd, st);
     if (items <= 32) return qk_launch<T, 2, 32, 1, IL>(a, bwd, st);
@@ -510,6 +599,7 @@ static int qk_check(const QkArgs &a, int dtype, int64_t B) {
     PT_REQUIRE(B >= 0 && a.S >= 0 && a.heads[0] >= 0 && a.heads[1] >= 0, "qk_norm_rope: negative extent");
     PT_REQUIRE(a.D >= 1 && a.D <= kQkMaxD && a.R >= 0 && a.R % 2 == 0 && a.R <= a.D,
                "qk_norm_rope: the head size must lie in [1, %d] and the rotated part be even and no larger (got %d, %d)", kQkMaxD, a.D, a.R);
+    PT_REQUIRE(a.T < (1ll << 31) && a.T * (a.heads[0] + (int64_t) a.heads[1]) < (1ll << 31), "qk_norm_rope: tokens x heads exceed 32-bit indices");
     PT_REQUIRE(a.pos_bytes == 0 || a.pos_bytes == 4 || a.pos_bytes == 8, "qk_norm_rope: positions must be int32 or int64");
     PT_REQUIRE((a.pos_bytes == 0) == (a.positions == nullptr), "qk_norm_rope: positions and their size go together");
     for (int r = 0; r < 2; ++r)
@@ -541,7 +631,7 @@ int pt_qk_norm_rope_fwd(const void *q, const void *k, int dtype, const void *q_g
     a.xb[0] = q_strides[0]; a.xt[0] = q_strides[1]; a.xh[0] = q_strides[2];
     a.xb[1] = k_strides[0]; a.xt[1] = k_strides[1]; a.xh[1] = k_strides[2];
     a.heads[0] = Hq; a.heads[1] = Hk; a.cos = cos; a.sin = sin; a.positions = positions; a.pos_bytes = pos_bytes;
-    a.T = B * S; a.S = S; a.P = P; a.D = D; a.R = R; a.eps = eps; a.g0 = zero_centered ? 1.f : 0.f; a.status = status;
+    a.T = B * S; a.S = S; a.P = P; a.D = D; a.R = R; a.eps = eps; a.inv_d = 1.f / (float) std::max(D, 1); a.g0 = zero_centered ? 1.f : 0.f; a.status = status;
     const int rc = qk_check(a, dtype, B);
     if (rc != PT_OK) return rc;
     if (a.T == 0 || Hq + Hk == 0) return PT_OK;
@@ -567,7 +657,7 @@ int pt_qk_norm_rope_bwd(const void *dq, const void *dk, const void *q, const voi
     a.gb[0] = dq_strides[0]; a.gt[0] = dq_strides[1]; a.gh[0] = dq_strides[2];
     a.gb[1] = dk_strides[0]; a.gt[1] = dk_strides[1]; a.gh[1] = dk_strides[2];
     a.heads[0] = Hq; a.heads[1] = Hk; a.cos = cos; a.sin = sin; a.positions = positions; a.pos_bytes = pos_bytes;
-    a.T = B * S; a.S = std::max<int64_t>(S, 1); a.P = P; a.D = D; a.R = R; a.eps = eps; a.g0 = zero_centered ? 1.f : 0.f; a.status = status;
+    a.T = B * S; a.S = std::max<int64_t>(S, 1); a.P = P; a.D = D; a.R = R; a.eps = eps; a.inv_d = 1.f / (float) std::max(D, 1); a.g0 = zero_centered ? 1.f : 0.f; a.status = status;
     const int rc = qk_check(a, dtype, B);
     if (rc != PT_OK) return rc;
     for (int r = 0; r < 2; ++r) PT_REQUIRE(a.T == 0 || a.heads[r] == 0 || a.dy[r], "qk_norm_rope backward: null pointer");

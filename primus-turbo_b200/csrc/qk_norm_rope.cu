@@ -594,6 +594,14 @@ template <typename T, bool IL> static int qk_dispatch(const QkArgs &a, bool bwd,
     return qk_launch<T, 2, 32, 2, IL>(a, bwd, st);
 }
 
+// Host strides (batch, token, head) into the arguments; the stride of an extent of one is never used, but would decide the
+// alignment of the vector accesses, so it counts as zero.
+static void qk_strides(const int64_t *s, int64_t B, int64_t S, int heads, int64_t &b, int64_t &t, int64_t &h) {
+    b = B > 1 ? s[0] : 0;
+    t = S > 1 ? s[1] : 0;
+    h = heads > 1 ? s[2] : 0;
+}
+
 static int qk_check(const QkArgs &a, int dtype, int64_t B) {
     PT_REQUIRE(dtype == PT_BF16 || dtype == PT_F16 || dtype == PT_F32, "qk_norm_rope: unsupported dtype %d", dtype);
     PT_REQUIRE(B >= 0 && a.S >= 0 && a.heads[0] >= 0 && a.heads[1] >= 0, "qk_norm_rope: negative extent");
@@ -628,8 +636,8 @@ int pt_qk_norm_rope_fwd(const void *q, const void *k, int dtype, const void *q_g
     QkArgs a{};
     PT_REQUIRE(q_strides && k_strides, "qk_norm_rope: strides required");
     a.x[0] = q; a.x[1] = k; a.gamma[0] = q_gamma; a.gamma[1] = k_gamma; a.out[0] = q_out; a.out[1] = k_out;
-    a.xb[0] = q_strides[0]; a.xt[0] = q_strides[1]; a.xh[0] = q_strides[2];
-    a.xb[1] = k_strides[0]; a.xt[1] = k_strides[1]; a.xh[1] = k_strides[2];
+    qk_strides(q_strides, B, S, Hq, a.xb[0], a.xt[0], a.xh[0]);
+    qk_strides(k_strides, B, S, Hk, a.xb[1], a.xt[1], a.xh[1]);
     a.heads[0] = Hq; a.heads[1] = Hk; a.cos = cos; a.sin = sin; a.positions = positions; a.pos_bytes = pos_bytes;
     a.T = B * S; a.S = S; a.P = P; a.D = D; a.R = R; a.eps = eps; a.inv_d = 1.f / (float) std::max(D, 1); a.g0 = zero_centered ? 1.f : 0.f; a.status = status;
     const int rc = qk_check(a, dtype, B);
@@ -652,10 +660,10 @@ int pt_qk_norm_rope_bwd(const void *dq, const void *dk, const void *q, const voi
     QkArgs a{};
     PT_REQUIRE(q_strides && k_strides && dq_strides && dk_strides, "qk_norm_rope backward: strides required");
     a.x[0] = q; a.x[1] = k; a.dy[0] = dq; a.dy[1] = dk; a.gamma[0] = q_gamma; a.gamma[1] = k_gamma; a.out[0] = dq_in; a.out[1] = dk_in;
-    a.xb[0] = q_strides[0]; a.xt[0] = q_strides[1]; a.xh[0] = q_strides[2];
-    a.xb[1] = k_strides[0]; a.xt[1] = k_strides[1]; a.xh[1] = k_strides[2];
-    a.gb[0] = dq_strides[0]; a.gt[0] = dq_strides[1]; a.gh[0] = dq_strides[2];
-    a.gb[1] = dk_strides[0]; a.gt[1] = dk_strides[1]; a.gh[1] = dk_strides[2];
+    qk_strides(q_strides, B, S, Hq, a.xb[0], a.xt[0], a.xh[0]);
+    qk_strides(k_strides, B, S, Hk, a.xb[1], a.xt[1], a.xh[1]);
+    qk_strides(dq_strides, B, S, Hq, a.gb[0], a.gt[0], a.gh[0]);
+    qk_strides(dk_strides, B, S, Hk, a.gb[1], a.gt[1], a.gh[1]);
     a.heads[0] = Hq; a.heads[1] = Hk; a.cos = cos; a.sin = sin; a.positions = positions; a.pos_bytes = pos_bytes;
     a.T = B * S; a.S = std::max<int64_t>(S, 1); a.P = P; a.D = D; a.R = R; a.eps = eps; a.inv_d = 1.f / (float) std::max(D, 1); a.g0 = zero_centered ? 1.f : 0.f; a.status = status;
     const int rc = qk_check(a, dtype, B);

@@ -40,11 +40,13 @@ def fmt_code(dtype) -> int:
 
 
 def ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()      # a plain int: ctypes converts it by the argument's type
 
 
 def stream(device=None):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    idx = None if device is None else device.index
+    # the handle alone: building a torch Stream object around it costs as much as a launch
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
 
 
 _NO_GUARD = contextlib.nullcontext()
@@ -54,7 +56,7 @@ def on_device(device):
     """Context in which `device` is the current CUDA device; free when it already is (the usual case: one process
     per GPU), a torch device guard otherwise."""
     idx = device.index
-    if idx is None or idx == torch.cuda.current_device():
+    if idx is None or idx == torch._C._cuda_getDevice():
         return _NO_GUARD
     return torch.cuda.device(device)
 
@@ -92,7 +94,7 @@ def host_status(device):
     w = _host_status.get(idx)
     if w is None:
         t = torch.zeros(1, dtype=torch.int32).pin_memory()
-        w = _host_status[idx] = (t, ctypes.c_int32.from_address(t.data_ptr()), ctypes.c_void_p(t.data_ptr()))
+        w = _host_status[idx] = (t, ctypes.c_int32.from_address(t.data_ptr()), t.data_ptr())
     return w
 
 
@@ -136,21 +138,19 @@ def poll_status(device):
         idx = torch.cuda.current_device()
     p = _poll.get(idx)
     if p is None:
-        p = _poll[idx] = {"host": torch.zeros(1, dtype=torch.int32).pin_memory(), "event": None}
+        p = _poll[idx] = {"host": torch.zeros(1, dtype=torch.int32).pin_memory(), "event": torch.cuda.Event(), "pending": False}
     if torch.cuda.is_current_stream_capturing():
         return
-    ev = p["event"]
-    if ev is not None:
-        if not ev.query():
+    if p["pending"]:
+        if not p["event"].query():
             return
-        p["event"] = None
+        p["pending"] = False
         code = int(p["host"][0])
         if code != 0:
             status_word(device).zero_()
             _raise(code)
     p["host"].copy_(status_word(device), non_blocking=True)
-    ev = torch.cuda.Event()
-    ev.record(torch.cuda.current_stream(idx))
-    p["event"] = ev
+    p["event"].record(torch.cuda.current_stream(idx))
+    p["pending"] = True
 
 

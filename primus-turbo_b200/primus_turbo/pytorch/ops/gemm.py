@@ -92,11 +92,11 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     out_dtype = a.dtype if out_dtype is None else out_dtype
     assert out_dtype in (torch.bfloat16, torch.float16, torch.float32), f"gemm_bias_act: unsupported out_dtype {out_dtype}"
     if bias is not None:
-        assert tuple(bias.shape) == (N,) and bias.dtype in (a.dtype, torch.float32), f"gemm_bias_act: bias must be [{N}] in a's dtype or float32"
+        assert bias.shape == (N,) and bias.dtype in (a.dtype, torch.float32), f"gemm_bias_act: bias must be [{N}] in a's dtype or float32"
     if residual is not None:
-        assert tuple(residual.shape) == (M, N) and residual.dtype == out_dtype, f"gemm_bias_act: residual must be [{M}, {N}] in {out_dtype}"
+        assert residual.shape == (M, N) and residual.dtype == out_dtype, f"gemm_bias_act: residual must be [{M}, {N}] in {out_dtype}"
     tensors = [t for t in (a, b, bias, residual) if t is not None]
-    assert len({t.device for t in tensors}) == 1, "gemm_bias_act: all tensors must be on one device"
+    assert all(t.device == a.device for t in tensors), "gemm_bias_act: all tensors must be on one device"
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         return GemmBiasActFunction.apply(a, b, bias, residual, trans_b, activation, out_dtype, fuse_bgrad_accum_pattern)
     return gemm_bias_act_impl(a, b, trans_b, bias, activation, residual, out_dtype, False)[0]

@@ -23,7 +23,7 @@
 //            next product's operand type.
 //   DOWN     a CTA keeps one [128 features][tokens] accumulator over ALL chosen experts, one column per token, so the weighted
 //            sum over a token's experts happens in tensor memory.  For every expert only the 16-token blocks that hold one of
-//            its tokens are multiplied; the other tokens of such a block read a row of zeros.  Its first weight blocks are
+//            its tokens are multiplied; the other tokens of such a block are rows of zeros in shared memory.  Its first weight blocks are
 //            fetched before the first kernel has finished (programmatic dependent launch): weights and routing do not depend
 //            on it.
 #include <algorithm>
@@ -50,7 +50,7 @@ struct FewRowsArgs {
     int n, k;                // features of the output (GATE_UP: of one half), contraction length
     int split;               // CTAs of a cluster
     int fmt;                 // 0 = fp16, 1 = bf16 operands
-    void *out;               // LINEAR / DOWN [rows, n]; GATE_UP [slots + 1, n], the last row zeros
+    void *out;               // LINEAR / DOWN [rows, n]; GATE_UP [slots, n]
     int out_dtype;
     int act;
     // LINEAR
@@ -92,6 +92,9 @@ __global__ void __launch_bounds__(kFrThreads, 2)
     __shared__ int s_abort, s_count;
     __shared__ uint32_t s_bits[kMoe ? 32 : 1];
     __shared__ int16_t s_active[KIND == FR_DOWN ? kMaxGroups : 1];
+    constexpr int kRowWords = (TOK + 31) / 32;
+    __shared__ uint32_t s_held[KIND == FR_DOWN ? kStages : 1][kRowWords];   // DOWN: the rows of a stage that are not zero,
+    __shared__ int s_stage_expert[KIND == FR_DOWN ? kStages : 1];           // and the expert they belong to
     __shared__ int s_row[kMoe ? TOK : 1], s_slot[KIND == FR_GATE_UP ? TOK : 1];
     __shared__ float s_prob[KIND == FR_GATE_UP ? TOK : 1];
 
@@ -114,6 +117,19 @@ __global__ void __launch_bounds__(kFrThreads, 2)
     if (warp == 1) {
         tmem_alloc(&s_tmem, Cfg::kTmemCols);
         tmem_relinquish();
+    }
+    if (KIND == FR_LINEAR && threadIdx.x == 64 && blockIdx.y == 0) {
+        // The first weight blocks on their way into L2 while the kernel before this one finishes.  A prefetch is not a read: were the
+        // weight being written, L2 would hold the new values all the same.
+        const int chunks = (a.k + 63) / 64, l0 = chunks * rank / a.split, l1 = chunks * (rank + 1) / a.split;
+        for (int l = l0; l < min(l1, l0 + kStages); ++l) {
+            if (a.w_mn) {
+                prefetch_l2_2d(&tmap_w, tile * kFrFeat * 2, l * 64);
+                prefetch_l2_2d(&tmap_w, tile * kFrFeat * 2 + 128, l * 64);
+            } else {
+                prefetch_l2_2d(&tmap_w, l * 128, tile * kFrFeat);
+            }
+        }
     }
     if (KIND != FR_DOWN) {   // DOWN waits later: what it reads up to there is not written by the kernel before it
         grid_dep_wait();
@@ -177,6 +193,13 @@ __global__ void __launch_bounds__(kFrThreads, 2)
                 if (lane == 0) s_count = base;
             }
         } else {
+            for (int i = threadIdx.x; i < kStages * (Cfg::kBBytes / 16); i += kFrThreads)
+                *reinterpret_cast<uint4 *>(ring + (i / (Cfg::kBBytes / 16)) * Cfg::kStageBytes + kFrABytes + (i % (Cfg::kBBytes / 16)) * 16) = make_uint4(0, 0, 0, 0);
+            if (threadIdx.x < kStages) {
+                s_stage_expert[threadIdx.x] = -1;
+                for (int w = 0; w < kRowWords; ++w) s_held[threadIdx.x][w] = 0;
+            }
+            fence_proxy_async_smem();
             if (warp == 0) {
                 int at = excl;
                 for (uint32_t b = bits; b != 0; b &= b - 1) s_active[at++] = (int16_t) (lane * 32 + __ffs(b) - 1);
@@ -228,63 +251,101 @@ __global__ void __launch_bounds__(kFrThreads, 2)
                 }
             }
         } else {
-            // rows of the activations of every token for the expert at hand (the row of zeros for the others), in s_row
+            // s_row: the row of activations of every token for the expert at hand, -1 for tokens that did not choose it; rows: those that
+            // did, as bits.  A stage holds them at the tokens' places and zeros everywhere else: rows that an earlier expert left in
+            // the stage are cleared, the others are zero since the start.  (Loading a row of zeros instead cost more than the weights:
+            // every CTA fetched the same line of L2, 16 of them for each token of the block.)
             int cur = -1;
-            uint32_t mask = 0;
+            uint32_t rows[kRowWords] = {};
             auto set_expert = [&](int ai) {
                 if (ai == cur) return;
                 cur = ai;
                 const int e = s_active[ai];
-                mask = 0;
                 __syncwarp();
-                for (int t0 = 0; t0 < TOK; t0 += 32) {
-                    const int t = t0 + lane;
-                    int row = T * a.top_k;
+#pragma unroll
+                for (int w = 0; w < kRowWords; ++w) {
+                    const int t = 32 * w + lane;
+                    int row = -1;
                     if (t < T)
                         for (int j = a.top_k - 1; j >= 0; --j)
                             if (s_ids[t * a.top_k + j] == e) row = t * a.top_k + j;   // the first of them
-                    const uint32_t has = __ballot_sync(0xffffffffu, row != T * a.top_k);
+                    rows[w] = __ballot_sync(0xffffffffu, row >= 0);
                     if (t < TOK) s_row[t] = row;
-                    mask |= (uint32_t) ((has & 0xFFFFu) != 0) << (t0 / 16) | (uint32_t) ((has >> 16) != 0) << (t0 / 16 + 1);
                 }
                 __syncwarp();
             };
-            auto load_w = [&](int l, uint32_t stage) {
-                s_mask[stage] = mask;
-                mbar_arrive_expect_tx(&full_bar[stage], kFrABytes + __popc(mask) * 2048);
-                tma_load_2d_hint(ring + stage * Cfg::kStageBytes, &tmap_w, &full_bar[stage], (l % chunks) * 128, s_active[cur] * a.n + tile * kFrFeat, stream_pol);
-            };
-            auto load_x = [&](int l, uint32_t stage) {
+            auto clear_stale = [&](uint32_t stage) {   // by the whole warp, once the stage is free
                 uint8_t *B = ring + stage * Cfg::kStageBytes + kFrABytes;
-                for (uint32_t m = mask; m != 0; m &= m - 1) {
-                    const int blk = __ffs(m) - 1;
+                bool any = false;
 #pragma unroll
-                    for (int g = 4 * blk; g < 4 * blk + 4; ++g)
-                        tma_gather4(B + g * 512, &tmap_x, &full_bar[stage], (l % chunks) * 128, s_row[4 * g], s_row[4 * g + 1], s_row[4 * g + 2], s_row[4 * g + 3], keep_pol);
-                }
-            };
-            const int pre = min(kStages, l1 - l0);   // the ring is empty: these stages need no wait
-            for (int i = 0; i < pre; ++i) {
-                set_expert((l0 + i) / chunks);
-                if (lane == 0) load_w(l0 + i, i);
-            }
-            grid_dep_wait();
-            for (int i = 0; i < pre; ++i) {
-                set_expert((l0 + i) / chunks);
-                if (lane == 0) load_x(l0 + i, i);
-            }
-            uint32_t stage = pre == kStages ? 0 : pre, phase = pre == kStages ? 1 : 0;
-            for (int l = l0 + pre; l < l1; ++l) {
-                set_expert(l / chunks);
-                int good = 1;
-                if (lane == 0) {
-                    good = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag);
-                    if (good) {
-                        load_w(l, stage);
-                        load_x(l, stage);
+                for (int w = 0; w < kRowWords; ++w) {
+                    uint32_t stale = s_held[stage][w] & ~rows[w];
+                    any |= stale != 0;
+                    for (; stale != 0; stale &= stale - 1) {
+                        const int t = 32 * w + __ffs(stale) - 1;
+                        *reinterpret_cast<uint32_t *>(B + t * 128 + lane * 4) = 0u;
                     }
                 }
-                if (!(ok = __shfl_sync(0xffffffffu, good, 0) != 0)) break;
+                __syncwarp();
+                if (lane == 0) {
+                    s_stage_expert[stage] = cur;
+#pragma unroll
+                    for (int w = 0; w < kRowWords; ++w) s_held[stage][w] = rows[w];
+                }
+                if (any) fence_proxy_async_smem();
+                __syncwarp();
+            };
+            auto load_w = [&](int chunk, uint32_t stage) {
+                uint32_t blocks = 0;
+                int n = 0;
+#pragma unroll
+                for (int w = 0; w < kRowWords; ++w) {
+                    blocks |= (uint32_t) ((rows[w] & 0xFFFFu) != 0) << (2 * w) | (uint32_t) ((rows[w] >> 16) != 0) << (2 * w + 1);
+                    n += __popc(rows[w]);
+                }
+                s_mask[stage] = blocks;
+                mbar_arrive_expect_tx(&full_bar[stage], kFrABytes + n * 128);
+                tma_load_2d_hint(ring + stage * Cfg::kStageBytes, &tmap_w, &full_bar[stage], chunk * 128, s_active[cur] * a.n + tile * kFrFeat, stream_pol);
+            };
+            auto load_x = [&](int chunk, uint32_t stage) {
+                uint8_t *B = ring + stage * Cfg::kStageBytes + kFrABytes;
+                const int k0 = chunk * 128;
+#pragma unroll
+                for (int w = 0; w < kRowWords; ++w)
+                    for (uint32_t m = rows[w]; m != 0;) {
+                        const int b = __ffs(m) - 1, t = 32 * w + b;
+                        if ((b & 3) == 0 && (m >> b & 15) == 15) {
+                            tma_gather4(B + t * 128, &tmap_x, &full_bar[stage], k0, s_row[t], s_row[t + 1], s_row[t + 2], s_row[t + 3], keep_pol);
+                            m &= ~(15u << b);
+                        } else {
+                            tma_load_2d_hint(B + t * 128, &tmap_x, &full_bar[stage], k0, s_row[t], keep_pol);
+                            m &= m - 1;
+                        }
+                    }
+            };
+            const int pre = min(kStages, l1 - l0);   // the ring is empty: these stages need no wait
+            int ai = l0 / max(chunks, 1), c = l0 - ai * chunks;
+            auto advance = [&]() { if (++c == chunks) { c = 0; ++ai; } };
+            for (int i = 0; i < pre; ++i, advance()) {
+                set_expert(ai);
+                clear_stale(i);
+                if (lane == 0) load_w(c, i);
+            }
+            grid_dep_wait();
+            ai = l0 / max(chunks, 1); c = l0 - ai * chunks;
+            for (int i = 0; i < pre; ++i, advance()) {
+                set_expert(ai);
+                if (lane == 0) load_x(c, i);
+            }
+            uint32_t stage = pre == kStages ? 0 : pre, phase = pre == kStages ? 1 : 0;
+            for (int l = l0 + pre; l < l1; ++l, advance()) {
+                set_expert(ai);
+                if (!(ok = mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag))) break;
+                if (ai != s_stage_expert[stage]) clear_stale(stage);
+                if (lane == 0) {
+                    load_w(c, stage);
+                    load_x(c, stage);
+                }
                 if (++stage == kStages) { stage = 0; phase ^= 1; }
             }
         }
@@ -364,32 +425,41 @@ __global__ void __launch_bounds__(kFrThreads, 2)
     if constexpr (KIND == FR_DOWN) grid_dep_wait();
 
     // ================================================================ sum over the cluster, epilogue, write-out
-    // a warp takes one token at a time, a lane four neighbouring features
-    if constexpr (KIND == FR_GATE_UP) {
-        if (blockIdx.y == 0 && rank == 0 && warp == 0) {   // the row of zeros that DOWN reads for tokens of other experts
-            const int f = tile * 64 + 2 * lane;
-            if (f < a.n) *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.out) + (int64_t) T * a.top_k * a.n + f) = 0u;
+    // a warp takes one token at a time
+    const uint32_t part_addr = smem_u32(part);
+    // The features of a lane: four neighbours, accessed together; where a row of the output does not take that (ragged N), four that
+    // lie 32 apart, so that the warp's scalar accesses stay coalesced.  GATE_UP: two of the gate half and the same two of the up half.
+    const bool vec = KIND != FR_LINEAR || a.vec_ok;
+    const uint32_t lane_at = KIND == FR_GATE_UP ? lane * 8 : vec ? lane * 16 : lane * 4;
+    float bias[4] = {0.f, 0.f, 0.f, 0.f};
+    const int f0 = KIND == FR_GATE_UP ? tile * 64 + 2 * lane : tile * kFrFeat + (vec ? 4 * lane : lane);
+    if (KIND == FR_LINEAR && a.bias != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int f = vec ? f0 + i : f0 + 32 * i;
+            if (f < a.n) bias[i] = load_as_f32(a.bias, a.bias_dtype, f);
         }
     }
-    const uint32_t part_addr = smem_u32(part);
     for (int t = rank + a.split * warp; t < cnt; t += a.split * (kFrThreads / 32)) {
         float vv[1][4] = {{0.f, 0.f, 0.f, 0.f}};
         float(&v)[4] = vv[0];
-        // GATE_UP: features 2 lane, 2 lane + 1 of the gate half and of the up half
-        constexpr uint32_t kSecond = KIND == FR_GATE_UP ? 256 : 8;
-        const uint32_t at = part_addr + (uint32_t) t * (kFrFeat * 4) + lane * (KIND == FR_GATE_UP ? 8 : 16);
+        const uint32_t at = part_addr + (uint32_t) t * (kFrFeat * 4) + lane_at;
+        auto load = [&](uint32_t src, bool remote, float (&w)[4]) {
+            if (vec) {
+                ld_cluster_f32x2(src, remote, w[0], w[1]);
+                ld_cluster_f32x2(src + (KIND == FR_GATE_UP ? 256 : 8), remote, w[2], w[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = ld_cluster_f32(src + 128 * i, remote);
+            }
+        };
         if (a.split == 1) {
-            ld_cluster_f32x2(at, false, v[0], v[1]);
-            ld_cluster_f32x2(at + kSecond, false, v[2], v[3]);
+            load(at, false, v);
         } else {
             float w[kFrMaxSplit][4];   // all loads on their way before the first addition: one remote round trip, not one per CTA
 #pragma unroll
-            for (int s = 0; s < kFrMaxSplit; ++s) {
-                if (s >= a.split) continue;
-                const uint32_t src = map_addr_to_rank(at, s);
-                ld_cluster_f32x2(src, true, w[s][0], w[s][1]);
-                ld_cluster_f32x2(src + kSecond, true, w[s][2], w[s][3]);
-            }
+            for (int s = 0; s < kFrMaxSplit; ++s)
+                if (s < a.split) load(map_addr_to_rank(at, s), true, w[s]);
 #pragma unroll
             for (int s = 0; s < kFrMaxSplit; ++s)
                 if (s < a.split) {
@@ -398,46 +468,41 @@ __global__ void __launch_bounds__(kFrThreads, 2)
                 }
         }
         if constexpr (KIND == FR_GATE_UP) {
-            const int f = tile * 64 + 2 * lane;
             const float p = s_prob[t];
             const float h0 = act_any(a.act, v[0]) * v[2] * p, h1 = act_any(a.act, v[1]) * v[3] * p;
-            if (f < a.n)
-                *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.out) + (int64_t) s_slot[t] * a.n + f) =
+            if (f0 < a.n)
+                *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.out) + (int64_t) s_slot[t] * a.n + f0) =
                     a.fmt ? pack2<__nv_bfloat16>(h0, h1) : pack2<__half>(h0, h1);
+        } else if constexpr (KIND == FR_DOWN) {
+            if (f0 < a.n) store4_from_f32(a.out, a.out_dtype, (int64_t) t * a.n + f0, v);
         } else {
-            const int f = tile * kFrFeat + 4 * lane;
-            const int64_t row = KIND == FR_LINEAR ? (int64_t) blockIdx.y * TOK + t : t;
-            const int64_t o = row * a.n + f;
-            if constexpr (KIND == FR_LINEAR) {
-                const int zt = a.fmt ? PT_BF16 : PT_F16;
-                if (a.vec_ok && f < a.n) {
-                    float x[4];
-                    if (a.bias != nullptr) {
-                        load4_as_f32(a.bias, a.bias_dtype, f, x);
+            const int64_t o = ((int64_t) blockIdx.y * TOK + t) * a.n + f0;
+            const int zt = a.fmt ? PT_BF16 : PT_F16;
+            float res[4] = {0.f, 0.f, 0.f, 0.f};
+            if (a.residual != nullptr) {
+                if (vec && f0 < a.n) load4_as_f32(a.residual, a.out_dtype, o, res);
+                if (!vec) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] += x[i];
-                    }
-                    if (a.z != nullptr) store4_from_f32(a.z, zt, o, v);
-                    act_any_all<1>(a.act, vv);
-                    if (a.residual != nullptr) {
-                        load4_as_f32(a.residual, a.out_dtype, o, x);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] += x[i];
-                    }
-                    store4_from_f32(a.out, a.out_dtype, o, v);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (f + i >= a.n) continue;
-                        if (a.bias != nullptr) v[i] += load_as_f32(a.bias, a.bias_dtype, f + i);
-                        if (a.z != nullptr) store_from_f32(a.z, zt, o + i, v[i]);
-                        v[i] = act_any(a.act, v[i]);
-                        if (a.residual != nullptr) v[i] += load_as_f32(a.residual, a.out_dtype, o + i);
-                        store_from_f32(a.out, a.out_dtype, o + i, v[i]);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        if (f0 + 32 * i < a.n) res[i] = load_as_f32(a.residual, a.out_dtype, o + 32 * i);
                 }
-            } else {
-                if (f < a.n) store4_from_f32(a.out, a.out_dtype, o, v);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += bias[i];
+            if (a.z != nullptr && vec && f0 < a.n) store4_from_f32(a.z, zt, o, v);
+            if (a.z != nullptr && !vec) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (f0 + 32 * i < a.n) store_from_f32(a.z, zt, o + 32 * i, v[i]);
+            }
+            act_any_all<1>(a.act, vv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += res[i];
+            if (vec && f0 < a.n) store4_from_f32(a.out, a.out_dtype, o, v);
+            if (!vec) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (f0 + 32 * i < a.n) store_from_f32(a.out, a.out_dtype, o + 32 * i, v[i]);
             }
         }
     }
@@ -475,9 +540,31 @@ static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRows
     return PT_OK;
 }
 
-// CTAs per cluster: double while the grid would still be resident at once (two CTAs per SM) and each CTA keeps a ring's worth of
-// blocks.
-static int fr_split(int64_t tiles, int64_t chunks) {
+// Estimated time of the kernel in us, less a constant of about 7.  `tiles` weight blocks wide, `blocks` times over them (blocks of
+// tokens), `chunks` 64-wide steps of the contraction, s CTAs per cluster.  A CTA alone on its SM takes 0.30 + 0.0008 TOK us per step (its
+// ring holds about 100 KiB); together they cannot pull the weights faster than 6.5 TB/s out of memory, nor their stages faster than
+// 14 TB/s out of L2; a CTA more in the cluster lengthens the exchange of partial sums by 0.006 TOK us; CTAs beyond the two per SM that
+// are resident start late, about 6 us per wave.  Measured (us) with 1, 2, 4, 8 CTAs per cluster, K 4096: 1 x 4096 21.1, 13.3, 10.1, 10.5;
+// 1 x 14336 25.9, 24.3, 28.1, 34.6; 128 x 4096 34.7, 23.7, 17.4, 20.4; 333 x 4096 34.8, 26.7, 35.6, 52.2.
+static double fr_cost(int tok, int64_t tiles, int64_t blocks, int64_t chunks, int s) {
+    const double steps = (double) ceil_div(chunks, s) * (0.30 + 0.0008 * tok);
+    const double memory = (double) tiles * (double) chunks * kFrABytes / 6.5e6;
+    const double l2 = (double) tiles * (double) (blocks * chunks) * (kFrABytes + tok * 128) / 14e6;
+    const double waves = (double) (tiles * blocks * s) / (2.0 * sm_count());
+    return std::max(steps, std::max(memory, l2)) + 0.006 * tok * s + 6.0 * std::max(0.0, waves - 1.0);
+}
+// CTAs per cluster that make it smallest
+static int fr_split(int tok, int64_t tiles, int64_t blocks, int64_t chunks) {
+    int best = 1;
+    for (int s = 2; s <= kFrMaxSplit && tiles * blocks * s <= 2 * (int64_t) sm_count() && chunks >= 2 * s; s *= 2)
+        if (fr_cost(tok, tiles, blocks, chunks, s) < fr_cost(tok, tiles, blocks, chunks, best)) best = s;
+    return best;
+}
+
+// The same for the experts' kernels, whose producers also gather rows: one CTA per SM does not saturate the memory there (DOWN of seven
+// experts of 4096 x 14336 with 128 CTAs 245 us, with 256 126 us), so the split doubles while the grid stays resident and every CTA keeps
+// four steps.
+static int fr_split_experts(int64_t tiles, int64_t chunks) {
     int s = 1;
     while (s < kFrMaxSplit && tiles * s * 2 <= 2 * (int64_t) sm_count() && chunks / (s * 2) >= 4) s *= 2;
     return s;
@@ -494,6 +581,12 @@ static int fr_dispatch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRo
 }
 static int fr_tokens(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
+double few_rows_us(int64_t M, int64_t N, int64_t K) {
+    const int tok = fr_tokens(M);
+    const int64_t tiles = ceil_div(N, kFrFeat), blocks = ceil_div(M, tok), chunks = ceil_div(K, 64);
+    return 7.0 + fr_cost(tok, tiles, blocks, chunks, fr_split(tok, tiles, blocks, chunks));
+}
+
 // y = act(a . b^T + bias) + residual for few rows of a
 int few_rows_linear(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
                     void *z, int act, int64_t M, int64_t N, int64_t K, int *status, cudaStream_t st) {
@@ -508,7 +601,7 @@ int few_rows_linear(const void *a, const void *b, int b_mn, int ab_dtype, const 
     const int esize = c_dtype == PT_F32 ? 4 : 2;
     r.vec_ok = N % 4 == 0 && aligned(c, 4 * esize) && aligned(residual, 4 * esize) && aligned(z, 8) && aligned(bias, bias_dtype == PT_F32 ? 16 : 8);
     const int64_t tiles = ceil_div(N, kFrFeat), grid_y = ceil_div(M, tok);
-    r.split = fr_split(tiles * grid_y, ceil_div(K, 64));
+    r.split = fr_split(tok, tiles, grid_y, ceil_div(K, 64));
     return fr_dispatch<FR_LINEAR>(tw, tx, r, tok, tiles, grid_y, st);
 }
 
@@ -520,7 +613,7 @@ extern "C" {
 
 size_t pt_moe_few_tokens_scratch_bytes(int64_t T, int top_k, int64_t I) {
     if (T <= 0 || top_k <= 0 || I <= 0) return 0;
-    return (size_t) ((T * top_k + 1) * I * 2);
+    return (size_t) (T * top_k * I * 2);
 }
 
 int pt_moe_few_tokens(const void *x, const void *gate_up, const void *down, int dtype, const void *ids, int id_bytes, const float *probs, int64_t T,
@@ -552,13 +645,13 @@ int pt_moe_few_tokens(const void *x, const void *gate_up, const void *down, int 
     if ((rc = make_tmap_bytes(&tx, x, T, 2 * H, 2 * H, 1)) != PT_OK) return rc;
     a.n = (int) I; a.k = (int) H; a.out = scratch;
     int64_t tiles = ceil_div(I, 64);
-    a.split = fr_split(tiles * most, ceil_div(H, 64));
+    a.split = fr_split_experts(tiles * most, ceil_div(H, 64));
     if ((rc = fr_dispatch<FR_GATE_UP>(tw, tx, a, tok, tiles, most, st)) != PT_OK) return rc;
     if ((rc = make_tmap_bytes(&tw, down, (int64_t) E * H, 2 * I, 2 * I, kFrFeat)) != PT_OK) return rc;
-    if ((rc = make_tmap_bytes(&tx, scratch, slots + 1, 2 * I, 2 * I, 1)) != PT_OK) return rc;
+    if ((rc = make_tmap_bytes(&tx, scratch, slots, 2 * I, 2 * I, 1)) != PT_OK) return rc;
     a.n = (int) H; a.k = (int) I; a.out = out;
     tiles = ceil_div(H, kFrFeat);
-    a.split = fr_split(tiles, std::min<int64_t>(most, T) * ceil_div(I, 64));
+    a.split = fr_split_experts(tiles, most * ceil_div(I, 64));
     return fr_dispatch<FR_DOWN>(tw, tx, a, tok, tiles, 1, st);
 }
 

@@ -102,6 +102,7 @@ __device__ __forceinline__ void store4_from_f32(void *p, int dtype, int64_t i, c
 // few_rows.cu: y = act(a . b^T + bias) + residual for few rows of a
 int few_rows_linear(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
                     void *z, int act, int64_t M, int64_t N, int64_t K, int *status, cudaStream_t st);
+double few_rows_us(int64_t M, int64_t N, int64_t K);   // its estimated time
 
 inline int raster_rows(int64_t a_rows, int64_t k_bytes) {
     if (const char *e = getenv("PT_GEMM_RASTER_M")) {   // row blocks (of 128 rows) per band, for experiments

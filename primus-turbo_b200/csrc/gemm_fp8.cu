@@ -31,8 +31,6 @@
 namespace ptb {
 using namespace sm100;
 
-constexpr int kNumEpiWarps = 4;
-constexpr int kGemmThreads = 32 * (2 + kNumEpiWarps);
 constexpr int kEpiWarp0 = 2;
 constexpr int kStagePitchMax = 128;  // staging row pitch (bytes) of the epilogue, fp32 worst case
 
@@ -82,7 +80,11 @@ template <int MODE> struct MnBox {
 
 // F4: packed e2m1 operands.  A 128-byte stage row then holds 256 elements = two 128-element scale blocks, so every
 // scale quantity per stage doubles (kSfPerStage) and one tcgen05.mma consumes 64 elements with two scales per row.
-template <int BLOCK_N, bool MX, bool F4 = false> struct GemmCfg {
+// EPI (GEMM_HP_EPI): two epilogue warps per quarter of the accumulator's rows, each taking half of its columns, and one group only.
+template <int BLOCK_N, bool MX, bool F4 = false, bool EPI = false> struct GemmCfg {
+    static constexpr int kEpiWarps = EPI ? 8 : 4;
+    static constexpr int kThreads = 32 * (2 + kEpiWarps);
+    static constexpr int kGroups = EPI ? 1 : kMaxGroups;
     static constexpr int kSfbBlocks = (BLOCK_N + 127) / 128;
     static constexpr int kSfPerStage = F4 ? 2 : 1;
     static constexpr int kSfColsHalf = 4 + 4 * kSfbBlocks;          // SFA block + SFB blocks of one 128-element scale block
@@ -96,9 +98,9 @@ template <int BLOCK_N, bool MX, bool F4 = false> struct GemmCfg {
     static constexpr int kBBytes = BLOCK_N * BLOCK_K;
     static constexpr int kSfBytes = MX ? 512 * (1 + kSfbBlocks) * kSfPerStage : 0;
     static constexpr int kStageBytes = kABytes + kBBytes + kSfBytes;
-    static constexpr int kEpiBytes = kNumEpiWarps * 32 * kStagePitchMax;
+    static constexpr int kEpiBytes = kEpiWarps * 32 * kStagePitchMax;
     static constexpr int kBarBytes = 1024;
-    static constexpr int kSmemBudget = 227 * 1024 - 1024 /* alignment slack */ - 4608 /* static shared: tile table */;
+    static constexpr int kSmemBudget = 227 * 1024 - 1024 /* alignment slack */ - (EPI ? 64 : 4608) /* static shared: tile table */;
     static constexpr int kStages = std::min(8, (kSmemBudget - kEpiBytes - kBarBytes) / kStageBytes);
     static constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + kBarBytes + 1024;
     static_assert(kStages >= 3, "not enough shared memory for a 3-stage ring");
@@ -394,11 +396,11 @@ __device__ __forceinline__ void epilogue_fused_block(const GemmParams &p, uint32
 }
 
 template <int BLOCK_N, int MODE>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__((GemmCfg<BLOCK_N, mode_is_mx(MODE), MODE == GEMM_MXF4, MODE == GEMM_HP_EPI>::kThreads), 1)
     gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, GemmParams p) {
     constexpr bool MX = mode_is_mx(MODE);
     constexpr bool F4 = MODE == GEMM_MXF4;
-    using Cfg = GemmCfg<BLOCK_N, MX, F4>;
+    using Cfg = GemmCfg<BLOCK_N, MX, F4, MODE == GEMM_HP_EPI>;
     using Mn = MnBox<MODE>;
     constexpr int kSfP = Cfg::kSfPerStage;
     constexpr int kStages = Cfg::kStages;
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     uint64_t *tmem_empty_bar = tmem_full_bar + kAccStages;
     uint32_t *tmem_base_slot = reinterpret_cast<uint32_t *>(tmem_empty_bar + kAccStages);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_base_slot + 1);
-    __shared__ int s_tile_start[kMaxGroups + 1];
+    __shared__ int s_tile_start[Cfg::kGroups + 1];
 
     const int warp = threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         for (int s = 0; s < kAccStages; ++s) {
             mbar_init(&tmem_full_bar[s], 1);
-            mbar_init(&tmem_empty_bar[s], kNumEpiWarps);
+            mbar_init(&tmem_empty_bar[s], Cfg::kEpiWarps);
         }
         fence_barrier_init();
         prefetch_tmap(&tmap_a);
@@ -605,7 +607,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const uint32_t taddr = tmem_base + ((uint32_t) (q * 32) << 16) + acc_stage * BLOCK_N;
             auto release = [&]() { mbar_arrive(&tmem_empty_bar[acc_stage]); };
             if constexpr (MODE == GEMM_HP_EPI)
-                epilogue_fused_block<BLOCK_N>(p, taddr, have_acc, tile_row0, c_row_end, n0, stg, lane, 0, (BLOCK_N + 31) / 32, release);
+                {
+                constexpr int kChunks = (BLOCK_N + 31) / 32;
+                const int half = (warp - kEpiWarp0) >> 2;
+                epilogue_fused_block<BLOCK_N>(p, taddr, have_acc, tile_row0, c_row_end, n0, stg, lane, half ? kChunks / 2 : 0, half ? kChunks : kChunks / 2, release);
+            }
             else
                 epilogue_store_block<BLOCK_N, MODE>(p, taddr, have_acc, tile_row0, c_row_end, n0, gi, stg, lane, 0, (BLOCK_N + 31) / 32, release);
             if (have_acc && ++acc_stage == kAccStages) { acc_stage = 0; acc_phase ^= 1; }
@@ -685,7 +691,7 @@ template <int MODE> static int make_tmap_mn(CUtensorMap *m, const void *base, in
 template <int BLOCK_N, int MODE>
 static int launch_gemm(const void *a, int64_t a_rows, const void *b, int64_t b_rows, GemmParams p, const MxScales &mx,
                        int max_ctas, int64_t max_tiles, cudaStream_t st) {
-    using Cfg = GemmCfg<BLOCK_N, mode_is_mx(MODE), MODE == GEMM_MXF4>;
+    using Cfg = GemmCfg<BLOCK_N, mode_is_mx(MODE), MODE == GEMM_MXF4, MODE == GEMM_HP_EPI>;
     if constexpr (mode_is_mx(MODE)) {
         int rc0 = prepare_mx_scales(p, mx, a_rows, b_rows, BLOCK_N, Cfg::kSfbBlocks, Cfg::kSfPerStage, st);
         if (rc0 != PT_OK) return rc0;
@@ -705,7 +711,7 @@ static int launch_gemm(const void *a, int64_t a_rows, const void *b, int64_t b_r
     int grid = (int) std::min<int64_t>(max_tiles, sm_count());
     if (max_ctas > 0) grid = std::min(grid, max_ctas);
     if (grid <= 0) return PT_OK;
-    PT_CUDA_OK(launch_overlapped(kern, dim3(grid), dim3(kGemmThreads), Cfg::kSmemBytes, st, ta, tb, p));
+    PT_CUDA_OK(launch_overlapped(kern, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmemBytes, st, ta, tb, p));
     return PT_OK;
 }
 
@@ -785,8 +791,11 @@ static int dispatch_block_n(int block_n, const void *a, int64_t a_rows, const vo
         const int64_t rows_per_group = p.koffs ? p.M : p.M / p.G;
         const int64_t out_elems = (p.koffs ? (int64_t) p.G : 1) * p.M * (int64_t) p.N;
         const bool grouped = p.offs_write != nullptr && !p.koffs;
-        if (block_n == 0 && max_ctas <= 0 && pair_enabled() && !g_pair_refused[current_device_slot()] && rows_per_group >= 1024 && p.N >= 512 &&
-            out_elems >= (int64_t) 4096 * 4096 && (!mode_is_mx(MODE) || aligned(mx.workspace, 128))) {
+        // HP_EPI comes here with more rows than few_rows.cu takes, and its pairs are faster from the first tile on (512 x 4096 x 4096: 32.0
+        // against 35.9 us, 2048 x 14336 x 4096: 167.2 / 167.5).
+        const bool large = rows_per_group >= 1024 && out_elems >= (int64_t) 4096 * 4096;
+        if (block_n == 0 && max_ctas <= 0 && pair_enabled() && !g_pair_refused[current_device_slot()] && (large || MODE == GEMM_HP_EPI) && p.N >= 512 &&
+            (!mode_is_mx(MODE) || aligned(mx.workspace, 128))) {
             if constexpr (mode_is_mx(MODE)) {
                 constexpr int kSfP = MODE == GEMM_MXF4 ? 2 : 1;
                 if (mx.workspace_bytes >= mx_workspace_bytes(p.M, p.N, p.K, p.koffs ? 1 : p.G, grouped, 224) * kSfP) {
@@ -903,8 +912,15 @@ int gemm_hp_host(const void *a, const void *b, int ab_dtype, void *c, int c_dtyp
     return dispatch_block_n<GEMM_HP>(0, a, a_rows_total, b, b_rows, p, mx, max_ctas, (cudaStream_t) stream);
 }
 
-// Up to this many rows the product runs on the weight-streaming kernels of few_rows.cu, from there on on the tiles above.
-static bool few_rows_better(int64_t M, int64_t N, int64_t K) { return M <= 128; }
+// Which kernels a product runs on: the weight-streaming ones of few_rows.cu or the tiles above (CTA pairs), whichever the estimate
+// makes faster.  The pairs take about 14 us and, per wave of 256 x 256 tiles, 4.35 us per 1024 of K plus 3 us of epilogue between waves.
+// Measured (us, SiLU epilogue) few rows / pairs: 129 x 4096 x 4096 (M, N, K) 20.0 / 31.7, 512 x 4096 x 4096 27.4 / 32.0, 768 x 4096 x 4096
+// 39.8 / 33.4; 129 x 14336 x 4096 41.2 / 37.5; 333 x 4096 x 14336 61.3 / 83.9, 768 x 4096 x 14336 115.8 / 82.7; 2048 x 1024 x 4096 26.7 / 31.2.
+static bool few_rows_better(int64_t M, int64_t N, int64_t K) {
+    if (M <= 64) return true;
+    const int64_t waves = ceil_div(ceil_div(M, 256) * ceil_div(N, 256), sm_count() / 2);
+    return few_rows_us(M, N, K) < 11.0 + (double) waves * (3.0 + 4.35 * (double) K / 1024.0);
+}
 
 static int gemm_bias_act_host(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
                               void *z, int act, int64_t M, int64_t N, int64_t K, int *status, cudaStream_t st) {

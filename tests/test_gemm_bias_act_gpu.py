@@ -36,6 +36,12 @@ def _assert_within(got, want, tol, what):
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} outside, worst {float((err / tol).max()):.2f} x tolerance"
 
 
+def _few(M, N, K):
+    """Whether the rule sends this size to the few-row kernels."""
+    from primus_turbo.pytorch.kernels import _native as nv
+    return bool(nv.lib().pt_gemm_bias_act_few_rows(M, N, (K + 7) // 8 * 8))
+
+
 def _check(M, N, K, dt, act, with_bias, with_res, trans_b=True, out_dtype=None, bias_dtype=None, grad=False, seed=0, a=None):
     from primus_turbo.pytorch.kernels import _native as nv
     from primus_turbo.pytorch.ops import gemm_bias_act
@@ -89,21 +95,26 @@ ACTS = [None, "relu", "silu", "gelu", "gelu_tanh"]
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("M,N,K", [(1, 128, 64), (1, 1, 8), (2, 129, 72), (3, 1000, 512), (7, 256, 4096), (16, 4101, 1024), (17, 64, 2048),
-                                   (31, 333, 264), (32, 128, 128), (33, 640, 136), (64, 257, 320), (65, 96, 1096), (100, 2049, 64), (128, 130, 512)])
+                                   (31, 333, 264), (32, 128, 128), (33, 640, 136), (64, 257, 320), (65, 96, 1096), (100, 2049, 64), (128, 130, 512), (129, 128, 64), (200, 257, 520), (300, 1001, 72),
+                                   (513, 512, 1024), (1030, 4, 16), (777, 1028, 256), (2000, 130, 1024), (40000, 8, 72)])
 def test_few_rows(dt, M, N, K):
+    assert _few(M, N, K)
     for i, act in enumerate(ACTS):
         _check(M, N, K, dt, act, with_bias=i % 2 == 0, with_res=i % 3 != 1, seed=10 * i)
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("M,N,K", [(129, 128, 64), (200, 257, 520), (300, 1001, 72), (513, 512, 1024), (1030, 4, 16), (777, 1028, 256)])
+@pytest.mark.parametrize("M,N,K", [(33000, 130, 1032), (20001, 257, 2048), (9000, 1001, 1000)])
 def test_tiles(dt, M, N, K):
+    """Enough tiles for the tile kernels: single CTAs below 512 columns, CTA pairs from there on."""
+    assert not _few(M, N, K)
     for i, act in enumerate(ACTS):
         _check(M, N, K, dt, act, with_bias=i % 2 == 0, with_res=i % 3 != 1, seed=10 * i)
 
 
 @pytest.mark.parametrize("M,N,K,act", [(4100, 4104, 192, "gelu"), (4097, 4101, 64, "silu"), (8192, 4096, 64, None)])
 def test_cta_pairs(M, N, K, act):
+    assert not _few(M, N, K)
     _check(M, N, K, torch.bfloat16, act, True, True)
 
 

@@ -169,4 +169,4 @@ def test_moe_few_tokens_abi_refusals():
                     (dict(act=2), b"activation"), (dict(I=1 << 21, E=1024), b"32-bit"), (dict(), b"null")):
         assert call(**kw) == -1 and msg in lib.pt_last_error(), kw
     assert call(T=0) == 0
-    assert lib.pt_moe_few_tokens_scratch_bytes(3, 2, 16) == 7 * 32
+    assert lib.pt_moe_few_tokens_scratch_bytes(3, 2, 16) == 6 * 32

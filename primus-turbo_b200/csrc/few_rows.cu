@@ -14,7 +14,7 @@
 //
 //   warp 0      producer (TMA; for experts also the lists of the tokens that chose them)
 //   warp 1      one thread issues the MMAs; owns the tensor memory
-//   warps 2-5   tensor memory -> shared memory; then all warps reduce and write out
+//   the others  tensor memory -> shared memory; then all warps reduce and write out
 //
 // Mixture, two kernels:
 //   GATE_UP  grid (blocks of 64 features x split, chosen experts): the block is 64 gate rows and the 64 up rows that belong to them.
@@ -36,7 +36,6 @@
 namespace ptb {
 using namespace sm100;
 
-constexpr int kFrThreads = 192;
 constexpr int kFrFeat = 128;              // features (weight rows) of a CTA
 constexpr int kFrABytes = kFrFeat * 128;  // a weight block: 128 rows of 64 16-bit elements
 constexpr int kFrMaxSlots = 2048;         // tokens x experts per token
@@ -67,19 +66,22 @@ struct FewRowsArgs {
 };
 
 template <int TOK> struct FrCfg {
+    static constexpr int kEpiWarps = TOK <= 32 ? 4 : 8;   // per quarter of the accumulator's rows: one, or two that share the tokens
+    static constexpr int kThreads = 64 + 32 * kEpiWarps;
     static constexpr int kBBytes = TOK * 128;
     static constexpr int kStageBytes = kFrABytes + kBBytes;
-    static constexpr int kStages = TOK <= 16 ? 6 : TOK <= 32 ? 5 : TOK <= 64 ? 4 : 3;   // two CTAs per SM
+    static constexpr int kCtas = TOK <= 128 ? 2 : 1;   // per SM
+    static constexpr int kStages = TOK <= 16 ? 6 : TOK <= 32 ? 5 : TOK <= 64 ? 4 : TOK <= 128 ? 3 : TOK <= 192 ? 5 : 4;
     static constexpr int kRing = kStages * kStageBytes;
     static constexpr int kIdSlots = TOK * kFrMaxTopK < kFrMaxSlots ? TOK * kFrMaxTopK : kFrMaxSlots;
     static constexpr int kSmem = kRing + 1024 /* alignment */ + 2 * kIdSlots;
-    static constexpr int kTmemCols = TOK < 32 ? 32 : TOK;
+    static constexpr int kTmemCols = TOK < 32 ? 32 : TOK > 128 ? 256 : TOK;
     static_assert(TOK * kFrFeat * 4 <= kRing, "the partial block must fit the ring");
-    static_assert(2 * (kSmem + 3584 /* static and reserved */) <= 228 * 1024, "two CTAs per SM");
+    static_assert(kCtas * (kSmem + 3584 /* static and reserved */) <= 228 * 1024, "CTAs per SM");
 };
 
 template <int TOK, int KIND>
-__global__ void __launch_bounds__(kFrThreads, 2)
+__global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
     few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, FewRowsArgs a) {
     using Cfg = FrCfg<TOK>;
     constexpr int kStages = Cfg::kStages;
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(kFrThreads, 2)
     if constexpr (kMoe) {
         if (threadIdx.x < 32) s_bits[threadIdx.x] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < T * a.top_k; i += kFrThreads) {
+        for (int i = threadIdx.x; i < T * a.top_k; i += Cfg::kThreads) {
             const int64_t id = a.id_bytes == 8 ? reinterpret_cast<const int64_t *>(a.ids)[i] : (int64_t) reinterpret_cast<const int *>(a.ids)[i];
             const bool valid = id >= 0 && id < a.experts;
             s_ids[i] = valid ? (int16_t) id : (int16_t) -1;
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(kFrThreads, 2)
                 if (lane == 0) s_count = base;
             }
         } else {
-            for (int i = threadIdx.x; i < kStages * (Cfg::kBBytes / 16); i += kFrThreads)
+            for (int i = threadIdx.x; i < kStages * (Cfg::kBBytes / 16); i += Cfg::kThreads)
                 *reinterpret_cast<uint4 *>(ring + (i / (Cfg::kBBytes / 16)) * Cfg::kStageBytes + kFrABytes + (i % (Cfg::kBBytes / 16)) * 16) = make_uint4(0, 0, 0, 0);
             if (threadIdx.x < kStages) {
                 s_stage_expert[threadIdx.x] = -1;
@@ -397,17 +399,21 @@ __global__ void __launch_bounds__(kFrThreads, 2)
         ok = mbar_wait_warp(&done_bar, 0, abort_flag);
         tc_fence_after_sync();
         const uint32_t touched = ok ? s_touched : 0;
-        for (int b = 0; b < blocks; ++b) {
-            uint32_t r[16];
-            if (touched >> b & 1) {
-                tmem_ld16(tmem + ((uint32_t) (q * 32) << 16) + 16 * b, r);
-                tmem_ld_wait();
-            } else {
+        // Two blocks of 16 tokens at a time, both loads in flight.  They are made whether or not the columns hold sums (a pair never
+        // reaches past the allocation): between a load and its wait nothing may touch the registers, a branch's merge neither.
+        for (int b = 2 * ((warp - 2) >> 2); b < blocks; b += Cfg::kEpiWarps / 2) {
+            uint32_t r[2][16];
+            const uint32_t at = tmem + ((uint32_t) (q * 32) << 16) + 16 * b;
+            tmem_ld16(at, r[0]);
+            tmem_ld16(at + 16, r[1]);
+            tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) r[i] = 0u;
+            for (int h = 0; h < 2; ++h) {
+                if (b + h >= blocks) continue;
+                const bool have = touched >> (b + h) & 1;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) part[(16 * (b + h) + i) * kFrFeat + q * 32 + lane] = have ? __uint_as_float(r[h][i]) : 0.f;
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) part[(16 * b + i) * kFrFeat + q * 32 + lane] = __uint_as_float(r[i]);
         }
     }
     if (!ok || s_abort) {
@@ -425,7 +431,6 @@ __global__ void __launch_bounds__(kFrThreads, 2)
     if constexpr (KIND == FR_DOWN) grid_dep_wait();
 
     // ================================================================ sum over the cluster, epilogue, write-out
-    // a warp takes one token at a time
     const uint32_t part_addr = smem_u32(part);
     // The features of a lane: four neighbours, accessed together; where a row of the output does not take that (ragged N), four that
     // lie 32 apart, so that the warp's scalar accesses stay coalesced.  GATE_UP: two of the gate half and the same two of the up half.
@@ -440,10 +445,12 @@ __global__ void __launch_bounds__(kFrThreads, 2)
             if (f < a.n) bias[i] = load_as_f32(a.bias, a.bias_dtype, f);
         }
     }
-    for (int t = rank + a.split * warp; t < cnt; t += a.split * (kFrThreads / 32)) {
-        float vv[1][4] = {{0.f, 0.f, 0.f, 0.f}};
-        float(&v)[4] = vv[0];
-        const uint32_t at = part_addr + (uint32_t) t * (kFrFeat * 4) + lane_at;
+    // A warp takes a token or two at once, the loads of several CTAs' blocks on their way before the first addition: one remote round trip
+    // for all of them.  The sums run in the order of the ranks.
+    constexpr int kAtOnce = TOK <= 16 ? 1 : 2;
+    const int step = a.split * (Cfg::kThreads / 32);   // tokens between two of this warp's
+    for (int t0 = rank + a.split * warp; t0 < cnt; t0 += kAtOnce * step) {
+        float v[kAtOnce][4];
         auto load = [&](uint32_t src, bool remote, float (&w)[4]) {
             if (vec) {
                 ld_cluster_f32x2(src, remote, w[0], w[1]);
@@ -453,56 +460,97 @@ __global__ void __launch_bounds__(kFrThreads, 2)
                 for (int i = 0; i < 4; ++i) w[i] = ld_cluster_f32(src + 128 * i, remote);
             }
         };
+        auto inside = [&](int u) { return u == 0 || t0 + u * step < cnt; };
+        auto row_at = [&](int u) { return part_addr + (uint32_t) (t0 + u * step) * (kFrFeat * 4) + lane_at; };
         if (a.split == 1) {
-            load(at, false, v);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (inside(u)) load(row_at(u), false, v[u]);
         } else {
-            float w[kFrMaxSplit][4];   // all loads on their way before the first addition: one remote round trip, not one per CTA
+            constexpr int kRanks = kAtOnce == 1 ? kFrMaxSplit : kFrMaxSplit / 2;
 #pragma unroll
-            for (int s = 0; s < kFrMaxSplit; ++s)
-                if (s < a.split) load(map_addr_to_rank(at, s), true, w[s]);
+            for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
-            for (int s = 0; s < kFrMaxSplit; ++s)
-                if (s < a.split) {
+                for (int i = 0; i < 4; ++i) v[u][i] = 0.f;
+            for (int s0 = 0; s0 < a.split; s0 += kRanks) {
+                float w[kRanks][kAtOnce][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] += w[s][i];
-                }
+                for (int s = 0; s < kRanks; ++s)
+                    if (s0 + s < a.split) {
+#pragma unroll
+                        for (int u = 0; u < kAtOnce; ++u)
+                            if (inside(u)) load(map_addr_to_rank(row_at(u), s0 + s), true, w[s][u]);
+                    }
+#pragma unroll
+                for (int s = 0; s < kRanks; ++s)
+                    if (s0 + s < a.split) {
+#pragma unroll
+                        for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[u][i] += w[s][u][i];
+                    }
+            }
         }
         if constexpr (KIND == FR_GATE_UP) {
-            const float p = s_prob[t];
-            const float h0 = act_any(a.act, v[0]) * v[2] * p, h1 = act_any(a.act, v[1]) * v[3] * p;
-            if (f0 < a.n)
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int t = t0 + u * step;
+                if (!inside(u) || f0 >= a.n) continue;
+                const float p = s_prob[t];
+                const float h0 = act_any(a.act, v[u][0]) * v[u][2] * p, h1 = act_any(a.act, v[u][1]) * v[u][3] * p;
                 *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.out) + (int64_t) s_slot[t] * a.n + f0) =
                     a.fmt ? pack2<__nv_bfloat16>(h0, h1) : pack2<__half>(h0, h1);
+            }
         } else if constexpr (KIND == FR_DOWN) {
-            if (f0 < a.n) store4_from_f32(a.out, a.out_dtype, (int64_t) t * a.n + f0, v);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int t = t0 + u * step;
+                if (inside(u) && f0 < a.n) store4_from_f32(a.out, a.out_dtype, (int64_t) t * a.n + f0, v[u]);
+            }
         } else {
-            const int64_t o = ((int64_t) blockIdx.y * TOK + t) * a.n + f0;
+            const int64_t o0 = ((int64_t) blockIdx.y * TOK + t0) * a.n + f0, o_step = (int64_t) step * a.n;
             const int zt = a.fmt ? PT_BF16 : PT_F16;
-            float res[4] = {0.f, 0.f, 0.f, 0.f};
-            if (a.residual != nullptr) {
-                if (vec && f0 < a.n) load4_as_f32(a.residual, a.out_dtype, o, res);
-                if (!vec) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (f0 + 32 * i < a.n) res[i] = load_as_f32(a.residual, a.out_dtype, o + 32 * i);
+            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[u][i] += bias[i];
+            if (vec) {
+                if (f0 >= a.n) continue;
+                uint4 res[kAtOnce];
+                if (a.residual != nullptr) {
+#pragma unroll
+                    for (int u = 0; u < kAtOnce; ++u)
+                        if (inside(u)) res[u] = load4_raw(a.residual, a.out_dtype, o0 + u * o_step);
                 }
-            }
+                if (a.z != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += bias[i];
-            if (a.z != nullptr && vec && f0 < a.n) store4_from_f32(a.z, zt, o, v);
-            if (a.z != nullptr && !vec) {
+                    for (int u = 0; u < kAtOnce; ++u)
+                        if (inside(u)) store4_from_f32(a.z, zt, o0 + u * o_step, v[u]);
+                }
+                act_any_all<kAtOnce>(a.act, v);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (f0 + 32 * i < a.n) store_from_f32(a.z, zt, o + 32 * i, v[i]);
-            }
-            act_any_all<1>(a.act, vv);
+                for (int u = 0; u < kAtOnce; ++u) {
+                    if (!inside(u)) continue;
+                    if (a.residual != nullptr) {
+                        float x[4];
+                        raw4_as_f32(res[u], a.out_dtype, x);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += res[i];
-            if (vec && f0 < a.n) store4_from_f32(a.out, a.out_dtype, o, v);
-            if (!vec) {
+                        for (int i = 0; i < 4; ++i) v[u][i] += x[i];
+                    }
+                    store4_from_f32(a.out, a.out_dtype, o0 + u * o_step, v[u]);
+                }
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (f0 + 32 * i < a.n) store_from_f32(a.out, a.out_dtype, o + 32 * i, v[i]);
+                for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (!inside(u) || f0 + 32 * i >= a.n) continue;
+                        const int64_t o = o0 + u * o_step + 32 * i;
+                        if (a.z != nullptr) store_from_f32(a.z, zt, o, v[u][i]);
+                        float y = act_any(a.act, v[u][i]);
+                        if (a.residual != nullptr) y += load_as_f32(a.residual, a.out_dtype, o);
+                        store_from_f32(a.out, a.out_dtype, o, y);
+                    }
             }
         }
     }
@@ -526,7 +574,7 @@ static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRows
     PT_REQUIRE(tiles * a.split < (1ll << 31) && grid_y < 65536, "few-row product: grid too large");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) (tiles * a.split), (unsigned) grid_y);
-    cfg.blockDim = dim3(kFrThreads);
+    cfg.blockDim = dim3(Cfg::kThreads);
     cfg.dynamicSmemBytes = Cfg::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -540,28 +588,38 @@ static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRows
     return PT_OK;
 }
 
-// Estimated time of the kernel in us, less a constant of about 7.  `tiles` weight blocks wide, `blocks` times over them (blocks of
-// tokens), `chunks` 64-wide steps of the contraction, s CTAs per cluster.  A CTA alone on its SM takes 0.30 + 0.0008 TOK us per step (its
-// ring holds about 100 KiB); together they cannot pull the weights faster than 6.5 TB/s out of memory, nor their stages faster than
-// 14 TB/s out of L2; a CTA more in the cluster lengthens the exchange of partial sums by 0.006 TOK us; CTAs beyond the two per SM that
-// are resident start late, about 6 us per wave.  Measured (us) with 1, 2, 4, 8 CTAs per cluster, K 4096: 1 x 4096 21.1, 13.3, 10.1, 10.5;
-// 1 x 14336 25.9, 24.3, 28.1, 34.6; 128 x 4096 34.7, 23.7, 17.4, 20.4; 333 x 4096 34.8, 26.7, 35.6, 52.2.
+// Estimated time of a launch in us: `tiles` weight blocks wide, `blocks` times over them (blocks of `tok` tokens), `chunks` 64-wide steps of
+// the contraction, s CTAs per cluster.  4.5 us of launch, first bytes and write-out; the exchange of partial sums, longer with every CTA of
+// the cluster; and the longest of: a CTA's own steps, the weights out of memory (one 100 KiB ring per SM does not quite saturate it),
+// all stages out of L2 (13 TB/s).  CTAs beyond those resident at once start late, about 6 us per wave.  Measured against estimated (us):
+// 1 x 4096 x 14336 (rows, features, K), s = 1, 4, 8: 65.5 / 67, 24.6 / 25.3, 21.6 / 23.6; 64 x 4096 x 4096, s = 1, 2, 4, 8: 25.7 / 26.6, 17.0 /
+// 17.1, 13.8 / 14.3, 16.3 / 17.7; 333 x 4096 x 4096, 128 / 192 / 256 tokens per block and s = 2: 25.2 / 24.1, 21.3 / 20.3, 25.4 / 23.9.
 static double fr_cost(int tok, int64_t tiles, int64_t blocks, int64_t chunks, int s) {
-    const double steps = (double) ceil_div(chunks, s) * (0.30 + 0.0008 * tok);
-    const double memory = (double) tiles * (double) chunks * kFrABytes / 6.5e6;
-    const double l2 = (double) tiles * (double) (blocks * chunks) * (kFrABytes + tok * 128) / 14e6;
-    const double waves = (double) (tiles * blocks * s) / (2.0 * sm_count());
-    return std::max(steps, std::max(memory, l2)) + 0.006 * tok * s + 6.0 * std::max(0.0, waves - 1.0);
+    const bool wide = tok > 128;   // one CTA per SM
+    const double ctas = (double) (tiles * blocks * s), resident = (wide ? 1.0 : 2.0) * sm_count();
+    const double steps = (double) ceil_div(chunks, s) * (wide ? 0.14 + 0.0012 * tok : 0.25 + 0.00125 * tok);
+    const double memory = (double) tiles * (double) chunks * kFrABytes / (!wide && ctas <= sm_count() ? 5.8e6 : 6.5e6);
+    const double l2 = (double) tiles * (double) (blocks * chunks) * (kFrABytes + tok * 128) / 13e6;
+    const double exchange = (tok <= 32 ? 0.008 : wide ? 0.0075 : 0.016) * tok * s;
+    return 4.5 + exchange + std::max(steps, std::max(memory, l2)) + 6.0 * std::max(0.0, ctas / resident - 1.0);
 }
-// CTAs per cluster that make it smallest
-static int fr_split(int tok, int64_t tiles, int64_t blocks, int64_t chunks) {
-    int best = 1;
-    for (int s = 2; s <= kFrMaxSplit && tiles * blocks * s <= 2 * (int64_t) sm_count() && chunks >= 2 * s; s *= 2)
-        if (fr_cost(tok, tiles, blocks, chunks, s) < fr_cost(tok, tiles, blocks, chunks, best)) best = s;
+// Tokens per block and CTAs per cluster with the smallest estimate.
+struct FrPlan { int tok, split; double us; };
+static FrPlan fr_plan(int64_t rows, int64_t n, int64_t k) {
+    const int64_t tiles = ceil_div(n, kFrFeat), chunks = ceil_div(k, 64);
+    FrPlan best{0, 1, 0.0};
+    for (int tok : {16, 32, 64, 128, 192, 256}) {
+        if ((tok < 128 && tok < rows) || (tok > 16 && tok <= 128 && tok / 2 >= rows) || (tok > 128 && rows <= 64)) continue;   // no room, or more than half of it empty
+        const int64_t blocks = ceil_div(rows, tok);
+        for (int s = 1; s <= kFrMaxSplit && (s == 1 || (tiles * blocks * s <= (tok > 128 ? 1 : 2) * (int64_t) sm_count() && chunks >= 2 * s)); s *= 2) {
+            const double us = fr_cost(tok, tiles, blocks, chunks, s);
+            if (best.tok == 0 || us < best.us) best = {tok, s, us};
+        }
+    }
     return best;
 }
 
-// The same for the experts' kernels, whose producers also gather rows: one CTA per SM does not saturate the memory there (DOWN of seven
+// CTAs per cluster of the experts' kernels, whose producers also gather rows: one CTA per SM does not saturate the memory there (DOWN of seven
 // experts of 4096 x 14336 with 128 CTAs 245 us, with 256 126 us), so the split doubles while the grid stays resident and every CTA keeps
 // four steps.
 static int fr_split_experts(int64_t tiles, int64_t chunks) {
@@ -576,21 +634,22 @@ static int fr_dispatch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRo
     case 16: return fr_launch<16, KIND>(tw, tx, a, tiles, grid_y, st);
     case 32: return fr_launch<32, KIND>(tw, tx, a, tiles, grid_y, st);
     case 64: return fr_launch<64, KIND>(tw, tx, a, tiles, grid_y, st);
-    default: return fr_launch<128, KIND>(tw, tx, a, tiles, grid_y, st);
+    case 128: return fr_launch<128, KIND>(tw, tx, a, tiles, grid_y, st);
     }
+    if constexpr (KIND == FR_LINEAR) {
+        if (tok == 192) return fr_launch<192, KIND>(tw, tx, a, tiles, grid_y, st);
+        if (tok == 256) return fr_launch<256, KIND>(tw, tx, a, tiles, grid_y, st);
+    }
+    return set_error(PT_ERR_INVALID, "few-row product: no kernel for %d tokens per block", tok);
 }
-static int fr_tokens(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
-double few_rows_us(int64_t M, int64_t N, int64_t K) {
-    const int tok = fr_tokens(M);
-    const int64_t tiles = ceil_div(N, kFrFeat), blocks = ceil_div(M, tok), chunks = ceil_div(K, 64);
-    return 7.0 + fr_cost(tok, tiles, blocks, chunks, fr_split(tok, tiles, blocks, chunks));
-}
+double few_rows_us(int64_t M, int64_t N, int64_t K) { return fr_plan(M, N, K).us; }
 
 // y = act(a . b^T + bias) + residual for few rows of a
 int few_rows_linear(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,
                     void *z, int act, int64_t M, int64_t N, int64_t K, int *status, cudaStream_t st) {
-    const int tok = fr_tokens(M);
+    const FrPlan plan = fr_plan(M, N, K);
+    const int tok = plan.tok;
     CUtensorMap tw, tx;
     int rc;
     if ((rc = b_mn ? make_tmap_bytes(&tw, b, K, 2 * N, 2 * N, 64) : make_tmap_bytes(&tw, b, N, 2 * K, 2 * K, kFrFeat)) != PT_OK) return rc;
@@ -601,7 +660,7 @@ int few_rows_linear(const void *a, const void *b, int b_mn, int ab_dtype, const 
     const int esize = c_dtype == PT_F32 ? 4 : 2;
     r.vec_ok = N % 4 == 0 && aligned(c, 4 * esize) && aligned(residual, 4 * esize) && aligned(z, 8) && aligned(bias, bias_dtype == PT_F32 ? 16 : 8);
     const int64_t tiles = ceil_div(N, kFrFeat), grid_y = ceil_div(M, tok);
-    r.split = fr_split(tok, tiles, grid_y, ceil_div(K, 64));
+    r.split = plan.split;
     return fr_dispatch<FR_LINEAR>(tw, tx, r, tok, tiles, grid_y, st);
 }
 
@@ -634,7 +693,7 @@ int pt_moe_few_tokens(const void *x, const void *gate_up, const void *down, int 
     PT_REQUIRE(scratch_bytes >= pt_moe_few_tokens_scratch_bytes(T, top_k, I) && aligned(scratch, 16), "moe_few_tokens: scratch too small or unaligned");
     PT_REQUIRE(aligned(out, 8), "moe_few_tokens: out must be 8-byte aligned");
     cudaStream_t st = (cudaStream_t) stream;
-    const int tok = fr_tokens(T);
+    const int tok = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
     const int64_t slots = T * top_k, most = std::min<int64_t>(E, slots);   // experts that can be chosen
     CUtensorMap tw, tx;
     int rc;

@@ -82,15 +82,10 @@ __device__ __forceinline__ void raw4_as_f32(const uint4 &w, int dtype, float (&v
         v[0] = lo_f32<__half>(w.x); v[1] = hi_f32<__half>(w.x); v[2] = lo_f32<__half>(w.y); v[3] = hi_f32<__half>(w.y);
     }
 }
-__device__ __forceinline__ void load4_as_f32(const void *p, int dtype, int64_t i, float (&v)[4]) {
-    uint4 w = {};
-    if (dtype == PT_F32) {
-        w = *reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(p) + i);
-    } else {
-        const uint2 h = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + i);
-        w.x = h.x; w.y = h.y;
-    }
-    raw4_as_f32(w, dtype, v);
+__device__ __forceinline__ uint4 load4_raw(const void *p, int dtype, int64_t i) {
+    if (dtype == PT_F32) return *reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(p) + i);
+    const uint2 h = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + i);
+    return make_uint4(h.x, h.y, 0u, 0u);
 }
 __device__ __forceinline__ void store4_from_f32(void *p, int dtype, int64_t i, const float (&v)[4]) {
     if (dtype == PT_F32) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);

@@ -104,7 +104,7 @@ def test_few_rows(dt, M, N, K):
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("M,N,K", [(33000, 130, 1032), (20001, 257, 2048), (9000, 1001, 1000)])
+@pytest.mark.parametrize("M,N,K", [(33000, 130, 1032), (40000, 257, 2048), (9000, 1001, 1000)])
 def test_tiles(dt, M, N, K):
     """Enough tiles for the tile kernels: single CTAs below 512 columns, CTA pairs from there on."""
     assert not _few(M, N, K)

@@ -513,23 +513,32 @@ __global__ void __launch_bounds__(kQkBwdThreads) qk_norm_rope_any_kernel(QkArgs 
     }
 }
 
-// dgamma = sum of the partial rows of its side, in a fixed order; blockIdx.y: 0 queries, 1 keys.
+// dgamma = sum of the partial rows of its side, in a fixed order; blockIdx.y: 0 queries, 1 keys.  A warp per 32 columns and every 32nd
+// row, up to 16 rows in flight: one or two memory latencies (with 16 warps and 4 rows in flight this tail took 7 us).
+constexpr int kDgWarps = 32;
 template <typename T>
-__global__ void __launch_bounds__(512) qk_dgamma_kernel(const float *__restrict__ partial, int parts_q, int parts, int D, T *dq_gamma, T *dk_gamma) {
-    __shared__ float s_sum[16][33];
+__global__ void __launch_bounds__(32 * kDgWarps) qk_dgamma_kernel(const float *__restrict__ partial, int parts_q, int parts, int D, T *dq_gamma,
+                                                                  T *dk_gamma) {
+    __shared__ float s_sum[kDgWarps][33];
     grid_dep_wait();
-    const int c = threadIdx.x & 31, lane = threadIdx.x >> 5, d = (int) blockIdx.x * 32 + c;
+    const int c = threadIdx.x & 31, warp = threadIdx.x >> 5, d = (int) blockIdx.x * 32 + c;
     const int first = blockIdx.y ? parts_q : 0, last = blockIdx.y ? parts : parts_q;
     float acc = 0.f;
-    if (d < D)
-#pragma unroll 4
-        for (int p = first + lane; p < last; p += 16) acc += partial[(int64_t) p * D + d];
-    s_sum[lane][c] = acc;
+    if (d < D) {
+        for (int p0 = first + warp; p0 < last; p0 += 16 * kDgWarps) {
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = p0 + i * kDgWarps < last ? partial[(int64_t) (p0 + i * kDgWarps) * D + d] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc += v[i];
+        }
+    }
+    s_sum[warp][c] = acc;
     __syncthreads();
-    if (lane == 0 && d < D) {
+    if (warp == 0 && d < D) {
         float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) t += s_sum[i][c];
+        for (int i = 0; i < kDgWarps; ++i) t += s_sum[i][c];
         (blockIdx.y ? dk_gamma : dq_gamma)[d] = qk_from_f<T>(t);
     }
 }
@@ -677,7 +686,7 @@ int pt_qk_norm_rope_bwd(const void *dq, const void *dk, const void *q, const voi
     PT_SWITCH_SRC(dtype, T, {
         const int rc2 = interleaved ? qk_dispatch<T, true>(a, true, st) : qk_dispatch<T, false>(a, true, st);
         if (rc2 != PT_OK) return rc2;
-        PT_CUDA_OK(launch_overlapped(qk_dgamma_kernel<T>, dim3((unsigned) ceil_div(D, 32), 2), dim3(512), 0, st, (const float *) partial, a.parts_q, a.parts, D,
+        PT_CUDA_OK(launch_overlapped(qk_dgamma_kernel<T>, dim3((unsigned) ceil_div(D, 32), 2), dim3(32 * kDgWarps), 0, st, (const float *) partial, a.parts_q, a.parts, D,
                                      (T *) dq_gamma, (T *) dk_gamma));
     });
     return PT_OK;

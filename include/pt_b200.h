@@ -477,8 +477,8 @@ int pt_moe_few_tokens(const void *x, const void *gate_up, const void *down, int 
  * c [M, N] = act(a . b^T + bias) + residual, fp32 accumulate, rounded once: a [M, K], b [N, K], or [K, N] with b_mn (N a multiple of
  * 8 then); PT_BF16 / PT_F16, K a multiple of 8, 16-byte aligned bases; bias [N] of any of the three types or null, residual [M, N] of c's type or null.  act 0 = SiLU, 1 = GELU
  * (erf), 2 = none, 3 = ReLU, 4 = GELU (tanh).  z: null, or [M, N] in the operands' type, receives a . b^T + bias (the backward's
- * input).  residual may be c itself.  status as in pt_gemm; calls for which pt_gemm_bias_act_few_rows is 1 may also be given a
- * mapped host word.  (The reference runs gemm and leaves bias, activation and residual to separate torch kernels:
+ * input).  residual may be c itself.  status: device or mapped host int, as in pt_gemm.  pt_gemm_bias_act_few_rows tells which kernels a
+ * size runs on (1: the weight-streaming ones for few rows, 0: the tiles of pt_gemm), for measurements.  (The reference runs gemm and leaves bias, activation and residual to separate torch kernels:
  * primus_turbo/pytorch/ops/gemm.py.) */
 int pt_gemm_bias_act_few_rows(int64_t M, int64_t N, int64_t K);
 int pt_gemm_bias_act(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype, void *z,

@@ -58,6 +58,12 @@ inline cudaError_t launch_overlapped(void (*kern)(KArgs...), dim3 grid, dim3 blo
     return cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
 }
 
+// An error into a status word (null: nobody asked).  A plain store, every writer storing the same code, so that the word may also lie in
+// mapped host memory.
+__device__ __forceinline__ void report_status(int *status, int code) {
+    if (status != nullptr) *reinterpret_cast<volatile int *>(status) = code;
+}
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t ceil_to(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 

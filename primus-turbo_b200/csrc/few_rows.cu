@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
         }
     }
     if (!ok || s_abort) {
-        if (a.status != nullptr && lane == 0) *reinterpret_cast<volatile int *>(a.status) = PT_ERR_TIMEOUT;
+        if (lane == 0) report_status(a.status, PT_ERR_TIMEOUT);
         __nanosleep(200000);   // let copies in flight land before the shared memory is released
     }
     tc_fence_before_sync();

@@ -123,12 +123,12 @@ inline EncodeTiledFn encode_tiled_fn() {
             fn = reinterpret_cast<EncodeTiledFn>(p);
     });
     // The driver call needs a context bound to the calling thread.  A thread that has made no runtime call yet
-    // (autograd's backward threads reach the quantizers this way) has none: cudaFree(nullptr) binds the device's
-    // primary context; once per thread.
+    // (autograd's backward threads reach the quantizers this way) has none: setting the current device binds its
+    // primary context, in a stream capture too (cudaFree(nullptr), the older idiom, is refused there); once per thread.
     thread_local bool bound = false;
     if (!bound) {
-        cudaFree(nullptr);
-        bound = true;
+        int dev = 0;
+        bound = cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
     }
     return fn;
 }

@@ -57,7 +57,7 @@ struct GemmParams {
     int64_t b_group_rows;       // rows between consecutive B[g] (N for [G, N, K])
     const int64_t *koffs;       // variable-K form: contraction range [koffs[g], koffs[g+1]) of group g (multiples of 128);
                                 // every group then yields a full [M, N] block of C (C is [G, M, N]), A and B are shared
-    int *status;                // device int: set to a PT_ERR_* code on a bounded-wait expiry
+    int *status;                // device or mapped host int: set to a PT_ERR_* code on a bounded-wait expiry
     int raster_m;               // row blocks per raster band
     int64_t sfb_line0;          // CTA-pair MX kernel: first 128-byte line of the re-tiled B scales in the scale buffer
     int a_mn, b_mn;             // one group, no block scales: the operand is stored [contraction, rows] (MN-major) and read in place
@@ -620,7 +620,7 @@ __global__ void __launch_bounds__((GemmCfg<BLOCK_N, mode_is_mx(MODE), MODE == GE
 
     // ---- teardown
     if (!ok || *abort_flag) {
-        if (p.status && lane == 0) atomicExch(p.status, (int) PT_ERR_TIMEOUT);
+        if (lane == 0) report_status(p.status, PT_ERR_TIMEOUT);
         __nanosleep(200000);  // let any TMA copy still in flight land before the shared memory is released
     }
     tc_fence_before_sync();
@@ -918,6 +918,7 @@ int gemm_hp_host(const void *a, const void *b, int ab_dtype, void *c, int c_dtyp
 // 33.5; 192 x 14336 x 4096 33.5 / 38.6, 512 x 14336 x 4096 76.0 / 57.5; 512 x 4096 x 14336 58.1 / 81.9, 768 x 4096 x 14336 79.6 / 84.8.
 static bool few_rows_better(int64_t M, int64_t N, int64_t K) {
     if (M <= 64) return true;
+    if (M > (int64_t) 65535 * 128) return false;   // blocks of tokens are the grid's second extent
     const int64_t waves = ceil_div(ceil_div(M, 256) * ceil_div(N, 256), sm_count() / 2);
     return few_rows_us(M, N, K) < 10.0 + (double) waves * (3.0 + 4.35 * (double) K / 1024.0);
 }

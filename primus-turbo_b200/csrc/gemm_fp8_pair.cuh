@@ -275,7 +275,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BLOCK_N, mo
 
     // ---- teardown: both CTAs leave together (the leader's MMAs read the peer's shared and tensor memory)
     if (!ok || *abort_flag) {
-        if (p.status && lane == 0) atomicExch(p.status, (int) PT_ERR_TIMEOUT);
+        if (lane == 0) report_status(p.status, PT_ERR_TIMEOUT);
         __nanosleep(200000);
     }
     tc_fence_before_sync();

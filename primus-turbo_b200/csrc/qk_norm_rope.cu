@@ -119,7 +119,7 @@ __device__ __forceinline__ int64_t qk_position(const QkArgs &a, uint32_t t, uint
     if (a.pos_bytes == 8) p = reinterpret_cast<const int64_t *>(a.positions)[t];
     else if (a.pos_bytes == 4) p = reinterpret_cast<const int *>(a.positions)[t];
     if (p < 0 || p >= a.P) {
-        if (a.status != nullptr) *reinterpret_cast<volatile int *>(a.status) = PT_ERR_INVALID;
+        report_status(a.status, PT_ERR_INVALID);
         return -1;
     }
     return p;

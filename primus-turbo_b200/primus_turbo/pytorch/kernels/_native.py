@@ -87,9 +87,9 @@ def status_word(device) -> torch.Tensor:
 
 
 def host_status(device):
-    """Per-device status word in pinned host memory, which the kernels of the operators built for single calls write directly
-    (mapped, so the address is the device's too).  Reading it is one host load: a copy and an event per call, as poll_status
-    makes, would cost such an operator as much as its kernel."""
+    """Per-device status word in pinned host memory, which the kernels of gemm_bias_act, qk_norm_rope and moe_few_tokens write
+    directly (mapped, so the address is the device's too).  Reading it is one host load: a copy and an event per call, as
+    poll_status makes, would cost an operator on one token as much as its kernel."""
     idx = device.index
     w = _host_status.get(idx)
     if w is None:

@@ -94,18 +94,11 @@ def gemm_bias_act_impl(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Op
     bias = None if bias is None else bias.contiguous()
     residual = None if residual is None else residual.contiguous()
     lib = nv.lib()
-    few = lib.pt_gemm_bias_act_few_rows(M, N, K)
-    if few:
-        nv.poll_host_status(a.device)
-        st = nv.host_status(a.device)[2]
-    else:
-        st = nv.ptr(nv.status_word(a.device))
+    nv.poll_host_status(a.device)
     with nv.on_device(a.device):
         nv.check(lib.pt_gemm_bias_act(nv.ptr(a_km), nv.ptr(b_km), int(b_mn), nv.src_code(a.dtype), nv.ptr(bias), 0 if bias is None else nv.src_code(bias.dtype),
-                                      nv.ptr(residual), nv.ptr(out), nv.src_code(out_dtype), nv.ptr(z), EPILOGUE_ACTS[act], M, N, K, st,
-                                      nv.stream(a.device)), "gemm_bias_act")
-    if not few:
-        nv.poll_status(a.device)
+                                      nv.ptr(residual), nv.ptr(out), nv.src_code(out_dtype), nv.ptr(z), EPILOGUE_ACTS[act], M, N, K,
+                                      nv.host_status(a.device)[2], nv.stream(a.device)), "gemm_bias_act")
     return out, z
 
 

@@ -6,6 +6,7 @@ the reference lacks, adds bias, activation and residual in the product's epilogu
 from typing import Optional, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ..kernels.gemm.gemm_impl import EPILOGUE_ACTS, act_bias_bwd_impl, gemm_accum_impl, gemm_bias_act_impl, gemm_impl
 from .utils import _get_dummy_wgrad, _setup_fused_grad_accum
@@ -57,6 +58,7 @@ class GemmBiasActFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         a, b, z = ctx.saved_tensors
         need_a, need_b, need_bias, need_residual = ctx.needs_input_grad[:4]

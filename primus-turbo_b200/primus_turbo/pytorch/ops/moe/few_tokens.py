@@ -20,7 +20,8 @@ def moe_few_tokens(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, t
     x [T, H], gate_up [E, 2 I, H] (gate rows first), down [E, H, I], bf16 or fp16; topk_indices int32 / int64 and topk_probs fp32
     [T, K].  An index outside of [0, E), such as -1 for an expert of another shard, adds nothing.  H and I are multiples of 8;
     T at most 128, E 1024, K 32, T * K 2048: longer inputs go through token_permute and grouped_gemm.  Forward only (no gradient);
-    act(gate) * up * prob is rounded to x's dtype between the two products.  act_type: "silu" or "gelu" (erf form)."""
+    act(gate) * up * prob is rounded to x's dtype between the two products.  The weights must be finite: the down product multiplies
+    the rows of an expert's weight with zeros for tokens that did not choose it, and an infinity would reach them.  act_type: "silu" or "gelu" (erf form)."""
     assert act_type in SUPPORTED_ACT_TYPES, f"Unsupported act_type: {act_type}. Supported types: {SUPPORTED_ACT_TYPES}"
     assert x.dim() == 2 and gate_up.dim() == 3 and down.dim() == 3, "moe_few_tokens: x must be [T, H], gate_up [E, 2I, H], down [E, H, I]"
     T, H = x.shape

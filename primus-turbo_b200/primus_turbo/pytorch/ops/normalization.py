@@ -3,6 +3,7 @@ qk_norm_rope, which the reference lacks: the norm of every query and key head an
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ..kernels.normalization.qk_norm_rope_impl import qk_norm_rope_bwd_impl, qk_norm_rope_fwd_impl
 
@@ -71,6 +72,7 @@ class _QKNormRopeFunction(torch.autograd.Function):
         return qk_norm_rope_fwd_impl(q, k, q_gamma, k_gamma, cos, sin, positions, eps, interleaved, zero_centered)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         q, k, q_gamma, k_gamma, cos, sin, positions = ctx.saved_tensors
         dq, dk = (d.to(q.dtype) if d.stride(-1) == 1 else d.to(q.dtype).contiguous() for d in (dq, dk))

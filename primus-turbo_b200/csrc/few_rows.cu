@@ -695,23 +695,23 @@ int pt_moe_few_tokens(const void *x, const void *gate_up, const void *down, int 
     cudaStream_t st = (cudaStream_t) stream;
     const int tok = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
     const int64_t slots = T * top_k, most = std::min<int64_t>(E, slots);   // experts that can be chosen
-    CUtensorMap tw, tx;
+    CUtensorMap t_gate_up, t_x, t_down, t_h;
     int rc;
+    if ((rc = make_tmap_bytes(&t_gate_up, gate_up, (int64_t) E * 2 * I, 2 * H, 2 * H, 64)) != PT_OK) return rc;
+    if ((rc = make_tmap_bytes(&t_x, x, T, 2 * H, 2 * H, 1)) != PT_OK) return rc;
+    if ((rc = make_tmap_bytes(&t_down, down, (int64_t) E * H, 2 * I, 2 * I, kFrFeat)) != PT_OK) return rc;
+    if ((rc = make_tmap_bytes(&t_h, scratch, slots, 2 * I, 2 * I, 1)) != PT_OK) return rc;
     FewRowsArgs a{};
     a.rows = (int) T; a.fmt = dtype == PT_BF16 ? 1 : 0; a.act = act; a.ids = ids; a.id_bytes = id_bytes; a.top_k = top_k; a.experts = E;
     a.probs = probs; a.status = status; a.out_dtype = dtype;
-    if ((rc = make_tmap_bytes(&tw, gate_up, (int64_t) E * 2 * I, 2 * H, 2 * H, 64)) != PT_OK) return rc;
-    if ((rc = make_tmap_bytes(&tx, x, T, 2 * H, 2 * H, 1)) != PT_OK) return rc;
     a.n = (int) I; a.k = (int) H; a.out = scratch;
     int64_t tiles = ceil_div(I, 64);
     a.split = fr_split_experts(tiles * most, ceil_div(H, 64));
-    if ((rc = fr_dispatch<FR_GATE_UP>(tw, tx, a, tok, tiles, most, st)) != PT_OK) return rc;
-    if ((rc = make_tmap_bytes(&tw, down, (int64_t) E * H, 2 * I, 2 * I, kFrFeat)) != PT_OK) return rc;
-    if ((rc = make_tmap_bytes(&tx, scratch, slots, 2 * I, 2 * I, 1)) != PT_OK) return rc;
+    if ((rc = fr_dispatch<FR_GATE_UP>(t_gate_up, t_x, a, tok, tiles, most, st)) != PT_OK) return rc;
     a.n = (int) H; a.k = (int) I; a.out = out;
     tiles = ceil_div(H, kFrFeat);
     a.split = fr_split_experts(tiles, most * ceil_div(I, 64));
-    return fr_dispatch<FR_DOWN>(tw, tx, a, tok, tiles, 1, st);
+    return fr_dispatch<FR_DOWN>(t_down, t_h, a, tok, tiles, 1, st);
 }
 
 }  // extern "C"

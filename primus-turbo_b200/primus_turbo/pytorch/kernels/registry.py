@@ -21,6 +21,8 @@ from .gemm import gemm_impl as _g16
 from .grouped_gemm import grouped_gemm_fp4_impl as _gg4
 from .grouped_gemm import grouped_gemm_fp8_impl as _gg8
 from .grouped_gemm import grouped_gemm_impl as _gg16
+from .moe import few_tokens_impl as _few
+from .normalization import qk_norm_rope_impl as _qk
 from .quantization import quantization_impl as _q
 
 _op = torch.library.custom_op
@@ -112,6 +114,42 @@ def gemm_accum_impl(a: torch.Tensor, trans_a: bool, b: torch.Tensor, trans_b: bo
 @gemm_accum_impl.register_fake
 def _(a, trans_a, b, trans_b, out_dtype, trans_c, out, default_backend):
     return None
+
+
+# ------------------------------------------------------------------------------------------------ around a decoder layer's products
+# (no counterpart in the reference; `ops` checks the arguments before it calls the same functions)
+@_op("primus_turbo::gemm_bias_act_impl", mutates_args=(), device_types="cuda")
+def gemm_bias_act_impl(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Optional[torch.Tensor], activation: Optional[str],
+                       residual: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    return _g16.gemm_bias_act_impl(a, b, trans_b, bias, activation, residual, out_dtype, False)[0]
+
+
+@gemm_bias_act_impl.register_fake
+def _(a, b, trans_b, bias, activation, residual, out_dtype):
+    return _out2d(a, b, False, trans_b, False, out_dtype)
+
+
+@_op("primus_turbo::qk_norm_rope_fwd_impl", mutates_args=(), device_types="cuda")
+def qk_norm_rope_fwd_impl(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor, k_gamma: torch.Tensor, cos: torch.Tensor,
+                          sin: torch.Tensor, positions: Optional[torch.Tensor], eps: float, interleaved: bool,
+                          zero_centered: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _qk.qk_norm_rope_fwd_impl(q, k, q_gamma, k_gamma, cos, sin, positions, eps, interleaved, zero_centered)
+
+
+@qk_norm_rope_fwd_impl.register_fake
+def _(q, k, q_gamma, k_gamma, cos, sin, positions, eps, interleaved, zero_centered):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+
+
+@_op("primus_turbo::moe_few_tokens_impl", mutates_args=(), device_types="cuda")
+def moe_few_tokens_impl(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, topk_indices: torch.Tensor, topk_probs: torch.Tensor,
+                        act_type: str) -> torch.Tensor:
+    return _few.moe_few_tokens_impl(x, gate_up, down, topk_indices, topk_probs, act_type)
+
+
+@moe_few_tokens_impl.register_fake
+def _(x, gate_up, down, topk_indices, topk_probs, act_type):
+    return torch.empty_like(x)
 
 
 # ------------------------------------------------------------------------------------------------ grouped GEMMs
@@ -363,5 +401,5 @@ REGISTERED = [
     "grouped_gemm_impl", "grouped_gemm_variable_k_impl", "grouped_gemm_variable_k_accum_impl",
     "quant_fp8_blockwise_impl", "dequant_fp8_blockwise_impl", "dequant_fp8_blockwise_for_weight_impl",
     "quant_fp8_blockwise_dual_impl", "quant_fp8_blockwise_for_weight_impl", "quant_fp8_blockwise_segment_m_row_col_impl",
-    "shuffle_scale", "shuffle_weight",
+    "shuffle_scale", "shuffle_weight", "gemm_bias_act_impl", "qk_norm_rope_fwd_impl", "moe_few_tokens_impl",
 ]

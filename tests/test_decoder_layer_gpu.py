@@ -201,3 +201,14 @@ print('captured')
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=240)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_registered_ops_are_the_operators():
+    from primus_turbo.pytorch import ops
+    w, x, t = _weights(), _rand((5, H), 29), torch.ops.primus_turbo
+    assert torch.equal(t.gemm_bias_act_impl(x, w["up"], True, w["bup"], "gelu", None, BF), ops.gemm_bias_act(x, w["up"], bias=w["bup"], activation="gelu", trans_b=True))
+    q = _rand((5, 4, D), 30)
+    got = t.qk_norm_rope_fwd_impl(q, q[:, :1], w["qg"], w["kg"], w["cos"], w["sin"], None, 1e-6, True, False)
+    assert all(torch.equal(a, b) for a, b in zip(got, ops.qk_norm_rope(q, q[:, :1], w["qg"], w["kg"], w["cos"], w["sin"], interleaved=True)))
+    p, ids = torch.rand(5, E, device="cuda").topk(K)
+    assert torch.equal(t.moe_few_tokens_impl(x, w["gate_up"], w["down"], ids, p, "gelu"), ops.moe_few_tokens(x, w["gate_up"], w["down"], ids, p, act_type="gelu"))

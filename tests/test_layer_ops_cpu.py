@@ -170,3 +170,17 @@ def test_moe_few_tokens_abi_refusals():
         assert call(**kw) == -1 and msg in lib.pt_last_error(), kw
     assert call(T=0) == 0
     assert lib.pt_moe_few_tokens_scratch_bytes(3, 2, 16) == 6 * 32
+
+
+# ------------------------------------------------------------------------------------------------ torch.library
+def test_custom_ops_have_fake_implementations():
+    import primus_turbo.pytorch  # noqa: F401
+    t = torch.ops.primus_turbo
+    with FakeTensorMode():
+        y = t.gemm_bias_act_impl(_e(5, 64), _e(64, 96), False, _e(96), "silu", None, torch.float32)
+        assert tuple(y.shape) == (5, 96) and y.dtype == torch.float32 and y.device.type == "cuda"
+        a = _qk_args()
+        q, k = t.qk_norm_rope_fwd_impl(a["q"], a["k"], a["q_gamma"], a["k_gamma"], a["cos"], a["sin"], None, 1e-6, False, False)
+        assert q.shape == a["q"].shape and k.shape == a["k"].shape and q.dtype == bf16
+        m = _moe_args()
+        assert t.moe_few_tokens_impl(m["x"], m["gate_up"], m["down"], m["topk_indices"], m["topk_probs"], "silu").shape == m["x"].shape

@@ -18,12 +18,12 @@
 //
 // Mixture, two kernels:
 //   GATE_UP  grid (blocks of 64 features x split, chosen experts): the block is 64 gate rows and the 64 up rows that belong to them.
-//            Rows of x are gathered by TMA (tile::gather4) from the list of the expert's tokens.  Writes p * act(g) * u, with p
+//            The expert's tokens are the narrow operand, copied row by row from the list of them.  Writes p * act(g) * u, with p
 //            the slot's probability (the sum of them where a token names an expert twice), rounded once to the tensors' type: the
 //            next product's operand type.
 //   DOWN     a CTA keeps one [128 features][tokens] accumulator over ALL chosen experts, one column per token, so the weighted
 //            sum over a token's experts happens in tensor memory.  For every expert only the 16-token blocks that hold one of
-//            its tokens are multiplied; the other tokens of such a block are rows of zeros in shared memory.  Its first weight blocks are
+//            its tokens are multiplied; the other tokens of such a block are rows of zeros.  Its first weight blocks are
 //            fetched before the first kernel has finished (programmatic dependent launch): weights and routing do not depend
 //            on it.
 #include <algorithm>
@@ -59,6 +59,8 @@ struct FewRowsArgs {
     void *z;                 // pre-activation in the operands' type, or null
     int vec_ok;              // rows of out / residual / z / bias take four elements at a time
     // mixture
+    const void *x;           // rows of x_pitch bytes: GATE_UP [tokens, k], DOWN [slots, k]
+    int64_t x_pitch;
     const void *ids;         // [tokens, top_k] int32 / int64
     int id_bytes, top_k, experts;
     const float *probs;
@@ -94,10 +96,7 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
     __shared__ int s_abort, s_count;
     __shared__ uint32_t s_bits[kMoe ? 32 : 1];
     __shared__ int16_t s_active[KIND == FR_DOWN ? kMaxGroups : 1];
-    constexpr int kRowWords = (TOK + 31) / 32;
-    __shared__ uint32_t s_held[KIND == FR_DOWN ? kStages : 1][kRowWords];   // DOWN: the rows of a stage that are not zero,
-    __shared__ int s_stage_expert[KIND == FR_DOWN ? kStages : 1];           // and the expert they belong to
-    __shared__ int s_row[kMoe ? TOK : 1], s_slot[KIND == FR_GATE_UP ? TOK : 1];
+    __shared__ int s_row[KIND == FR_GATE_UP ? TOK : 1], s_slot[KIND == FR_GATE_UP ? TOK : 1];
     __shared__ float s_prob[KIND == FR_GATE_UP ? TOK : 1];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -108,7 +107,7 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
     if (threadIdx.x == 0) {
         s_abort = 0;
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(&full_bar[s], 1);
+            mbar_init(&full_bar[s], kMoe ? 1 + 32 * Cfg::kEpiWarps : 1);   // the weights' bytes, and the copying threads
             mbar_init(&empty_bar[s], 1);
         }
         mbar_init(&done_bar, 2);   // the MMA thread's own arrival (publishes s_touched) and its commit
@@ -190,18 +189,9 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
                     }
                     base += __popc(has);
                 }
-                __syncwarp();
-                if (lane < 3 && base + lane < TOK && (base + lane) / 4 == (base - 1) / 4) s_row[base + lane] = s_row[0];   // fill the last group of four
                 if (lane == 0) s_count = base;
             }
         } else {
-            for (int i = threadIdx.x; i < kStages * (Cfg::kBBytes / 16); i += Cfg::kThreads)
-                *reinterpret_cast<uint4 *>(ring + (i / (Cfg::kBBytes / 16)) * Cfg::kStageBytes + kFrABytes + (i % (Cfg::kBBytes / 16)) * 16) = make_uint4(0, 0, 0, 0);
-            if (threadIdx.x < kStages) {
-                s_stage_expert[threadIdx.x] = -1;
-                for (int w = 0; w < kRowWords; ++w) s_held[threadIdx.x][w] = 0;
-            }
-            fence_proxy_async_smem();
             if (warp == 0) {
                 int at = excl;
                 for (uint32_t b = bits; b != 0; b &= b - 1) s_active[at++] = (int16_t) (lane * 32 + __ffs(b) - 1);
@@ -227,127 +217,51 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
         const uint64_t stream_pol = l2_policy_evict_first(), keep_pol = l2_policy_evict_last();
         if constexpr (KIND != FR_DOWN) {
             if (elect_one()) {
-                const int groups = (cnt + 3) / 4;
-                const uint32_t bytes = kFrABytes + (KIND == FR_LINEAR ? Cfg::kBBytes : groups * 512);
+                const int expert_row = expert * 2 * a.n + tile * 64;
                 uint32_t stage = 0, phase = 0;
                 for (int l = l0; l < l1; ++l) {
                     if (!(ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag))) break;
-                    uint8_t *A = ring + stage * Cfg::kStageBytes, *B = A + kFrABytes;
-                    mbar_arrive_expect_tx(&full_bar[stage], bytes);
-                    if constexpr (KIND == FR_LINEAR) {
+                    uint8_t *A = ring + stage * Cfg::kStageBytes;
+                    mbar_arrive_expect_tx(&full_bar[stage], kFrABytes + (kMoe ? 0 : Cfg::kBBytes));
+                    if (KIND == FR_GATE_UP) {
+                        tma_load_2d_hint(A, &tmap_w, &full_bar[stage], l * 128, expert_row, stream_pol);
+                        tma_load_2d_hint(A + kFrABytes / 2, &tmap_w, &full_bar[stage], l * 128, expert_row + a.n, stream_pol);
+                    } else {
                         if (a.w_mn) {
                             tma_load_2d_hint(A, &tmap_w, &full_bar[stage], tile * kFrFeat * 2, l * 64, stream_pol);
                             tma_load_2d_hint(A + kFrABytes / 2, &tmap_w, &full_bar[stage], tile * kFrFeat * 2 + 128, l * 64, stream_pol);
                         } else {
                             tma_load_2d_hint(A, &tmap_w, &full_bar[stage], l * 128, tile * kFrFeat, stream_pol);
                         }
-                        tma_load_2d_hint(B, &tmap_x, &full_bar[stage], l * 128, (int) blockIdx.y * TOK, keep_pol);
-                    } else {
-                        const int row = expert * 2 * a.n + tile * 64;
-                        tma_load_2d_hint(A, &tmap_w, &full_bar[stage], l * 128, row, stream_pol);
-                        tma_load_2d_hint(A + kFrABytes / 2, &tmap_w, &full_bar[stage], l * 128, row + a.n, stream_pol);
-                        for (int g = 0; g < groups; ++g)
-                            tma_gather4(B + g * 512, &tmap_x, &full_bar[stage], l * 128, s_row[4 * g], s_row[4 * g + 1], s_row[4 * g + 2], s_row[4 * g + 3], keep_pol);
+                        tma_load_2d_hint(A + kFrABytes, &tmap_x, &full_bar[stage], l * 128, (int) blockIdx.y * TOK, keep_pol);
                     }
                     if (++stage == kStages) { stage = 0; phase ^= 1; }
                 }
             }
         } else {
-            // s_row: the row of activations of every token for the expert at hand, -1 for tokens that did not choose it; rows: those that
-            // did, as bits.  A stage holds them at the tokens' places and zeros everywhere else: rows that an earlier expert left in
-            // the stage are cleared, the others are zero since the start.  (Loading a row of zeros instead cost more than the weights:
-            // every CTA fetched the same line of L2, 16 of them for each token of the block.)
-            int cur = -1;
-            uint32_t rows[kRowWords] = {};
-            auto set_expert = [&](int ai) {
-                if (ai == cur) return;
-                cur = ai;
-                const int e = s_active[ai];
-                __syncwarp();
-#pragma unroll
-                for (int w = 0; w < kRowWords; ++w) {
-                    const int t = 32 * w + lane;
-                    int row = -1;
-                    if (t < T)
-                        for (int j = a.top_k - 1; j >= 0; --j)
-                            if (s_ids[t * a.top_k + j] == e) row = t * a.top_k + j;   // the first of them
-                    rows[w] = __ballot_sync(0xffffffffu, row >= 0);
-                    if (t < TOK) s_row[t] = row;
-                }
-                __syncwarp();
-            };
-            auto clear_stale = [&](uint32_t stage) {   // by the whole warp, once the stage is free
-                uint8_t *B = ring + stage * Cfg::kStageBytes + kFrABytes;
-                bool any = false;
-#pragma unroll
-                for (int w = 0; w < kRowWords; ++w) {
-                    uint32_t stale = s_held[stage][w] & ~rows[w];
-                    any |= stale != 0;
-                    for (; stale != 0; stale &= stale - 1) {
-                        const int t = 32 * w + __ffs(stale) - 1;
-                        *reinterpret_cast<uint32_t *>(B + t * 128 + lane * 4) = 0u;
+            // the weights of the chosen experts one after the other, and for every stage which 16-token blocks hold one of its tokens;
+            // nothing here depends on the kernel before this one
+            int ai = l0 / max(chunks, 1), c = l0 - ai * chunks, cur = -1;
+            uint32_t blocks = 0, stage = 0, phase = 0;
+            for (int l = l0; l < l1; ++l) {
+                if (ai != cur) {
+                    cur = ai;
+                    blocks = 0;
+                    for (int t0 = 0; t0 < TOK; t0 += 32) {
+                        bool has = false;
+                        if (t0 + lane < T)
+                            for (int j = 0; j < a.top_k; ++j) has |= s_ids[(t0 + lane) * a.top_k + j] == s_active[ai];
+                        const uint32_t who = __ballot_sync(0xffffffffu, has);
+                        blocks |= (uint32_t) ((who & 0xFFFFu) != 0) << (t0 / 16) | (uint32_t) ((who >> 16) != 0) << (t0 / 16 + 1);
                     }
                 }
-                __syncwarp();
-                if (lane == 0) {
-                    s_stage_expert[stage] = cur;
-#pragma unroll
-                    for (int w = 0; w < kRowWords; ++w) s_held[stage][w] = rows[w];
+                if (lane == 0 && (ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag))) {
+                    s_mask[stage] = blocks;
+                    mbar_arrive_expect_tx(&full_bar[stage], kFrABytes);
+                    tma_load_2d_hint(ring + stage * Cfg::kStageBytes, &tmap_w, &full_bar[stage], c * 128, s_active[ai] * a.n + tile * kFrFeat, stream_pol);
                 }
-                if (any) fence_proxy_async_smem();
-                __syncwarp();
-            };
-            auto load_w = [&](int chunk, uint32_t stage) {
-                uint32_t blocks = 0;
-                int n = 0;
-#pragma unroll
-                for (int w = 0; w < kRowWords; ++w) {
-                    blocks |= (uint32_t) ((rows[w] & 0xFFFFu) != 0) << (2 * w) | (uint32_t) ((rows[w] >> 16) != 0) << (2 * w + 1);
-                    n += __popc(rows[w]);
-                }
-                s_mask[stage] = blocks;
-                mbar_arrive_expect_tx(&full_bar[stage], kFrABytes + n * 128);
-                tma_load_2d_hint(ring + stage * Cfg::kStageBytes, &tmap_w, &full_bar[stage], chunk * 128, s_active[cur] * a.n + tile * kFrFeat, stream_pol);
-            };
-            auto load_x = [&](int chunk, uint32_t stage) {
-                uint8_t *B = ring + stage * Cfg::kStageBytes + kFrABytes;
-                const int k0 = chunk * 128;
-#pragma unroll
-                for (int w = 0; w < kRowWords; ++w)
-                    for (uint32_t m = rows[w]; m != 0;) {
-                        const int b = __ffs(m) - 1, t = 32 * w + b;
-                        if ((b & 3) == 0 && (m >> b & 15) == 15) {
-                            tma_gather4(B + t * 128, &tmap_x, &full_bar[stage], k0, s_row[t], s_row[t + 1], s_row[t + 2], s_row[t + 3], keep_pol);
-                            m &= ~(15u << b);
-                        } else {
-                            tma_load_2d_hint(B + t * 128, &tmap_x, &full_bar[stage], k0, s_row[t], keep_pol);
-                            m &= m - 1;
-                        }
-                    }
-            };
-            const int pre = min(kStages, l1 - l0);   // the ring is empty: these stages need no wait
-            int ai = l0 / max(chunks, 1), c = l0 - ai * chunks;
-            auto advance = [&]() { if (++c == chunks) { c = 0; ++ai; } };
-            for (int i = 0; i < pre; ++i, advance()) {
-                set_expert(ai);
-                clear_stale(i);
-                if (lane == 0) load_w(c, i);
-            }
-            grid_dep_wait();
-            ai = l0 / max(chunks, 1); c = l0 - ai * chunks;
-            for (int i = 0; i < pre; ++i, advance()) {
-                set_expert(ai);
-                if (lane == 0) load_x(c, i);
-            }
-            uint32_t stage = pre == kStages ? 0 : pre, phase = pre == kStages ? 1 : 0;
-            for (int l = l0 + pre; l < l1; ++l, advance()) {
-                set_expert(ai);
-                if (!(ok = mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag))) break;
-                if (ai != s_stage_expert[stage]) clear_stale(stage);
-                if (lane == 0) {
-                    load_w(c, stage);
-                    load_x(c, stage);
-                }
+                if (!(ok = __shfl_sync(0xffffffffu, (int) ok, 0) != 0)) break;
+                if (++c == chunks) { c = 0; ++ai; }
                 if (++stage == kStages) { stage = 0; phase ^= 1; }
             }
         }
@@ -362,6 +276,7 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
             uint32_t stage = 0, phase = 0;
             for (int l = l0; l < l1; ++l) {
                 if (!(ok = mbar_wait(&full_bar[stage], phase, abort_flag))) break;
+                if constexpr (kMoe) fence_proxy_async_smem();   // the copied rows were written through the generic proxy
                 tc_fence_after_sync();
                 const uint32_t A = smem_u32(ring + stage * Cfg::kStageBytes);
                 const uint64_t a_desc = w_mn ? smem_desc_sw128_mn(A, kFrABytes / 2) : smem_desc_sw128(A);
@@ -388,6 +303,61 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
                 s_touched = touched;
                 mbar_arrive(&done_bar);
                 tc_commit(&done_bar);
+            }
+        }
+    }
+    if constexpr (kMoe) {
+        if (warp >= 2) {
+            // ================================================================ rows of activations (the epilogue's warps, idle until then)
+            // Every warp owns kMine consecutive rows of the token tile.  Eight lanes copy the 128 bytes of a row, 16 each, to where the swizzle
+            // of the weights' TMA would put them; rows of other tokens and what lies past the contraction's end become zeros.  (TMA loads of
+            // single rows, or of four with tile::gather4, cost their issuing thread 100 to 250 cycles each, and one warp copying all rows is
+            // as slow: 816 and 617 us for 64 tokens on eight experts of 4096 x 14336.)
+            constexpr int kMine = TOK / Cfg::kEpiWarps, kCopies = kMine / 4;
+            static_assert(kMine % 4 == 0 && (16 % kMine == 0 || kMine % 16 == 0), "rows of a warp");
+            const int first = (warp - 2) * kMine, c16 = (lane & 7) * 16;
+            const uint8_t *base = reinterpret_cast<const uint8_t *>(a.x) + c16;
+            const uint8_t *src[kCopies];   // null: a row of zeros
+            uint32_t dst[kCopies];
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                const int t = first + 4 * i + (lane >> 3);
+                dst[i] = (uint32_t) (kFrABytes + t * 128 + (c16 ^ ((t & 7) << 4)));
+                src[i] = KIND == FR_GATE_UP && t < cnt ? base + s_row[t] * a.x_pitch : nullptr;
+            }
+            bool needed = KIND == FR_GATE_UP && first / 16 * 16 < cnt;   // the multiplication reads the block these rows lie in
+            if constexpr (KIND == FR_DOWN) grid_dep_wait();
+            int ai = KIND == FR_DOWN ? l0 / max(chunks, 1) : 0, c = l0 - ai * chunks, cur = -1;
+            uint32_t stage = 0, phase = 0;
+            for (int l = l0; l < l1; ++l) {
+                if (KIND == FR_DOWN && ai != cur) {   // the slots in which this warp's block of 16 tokens names the next expert
+                    cur = ai;
+                    const int t = first / 16 * 16 + (lane & 15);
+                    int slot = -1;
+                    if (t < T)
+                        for (int j = a.top_k - 1; j >= 0; --j)
+                            if (s_ids[t * a.top_k + j] == s_active[ai]) slot = t * a.top_k + j;   // the first of them
+                    needed = __any_sync(0xffffffffu, slot >= 0);
+#pragma unroll
+                    for (int i = 0; i < kCopies; ++i) {
+                        const int mine = __shfl_sync(0xffffffffu, slot, first % 16 + 4 * i + (lane >> 3));
+                        src[i] = mine >= 0 ? base + mine * a.x_pitch : nullptr;
+                    }
+                }
+                int good = 1;
+                if (lane == 0) good = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag);
+                if (!(ok = __shfl_sync(0xffffffffu, good, 0) != 0)) break;
+                if (needed) {
+                    const int64_t k0 = (int64_t) c * 128;
+                    const bool inside = k0 + c16 < a.x_pitch;
+#pragma unroll
+                    for (int i = 0; i < kCopies; ++i)
+                        cp_async_16_or_zero(ring + stage * Cfg::kStageBytes + dst[i], src[i] != nullptr && inside ? src[i] + k0 : reinterpret_cast<const uint8_t *>(a.x),
+                                            src[i] != nullptr && inside);
+                }
+                cp_async_arrive_noinc(&full_bar[stage]);
+                if (++c == chunks) { c = 0; ++ai; }
+                if (++stage == kStages) { stage = 0; phase ^= 1; }
             }
         }
     }
@@ -691,27 +661,25 @@ int pt_moe_few_tokens(const void *x, const void *gate_up, const void *down, int 
     if (T == 0) return PT_OK;
     PT_REQUIRE(x && gate_up && down && ids && probs && scratch && out, "moe_few_tokens: null pointer");
     PT_REQUIRE(scratch_bytes >= pt_moe_few_tokens_scratch_bytes(T, top_k, I) && aligned(scratch, 16), "moe_few_tokens: scratch too small or unaligned");
-    PT_REQUIRE(aligned(out, 8), "moe_few_tokens: out must be 8-byte aligned");
+    PT_REQUIRE(aligned(x, 16) && aligned(out, 8), "moe_few_tokens: x must be 16-byte and out 8-byte aligned");
     cudaStream_t st = (cudaStream_t) stream;
     const int tok = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
     const int64_t slots = T * top_k, most = std::min<int64_t>(E, slots);   // experts that can be chosen
-    CUtensorMap t_gate_up, t_x, t_down, t_h;
+    CUtensorMap t_gate_up, t_down;
     int rc;
     if ((rc = make_tmap_bytes(&t_gate_up, gate_up, (int64_t) E * 2 * I, 2 * H, 2 * H, 64)) != PT_OK) return rc;
-    if ((rc = make_tmap_bytes(&t_x, x, T, 2 * H, 2 * H, 1)) != PT_OK) return rc;
     if ((rc = make_tmap_bytes(&t_down, down, (int64_t) E * H, 2 * I, 2 * I, kFrFeat)) != PT_OK) return rc;
-    if ((rc = make_tmap_bytes(&t_h, scratch, slots, 2 * I, 2 * I, 1)) != PT_OK) return rc;
     FewRowsArgs a{};
     a.rows = (int) T; a.fmt = dtype == PT_BF16 ? 1 : 0; a.act = act; a.ids = ids; a.id_bytes = id_bytes; a.top_k = top_k; a.experts = E;
     a.probs = probs; a.status = status; a.out_dtype = dtype;
-    a.n = (int) I; a.k = (int) H; a.out = scratch;
+    a.n = (int) I; a.k = (int) H; a.out = scratch; a.x = x; a.x_pitch = 2 * H;
     int64_t tiles = ceil_div(I, 64);
     a.split = fr_split_experts(tiles * most, ceil_div(H, 64));
-    if ((rc = fr_dispatch<FR_GATE_UP>(t_gate_up, t_x, a, tok, tiles, most, st)) != PT_OK) return rc;
-    a.n = (int) H; a.k = (int) I; a.out = out;
+    if ((rc = fr_dispatch<FR_GATE_UP>(t_gate_up, t_gate_up, a, tok, tiles, most, st)) != PT_OK) return rc;
+    a.n = (int) H; a.k = (int) I; a.out = out; a.x = scratch; a.x_pitch = 2 * I;
     tiles = ceil_div(H, kFrFeat);
     a.split = fr_split_experts(tiles, most * ceil_div(I, 64));
-    return fr_dispatch<FR_DOWN>(t_down, t_h, a, tok, tiles, 1, st);
+    return fr_dispatch<FR_DOWN>(t_down, t_down, a, tok, tiles, 1, st);
 }
 
 }  // extern "C"

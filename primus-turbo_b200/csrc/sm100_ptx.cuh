@@ -120,6 +120,11 @@ __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wa
 __device__ __forceinline__ void cp_async_4(void *smem_dst, const void *gsrc) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(gsrc)) : "memory");
 }
+// 16-byte asynchronous copy global -> shared; without `has` the source is not read and the 16 bytes become zeros
+__device__ __forceinline__ void cp_async_16_or_zero(void *smem_dst, const void *gsrc, bool has) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(gsrc)), "r"(has ? 16 : 0)
+                 : "memory");
+}
 // The barrier receives one arrival from this thread once all of its earlier cp.async copies have landed.
 __device__ __forceinline__ void cp_async_arrive_noinc(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -322,14 +327,6 @@ __device__ __forceinline__ void tma_load_2d_pair_hint(void *smem_dst, const CUte
     asm volatile(
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
         ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster_addr), "r"(c0), "r"(c1), "l"(policy)
-        : "memory");
-}
-// Four rows r0 .. r3 of a 2-D tensor (box one row high), 128 bytes each at column c0, as consecutive rows of the swizzled tile.
-__device__ __forceinline__ void tma_gather4(void *smem_dst, const CUtensorMap *m, uint64_t *bar, int c0, int r0, int r1, int r2, int r3,
-                                            uint64_t policy) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
-        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "l"(policy)
         : "memory");
 }
 // shared::cluster address of a shared::cta address in the CTA of cluster rank `rank`

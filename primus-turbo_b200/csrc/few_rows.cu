@@ -589,13 +589,12 @@ static FrPlan fr_plan(int64_t rows, int64_t n, int64_t k) {
     return best;
 }
 
-// CTAs per cluster of the experts' kernels, whose producers also gather rows: one CTA per SM does not saturate the memory there (DOWN of seven
-// experts of 4096 x 14336 with 128 CTAs 245 us, with 256 126 us), so the split doubles while the grid stays resident and every CTA keeps
-// four steps.
-static int fr_split_experts(int64_t tiles, int64_t chunks) {
-    int s = 1;
-    while (s < kFrMaxSplit && tiles * s * 2 <= 2 * (int64_t) sm_count() && chunks / (s * 2) >= 4) s *= 2;
-    return s;
+// CTAs per cluster of the experts' kernels, by the same estimate with the number of experts that can be chosen.
+static int fr_split_experts(int tok, int64_t tiles, int64_t chunks) {
+    int best = 1;
+    for (int s = 2; s <= kFrMaxSplit && tiles * s <= 2 * (int64_t) sm_count() && chunks >= 2 * s; s *= 2)
+        if (fr_cost(tok, tiles, 1, chunks, s) < fr_cost(tok, tiles, 1, chunks, best)) best = s;
+    return best;
 }
 
 template <int KIND>
@@ -674,11 +673,11 @@ int pt_moe_few_tokens(const void *x, const void *gate_up, const void *down, int 
     a.probs = probs; a.status = status; a.out_dtype = dtype;
     a.n = (int) I; a.k = (int) H; a.out = scratch; a.x = x; a.x_pitch = 2 * H;
     int64_t tiles = ceil_div(I, 64);
-    a.split = fr_split_experts(tiles * most, ceil_div(H, 64));
+    a.split = fr_split_experts(tok, tiles * most, ceil_div(H, 64));
     if ((rc = fr_dispatch<FR_GATE_UP>(t_gate_up, t_gate_up, a, tok, tiles, most, st)) != PT_OK) return rc;
     a.n = (int) H; a.k = (int) I; a.out = out; a.x = scratch; a.x_pitch = 2 * I;
     tiles = ceil_div(H, kFrFeat);
-    a.split = fr_split_experts(tiles, most * ceil_div(I, 64));
+    a.split = fr_split_experts(tok, tiles, most * ceil_div(I, 64));
     return fr_dispatch<FR_DOWN>(t_down, t_down, a, tok, tiles, 1, st);
 }
 

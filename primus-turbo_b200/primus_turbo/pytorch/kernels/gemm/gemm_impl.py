@@ -34,19 +34,24 @@ def _in_place(x, trans, other, other_trans):
     return trans and x.is_contiguous() and fits(x) and (x.shape[0] % 8 == 0 or (other_trans and other.is_contiguous() and fits(other)))
 
 
-def _launch(a, a_mn, b, b_mn, out, beta):
+def _launch(a, a_mn, b, b_mn, out, beta, mapped_status=False):
     (M, K) = a.shape[::-1] if a_mn else a.shape
     (N, Kb) = b.shape[::-1] if b_mn else b.shape
     assert Kb == K, f"contraction mismatch: {tuple(a.shape)} vs {tuple(b.shape)}"
-    st = nv.status_word(out.device)
+    if mapped_status:
+        nv.poll_host_status(out.device)
+        st = nv.host_status(out.device)[2]
+    else:
+        st = nv.ptr(nv.status_word(out.device))
     with nv.on_device(out.device):
         nv.check(nv.lib().pt_gemm_mn(nv.ptr(a), int(a_mn), nv.ptr(b), int(b_mn), nv.src_code(a.dtype), nv.ptr(out), nv.src_code(out.dtype), M, N, K,
-                                     float(beta), nv.ptr(st), nv.stream(out.device)), "gemm")
-    nv.poll_status(out.device)
+                                     float(beta), st, nv.stream(out.device)), "gemm")
+    if not mapped_status:
+        nv.poll_status(out.device)
     return out
 
 
-def _gemm(a, trans_a, b, trans_b, out_dtype, trans_c, out=None):
+def _gemm(a, trans_a, b, trans_b, out_dtype, trans_c, out=None, mapped_status=False):
     nv.require_cuda(a, b)
     assert a.dim() == 2 and b.dim() == 2, "Only 2D tensors are supported"
     assert a.dtype == b.dtype and a.dtype in (torch.bfloat16, torch.float16), "a and b must both be bf16 or fp16"
@@ -61,7 +66,9 @@ def _gemm(a, trans_a, b, trans_b, out_dtype, trans_c, out=None):
         out = torch.empty((N, M) if trans_c else (M, N), dtype=out_dtype, device=a.device)
     else:
         assert out.is_contiguous() and tuple(out.shape) == ((N, M) if trans_c else (M, N))
-    return _launch(b, b_mn, a, a_mn, out, beta) if trans_c else _launch(a, a_mn, b, b_mn, out, beta)
+    if trans_c:
+        a, a_mn, b, b_mn = b, b_mn, a, a_mn
+    return _launch(a, a_mn, b, b_mn, out, beta, mapped_status)
 
 
 def gemm_impl(a: torch.Tensor, trans_a: bool, b: torch.Tensor, trans_b: bool, out_dtype: torch.dtype, trans_c: bool,
@@ -127,3 +134,13 @@ def act_bias_bwd_impl(grad_out: torch.Tensor, z: Optional[torch.Tensor], act: Op
                                      nv.ptr(dz), nv.ptr(dbias), 0 if dbias is None else nv.src_code(bias_dtype), nv.ptr(partial), parts,
                                      nv.stream(grad_out.device)), "act_bias_bwd")
     return (grad_out if same else dz), dbias
+
+
+def bias_act_dgrad_impl(dz: torch.Tensor, b: torch.Tensor, trans_b: bool) -> torch.Tensor:
+    """dz . op(b)^T: the product again, on the kernel that suits its rows."""
+    return gemm_bias_act_impl(dz, b, not trans_b, None, None, None, dz.dtype, False)[0]
+
+
+def bias_act_wgrad_impl(a: torch.Tensor, dz: torch.Tensor, trans_b: bool, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """a^T . dz in the layout of b; added to `out` when it is given."""
+    return _gemm(a, True, dz, False, dz.dtype if out is None else out.dtype, trans_b, out=out, mapped_status=True)

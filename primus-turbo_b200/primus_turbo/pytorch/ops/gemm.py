@@ -8,7 +8,15 @@ from typing import Optional, Union
 import torch
 from torch.autograd.function import once_differentiable
 
-from ..kernels.gemm.gemm_impl import EPILOGUE_ACTS, act_bias_bwd_impl, gemm_accum_impl, gemm_bias_act_impl, gemm_impl
+from ..kernels.gemm.gemm_impl import (
+    EPILOGUE_ACTS,
+    act_bias_bwd_impl,
+    bias_act_dgrad_impl,
+    bias_act_wgrad_impl,
+    gemm_accum_impl,
+    gemm_bias_act_impl,
+    gemm_impl,
+)
 from .utils import _get_dummy_wgrad, _setup_fused_grad_accum
 
 __all__ = ["gemm", "gemm_bias_act"]
@@ -67,13 +75,13 @@ class GemmBiasActFunction(torch.autograd.Function):
             dz, grad_bias = act_bias_bwd_impl(grad_out, z, ctx.act, a.dtype, ctx.bias_dtype if need_bias else None, need_a or need_b)
         # an empty contraction (no columns for grad_a, no rows for grad_b) is a sum of nothing
         if need_a:                                                                         # dz . op(b)^T
-            grad_a = gemm_impl(dz, False, b, not ctx.trans_b, a.dtype, False) if dz.shape[1] else torch.zeros_like(a)
+            grad_a = bias_act_dgrad_impl(dz, b, ctx.trans_b) if dz.shape[1] else torch.zeros_like(a)
         if need_b and ctx.fuse:
             if a.shape[0]:
-                gemm_accum_impl(a, True, dz, False, b.dtype, ctx.trans_b, out=ctx.main_grad)
+                bias_act_wgrad_impl(a, dz, ctx.trans_b, out=ctx.main_grad)
             grad_b = _get_dummy_wgrad(b.shape, b.dtype, device=b.device)
         elif need_b:                                                                       # a^T . dz
-            grad_b = gemm_impl(a, True, dz, False, b.dtype, ctx.trans_b) if a.shape[0] else torch.zeros_like(b)
+            grad_b = bias_act_wgrad_impl(a, dz, ctx.trans_b) if a.shape[0] else torch.zeros_like(b)
         return grad_a, grad_b, grad_bias, (grad_out if need_residual else None), None, None, None, None
 
 

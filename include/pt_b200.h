@@ -485,7 +485,7 @@ int pt_gemm_bias_act(const void *a, const void *b, int b_mn, int ab_dtype, const
                      int act, int64_t M, int64_t N, int64_t K, int *status, void *stream);
 /* Its element-wise backward: dz [M, N] = dy * act'(z) in the operands' type `dtype` (null: not written), dbias [N] = column sums of
  * the unrounded dz (null: none).  dy of type `dtype` or fp32; z may be null with act 2.  partial fp32 [parts, N] with
- * parts = pt_act_bias_bwd_parts(M, N) when dbias is given.  Same bits every run. */
+ * parts = pt_act_bias_bwd_parts(M, N) when dbias is given (null with one part).  Same bits every run. */
 int pt_act_bias_bwd_parts(int64_t M, int64_t N);
 int pt_act_bias_bwd(const void *dy, int dy_dtype, const void *z, int dtype, int act, int64_t M, int64_t N, void *dz, void *dbias, int dbias_dtype,
                     float *partial, int parts, void *stream);

@@ -10,6 +10,7 @@
 
 #include "act_math.cuh"
 #include "common.cuh"
+#include "gemm_common.cuh"
 #include "sm100_ptx.cuh"
 
 namespace ptb {
@@ -503,7 +504,8 @@ template <typename T, int V> __device__ __forceinline__ void ab_to_f(const Vec<T
 
 template <typename T, typename DyT, int V, bool ACT>
 __global__ void __launch_bounds__(32 * kAbWarps, 4) act_bias_bwd_kernel(const DyT *__restrict__ dy, const T *__restrict__ z, int act, int64_t M, int64_t N,
-                                                                        int64_t rows_per_cta, T *__restrict__ dz, float *__restrict__ partial) {
+                                                                        int64_t rows_per_cta, T *__restrict__ dz, float *__restrict__ partial,
+                                                                        void *__restrict__ dbias, int dbias_dtype) {
     constexpr int kAbRows = sizeof(DyT) == 4 ? 2 : 4;   // rows of a warp in flight
     __shared__ float s_sum[kAbWarps][32 * V + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -569,7 +571,7 @@ __global__ void __launch_bounds__(32 * kAbWarps, 4) act_bias_bwd_kernel(const Dy
             if (po != nullptr) po += step;
         }
     }
-    if (partial == nullptr) return;
+    if (partial == nullptr && dbias == nullptr) return;
 #pragma unroll
     for (int i = 0; i < V; ++i) s_sum[warp][lane * V + i] = sum[i];
     __syncthreads();
@@ -579,7 +581,8 @@ __global__ void __launch_bounds__(32 * kAbWarps, 4) act_bias_bwd_kernel(const Dy
         float t = 0.f;
 #pragma unroll
         for (int w = 0; w < kAbWarps; ++w) t += s_sum[w][c];
-        partial[(int64_t) blockIdx.y * N + n] = t;
+        if (partial != nullptr) partial[(int64_t) blockIdx.y * N + n] = t;
+        else store_from_f32(dbias, dbias_dtype, n, t);   // one CTA per strip: its sum is the gradient
     }
 }
 
@@ -729,19 +732,20 @@ int pt_act_bias_bwd(const void *dy, int dy_dtype, const void *z, int dtype, int 
     PT_REQUIRE(dy_dtype == PT_BF16 || dy_dtype == PT_F16 || dy_dtype == PT_F32, "act_bias backward: bad gradient dtype");
     PT_REQUIRE(!dbias || dbias_dtype == PT_BF16 || dbias_dtype == PT_F16 || dbias_dtype == PT_F32, "act_bias backward: bad bias dtype");
     PT_REQUIRE(act >= PT_ACT_SILU && act <= PT_ACT_GELU_TANH, "act_bias backward: bad activation %d", act);
-    PT_REQUIRE(!dbias || (partial && parts == pt_act_bias_bwd_parts(M, N)), "act_bias backward: bias buffers / part count");
+    PT_REQUIRE(!dbias || (parts == pt_act_bias_bwd_parts(M, N) && (partial || parts == 1)), "act_bias backward: bias buffers / part count");
     if (N == 0) return PT_OK;
     const bool with_act = act != PT_ACT_NONE;
     PT_REQUIRE(M == 0 || (dy && (!with_act || z)), "act_bias backward: null pointer");
     cudaStream_t st = (cudaStream_t) stream;
     const int64_t rows_per_cta = ceil_div(std::max<int64_t>(M, 1), parts > 0 ? parts : pt_act_bias_bwd_parts(M, N));
     const int64_t row_ctas = dbias ? parts : ceil_div(M, rows_per_cta);
-    float *part = dbias ? partial : nullptr;
+    float *part = dbias && parts > 1 ? partial : nullptr;
+    void *direct = dbias && parts == 1 ? dbias : nullptr;
     if (row_ctas > 0) {
         PT_REQUIRE(row_ctas < 65536 && ceil_div(N, 32) < (1ll << 31), "act_bias backward: grid too large");
 #define PT_AB(V_, ACT_, DY_)                                                                                                                      \
     act_bias_bwd_kernel<T, DY_, V_, ACT_><<<dim3((unsigned) ceil_div(N, 32 * V_), (unsigned) row_ctas), 32 * kAbWarps, 0, st>>>(                  \
-        (const DY_ *) dy, (const T *) z, act, M, N, rows_per_cta, (T *) dz, part)
+        (const DY_ *) dy, (const T *) z, act, M, N, rows_per_cta, (T *) dz, part, direct, dbias_dtype)
 #define PT_AB_DY(DY_)                                                                                                                            \
     do {                                                                                                                                          \
         if (N % 8 == 0 && aligned(dy, 8 * sizeof(DY_)) && aligned(z, 16) && aligned(dz, 16)) {                                                    \
@@ -759,7 +763,7 @@ int pt_act_bias_bwd(const void *dy, int dy_dtype, const void *z, int dtype, int 
         if (dtype == PT_BF16) PT_AB_T(__nv_bfloat16); else PT_AB_T(__half);
         PT_LAUNCH_OK();
     }
-    if (dbias) {
+    if (part) {
         PT_SWITCH_SRC(dbias_dtype, T, (bias_grad_kernel<T><<<(unsigned) ceil_div(N, 32), 256, 0, st>>>(partial, parts, N, (T *) dbias)));
         PT_LAUNCH_OK();
     }

@@ -86,25 +86,19 @@ def status_word(device) -> torch.Tensor:
     return _status[idx]
 
 
-def host_status(device):
-    """Per-device status word in pinned host memory, which the kernels of gemm_bias_act, qk_norm_rope and moe_few_tokens write
-    directly (mapped, so the address is the device's too).  Reading it is one host load: a copy and an event per call, as
-    poll_status makes, would cost an operator on one token as much as its kernel."""
-    idx = device.index
-    w = _host_status.get(idx)
+def mapped_status(device):
+    """Address of the device's status word in pinned host memory, which the kernels of gemm_bias_act, qk_norm_rope and
+    moe_few_tokens write directly (mapped, so the address is the device's too).  Raises if a kernel launched earlier has reported
+    an error into it: nothing is waited for, the error of a launch surfaces at a following call, or at check_status().  One host
+    load: a copy and an event per call, as poll_status makes, would cost an operator on one token as much as its kernel."""
+    w = _host_status.get(device.index)
     if w is None:
         t = torch.zeros(1, dtype=torch.int32).pin_memory()
-        w = _host_status[idx] = (t, ctypes.c_int32.from_address(t.data_ptr()), t.data_ptr())
-    return w
-
-
-def poll_host_status(device):
-    """Raises if a kernel launched earlier has reported an error into the host status word (it is not waited for: the error
-    of a launch surfaces at a following call, or at check_status())."""
-    w = _host_status.get(device.index)
-    if w is not None and w[1].value != 0:
+        w = _host_status[device.index] = (t, ctypes.c_int32.from_address(t.data_ptr()), t.data_ptr())
+    if w[1].value != 0:
         code, w[1].value = w[1].value, 0
         _raise(code)
+    return w[2]
 
 
 def _raise(code):
@@ -121,7 +115,7 @@ def check_status(device):
     if code != 0:
         s.zero_()
         _raise(code)
-    poll_host_status(s.device)
+    mapped_status(s.device)
 
 
 def poll_status(device):

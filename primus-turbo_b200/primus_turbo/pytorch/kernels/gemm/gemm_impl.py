@@ -38,11 +38,7 @@ def _launch(a, a_mn, b, b_mn, out, beta, mapped_status=False):
     (M, K) = a.shape[::-1] if a_mn else a.shape
     (N, Kb) = b.shape[::-1] if b_mn else b.shape
     assert Kb == K, f"contraction mismatch: {tuple(a.shape)} vs {tuple(b.shape)}"
-    if mapped_status:
-        nv.poll_host_status(out.device)
-        st = nv.host_status(out.device)[2]
-    else:
-        st = nv.ptr(nv.status_word(out.device))
+    st = nv.mapped_status(out.device) if mapped_status else nv.ptr(nv.status_word(out.device))
     with nv.on_device(out.device):
         nv.check(nv.lib().pt_gemm_mn(nv.ptr(a), int(a_mn), nv.ptr(b), int(b_mn), nv.src_code(a.dtype), nv.ptr(out), nv.src_code(out.dtype), M, N, K,
                                      float(beta), st, nv.stream(out.device)), "gemm")
@@ -90,22 +86,24 @@ def gemm_bias_act_impl(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Op
                        residual: Optional[torch.Tensor], out_dtype: torch.dtype, want_z: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(act(a . op(b) + bias) + residual, the pre-activation in a's type or None) in one kernel."""
     nv.require_cuda(a, b, bias, residual)
-    b_mn = _in_place(b, not trans_b, a, False)
-    a_km = _k_major16(a, False)                          # [M, K]
-    b_km = b if b_mn else _k_major16(b, not trans_b)     # [N, K]
-    if a_km.data_ptr() % 16:             # a view into a larger buffer; TMA reads from 16-byte boundaries
-        a_km = a_km.clone()
-    (M, K), N = a_km.shape, b_km.shape[1 if b_mn else 0]
-    out = torch.empty((M, N), dtype=out_dtype, device=a.device)
-    z = torch.empty((M, N), dtype=a.dtype, device=a.device) if want_z else None
+    device, dtype, (M, K) = a.device, a.dtype, a.shape
+    b_mn = not trans_b and _in_place(b, True, a, False)
+    N = b.shape[0 if trans_b else 1]
+    if K % 8 or not a.is_contiguous():
+        a = _k_major16(a, False)                         # [M, K]
+    if not b_mn and (K % 8 or not trans_b or not b.is_contiguous()):
+        b = _k_major16(b, not trans_b)                   # [N, K]
+    if a.data_ptr() % 16:                                # a view into a larger buffer; TMA reads from 16-byte boundaries
+        a = a.clone()
+    out = torch.empty((M, N), dtype=out_dtype, device=device)
+    z = torch.empty((M, N), dtype=dtype, device=device) if want_z else None
     bias = None if bias is None else bias.contiguous()
     residual = None if residual is None else residual.contiguous()
-    lib = nv.lib()
-    nv.poll_host_status(a.device)
-    with nv.on_device(a.device):
-        nv.check(lib.pt_gemm_bias_act(nv.ptr(a_km), nv.ptr(b_km), int(b_mn), nv.src_code(a.dtype), nv.ptr(bias), 0 if bias is None else nv.src_code(bias.dtype),
-                                      nv.ptr(residual), nv.ptr(out), nv.src_code(out_dtype), nv.ptr(z), EPILOGUE_ACTS[act], M, N, K,
-                                      nv.host_status(a.device)[2], nv.stream(a.device)), "gemm_bias_act")
+    with nv.on_device(device):
+        nv.check(nv.lib().pt_gemm_bias_act(a.data_ptr(), b.data_ptr(), b_mn, nv.src_code(dtype), nv.ptr(bias),
+                                           0 if bias is None else nv.src_code(bias.dtype), nv.ptr(residual), out.data_ptr(),
+                                           nv.src_code(out_dtype), nv.ptr(z), EPILOGUE_ACTS[act], M, N, (K + 7) // 8 * 8,
+                                           nv.mapped_status(device), nv.stream(device)), "gemm_bias_act")
     return out, z
 
 
@@ -117,22 +115,23 @@ def act_bias_bwd_impl(grad_out: torch.Tensor, z: Optional[torch.Tensor], act: Op
     grad_out = grad_out.contiguous()
     if grad_out.dtype not in (dtype, torch.float32):
         grad_out = grad_out.to(torch.float32)
-    M, N = grad_out.shape
+    device, (M, N) = grad_out.device, grad_out.shape
     same = act is None and grad_out.dtype == dtype
-    dz = torch.empty((M, N), dtype=dtype, device=grad_out.device) if want_dz and not same else None
+    dz = torch.empty((M, N), dtype=dtype, device=device) if want_dz and not same else None
     if dz is None and bias_dtype is None:
         return (grad_out if same else None), None
     lib = nv.lib()
-    with nv.on_device(grad_out.device):
+    with nv.on_device(device):
         dbias = partial = None
         parts = 0
         if bias_dtype is not None:
             parts = lib.pt_act_bias_bwd_parts(M, N)
-            dbias = torch.empty((N,), dtype=bias_dtype, device=grad_out.device)
-            partial = torch.empty((parts, N), dtype=torch.float32, device=grad_out.device)
-        nv.check(lib.pt_act_bias_bwd(nv.ptr(grad_out), nv.src_code(grad_out.dtype), nv.ptr(z), nv.src_code(dtype), EPILOGUE_ACTS[act], M, N,
+            dbias = torch.empty((N,), dtype=bias_dtype, device=device)
+            if parts > 1:
+                partial = torch.empty((parts, N), dtype=torch.float32, device=device)
+        nv.check(lib.pt_act_bias_bwd(grad_out.data_ptr(), nv.src_code(grad_out.dtype), nv.ptr(z), nv.src_code(dtype), EPILOGUE_ACTS[act], M, N,
                                      nv.ptr(dz), nv.ptr(dbias), 0 if dbias is None else nv.src_code(bias_dtype), nv.ptr(partial), parts,
-                                     nv.stream(grad_out.device)), "act_bias_bwd")
+                                     nv.stream(device)), "act_bias_bwd")
     return (grad_out if same else dz), dbias
 
 

@@ -29,12 +29,12 @@ def qk_norm_rope_fwd_impl(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tenso
     P, half = cos.shape
     q_out = torch.empty(q.shape, dtype=dtype, device=device)
     k_out = torch.empty(k.shape, dtype=dtype, device=device)
-    nv.poll_host_status(device)
+    status = nv.mapped_status(device)
     with nv.on_device(device):
         nv.check(nv.lib().pt_qk_norm_rope_fwd(q.data_ptr(), k.data_ptr(), nv.src_code(dtype), q_gamma.data_ptr(), k_gamma.data_ptr(),
                                               cos.data_ptr(), sin.data_ptr(), nv.ptr(positions), 0 if positions is None else positions.element_size(),
                                               B, S, P, Hq, Hk, D, 2 * half, _strides(q), _strides(k), eps, interleaved, zero_centered,
-                                              q_out.data_ptr(), k_out.data_ptr(), nv.host_status(device)[2], nv.stream(device)), "qk_norm_rope_fwd")
+                                              q_out.data_ptr(), k_out.data_ptr(), status, nv.stream(device)), "qk_norm_rope_fwd")
     return q_out, k_out
 
 
@@ -50,7 +50,7 @@ def qk_norm_rope_bwd_impl(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     k_in = torch.empty(k.shape, dtype=dtype, device=device)
     dqg, dkg = torch.empty_like(q_gamma), torch.empty_like(k_gamma)
     lib = nv.lib()
-    nv.poll_host_status(device)
+    status = nv.mapped_status(device)
     with nv.on_device(device):
         parts = lib.pt_qk_norm_rope_bwd_parts(B * S, Hq, Hk)
         partial = torch.empty((parts, D), dtype=torch.float32, device=device)
@@ -59,5 +59,5 @@ def qk_norm_rope_bwd_impl(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
                                          0 if positions is None else positions.element_size(), B, S, P, Hq, Hk, D, 2 * half, _strides(dq),
                                          _strides(dk), _strides(q), _strides(k), eps, interleaved, zero_centered, q_in.data_ptr(),
                                          k_in.data_ptr(), dqg.data_ptr(), dkg.data_ptr(), partial.data_ptr(), parts,
-                                         nv.host_status(device)[2], nv.stream(device)), "qk_norm_rope_bwd")
+                                         status, nv.stream(device)), "qk_norm_rope_bwd")
     return q_in, k_in, dqg, dkg

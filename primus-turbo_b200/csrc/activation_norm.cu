@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(32 * kDgLanes) rmsnorm_dgamma_kernel(const flo
 constexpr int kAbWarps = 8;
 
 // The registers are cut to four CTAs per SM: left alone, the compiler converts on arrival and holds 155, one CTA per SM (99 us where
-// this form takes 60, 4096 x 14336 bf16, SiLU).
+// this form takes 56, 4096 x 14336 bf16, SiLU).
 template <typename T, int V> __device__ __forceinline__ void ab_to_f(const Vec<T, V> &r, float (&f)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = an_to_f<T>(r.e[i]);

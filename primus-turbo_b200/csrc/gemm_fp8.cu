@@ -291,7 +291,8 @@ __device__ __forceinline__ void epilogue_store_block(const GemmParams &p, uint32
 // four neighbouring columns of a row, the same columns in each of its eight rows: the bias is loaded once per 32-column chunk, the
 // residual, the pre-activation and the output are accessed in whole 32-byte sectors, and the result is rounded once.  The
 // residual's loads are issued before the accumulators are read, so that they return behind the tensor-memory load.  The lane's 32
-// values pass the activation together, under one branch: its exponentials and divisions then overlap each other.
+// values pass the activation together, under one branch: its exponentials and divisions then overlap each other.  Measured on 8192 x 14336
+// x 4096, bf16: SiLU 621 us, GELU 636, none 607, the plain product 601 (with four values under a branch and four warps SiLU took 994).
 template <int BLOCK_N, typename Release>
 __device__ __forceinline__ void epilogue_fused_block(const GemmParams &p, uint32_t taddr, bool have_acc, int64_t tile_row0, int64_t c_row_end, int n0,
                                                      uint8_t *stg, int lane, int c_begin, int c_end, Release release) {

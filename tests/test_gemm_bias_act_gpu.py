@@ -288,3 +288,14 @@ def test_weight_read_contraction_major(M):
         y = _check(M, N, K, torch.bfloat16, "silu", True, True, trans_b=False)
         assert y.shape == (M, N)
         assert torch.equal(gemm_bias_act(a, b, bias=bias, activation="gelu"), gemm_bias_act(a, b.t().contiguous(), bias=bias, activation="gelu", trans_b=True))
+
+
+@pytest.mark.parametrize("M,N", [(66000, 33000), (40, 2 ** 26)])
+def test_outputs_beyond_32_bits(M, N):
+    from primus_turbo.pytorch.ops import gemm_bias_act
+    a, b, res = _make((M, 64), torch.bfloat16, 1), _make((N, 64), torch.bfloat16, 2, 0.125), None
+    assert M * N > 2 ** 31
+    y = gemm_bias_act(a, b, activation="relu", trans_b=True)
+    A, B = a[-3:].double(), b[-500:].double()
+    want = (A @ B.t()).relu()
+    _assert_within(y[-3:, -500:], want, _mm_bound(A, B.t(), 64) + (HALF[torch.bfloat16] + U) * (want + 1e-3) + 1e-6, "last rows and columns")

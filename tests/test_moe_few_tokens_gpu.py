@@ -170,3 +170,17 @@ def test_same_bits_on_streams_and_in_graphs(T, E, K):
     graphs[0].replay()
     torch.cuda.synchronize()
     assert torch.equal(held[0], want[1])
+
+
+def test_weights_beyond_32_bits():
+    """The last of 150 experts of 7168 x 1024: its gate rows start past 2^31 elements."""
+    from primus_turbo.pytorch.ops import moe_few_tokens
+    E, H, I = 150, 7168, 1024
+    gu, dn = _make((1, 2 * I, H), torch.bfloat16, 1, H ** -0.5), _make((1, H, I), torch.bfloat16, 2, I ** -0.5)
+    big_gu, big_dn = torch.zeros((E, 2 * I, H), dtype=torch.bfloat16, device="cuda"), torch.zeros((E, H, I), dtype=torch.bfloat16, device="cuda")
+    assert (E - 1) * 2 * I * H > 2 ** 31
+    big_gu[-1], big_dn[-1] = gu[0], dn[0]
+    x, p = _make((3, H), torch.bfloat16, 3), torch.rand(3, 1, device="cuda")
+    ids = torch.full((3, 1), E - 1, device="cuda")
+    want, tol = _oracle(x, gu, dn, torch.zeros_like(ids), p, "silu")
+    assert ((moe_few_tokens(x, big_gu, big_dn, ids, p).double() - want).abs() <= tol).all()

@@ -247,3 +247,25 @@ def test_same_bits_every_run_on_another_stream_and_in_a_graph():
         graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, held))
+
+
+def test_offsets_beyond_32_bits():
+    """Tokens more than 2^31 elements apart, read in place and written beyond 2^31 elements of the output."""
+    from primus_turbo.pytorch.ops import qk_norm_rope
+    cos, sin = _tables(4, 64)
+    g = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    wide = torch.empty(3, 2 ** 30 + 128, dtype=torch.bfloat16, device="cuda")
+    q, k = wide[:, 64:64 + 4 * 64].view(3, 4, 64), wide[:, -128:].view(3, 2, 64)
+    q.copy_(_make((3, 4, 64), torch.bfloat16, 1))
+    k.copy_(_make((3, 2, 64), torch.bfloat16, 2))
+    _check(q, k, g, g, cos, sin, None, False, False, 1e-6, _make((3, 4, 64), torch.bfloat16, 3), _make((3, 2, 64), torch.bfloat16, 4))
+    del wide
+    T = 2 ** 31 // (8 * 128) + 5
+    big = torch.empty(T, 8, 128, dtype=torch.bfloat16, device="cuda")
+    big[-3:].copy_(_make((3, 8, 128), torch.bfloat16, 5))
+    g = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    cos, sin = _tables(8, 128)
+    pos = torch.arange(T, device="cuda") % 8
+    out = qk_norm_rope(big, big[:, :1], g, g, cos, sin, positions=pos)
+    want = qk_norm_rope(big[-3:], big[-3:, :1], g, g, cos, sin, positions=pos[-3:])
+    assert torch.equal(out[0][-3:], want[0]) and torch.equal(out[1][-3:], want[1])

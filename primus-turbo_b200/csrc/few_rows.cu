@@ -515,16 +515,34 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
                     store4_from_f32(a.out, a.out_dtype, o0 + u * o_step, v[u]);
                 }
             } else {
+                uint32_t res[kAtOnce][4];   // raw, all on their way before the first is used
+                if (a.residual != nullptr) {
+                    auto fetch = [&](auto *p) {
+#pragma unroll
+                        for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (inside(u) && f0 + 32 * i < a.n) res[u][i] = p[o0 + u * o_step + 32 * i];
+                    };
+                    if (a.out_dtype == PT_F32) fetch(reinterpret_cast<const uint32_t *>(a.residual));
+                    else fetch(reinterpret_cast<const uint16_t *>(a.residual));
+                }
+                if (a.z != nullptr) {
+#pragma unroll
+                    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (inside(u) && f0 + 32 * i < a.n) store_from_f32(a.z, zt, o0 + u * o_step + 32 * i, v[u][i]);
+                }
+                act_any_all<kAtOnce>(a.act, v);
 #pragma unroll
                 for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if (!inside(u) || f0 + 32 * i >= a.n) continue;
-                        const int64_t o = o0 + u * o_step + 32 * i;
-                        if (a.z != nullptr) store_from_f32(a.z, zt, o, v[u][i]);
-                        float y = act_any(a.act, v[u][i]);
-                        if (a.residual != nullptr) y += load_as_f32(a.residual, a.out_dtype, o);
-                        store_from_f32(a.out, a.out_dtype, o, y);
+                        if (a.residual != nullptr)
+                            v[u][i] += a.out_dtype == PT_F32 ? __uint_as_float(res[u][i]) : a.out_dtype == PT_BF16 ? lo_f32<__nv_bfloat16>(res[u][i]) : lo_f32<__half>(res[u][i]);
+                        store_from_f32(a.out, a.out_dtype, o0 + u * o_step + 32 * i, v[u][i]);
                     }
             }
         }

@@ -65,7 +65,7 @@ struct GemmParams {
     // HP_EPI: C = act(acc + bias[n]) + residual[m, n]; z (the operands' type) receives acc + bias.  Each may be null.
     const void *bias, *residual;
     void *z;
-    int bias_dtype, act;
+    int bias_dtype, act, bias_vec;   // bias_vec: four neighbours of the bias may be loaded at once
 };
 
 // How a stage of an MN-major operand arrives: boxes of 128 bytes of row indices x the stage's contraction rows, one after the
@@ -287,47 +287,101 @@ __device__ __forceinline__ void epilogue_store_block(const GemmParams &p, uint32
     }
 }
 
+// Four neighbouring values of every row of a lane, in type T: raw loads, conversion and store.
+template <typename T> struct Quad {
+    static __device__ __forceinline__ uint4 load(const void *p) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(p);
+        return make_uint4(w.x, w.y, 0u, 0u);
+    }
+    static __device__ __forceinline__ void add(const uint4 &w, float (&v)[4]) {
+        v[0] += lo_f32<T>(w.x); v[1] += hi_f32<T>(w.x); v[2] += lo_f32<T>(w.y); v[3] += hi_f32<T>(w.y);
+    }
+    static __device__ __forceinline__ void store(void *p, const float (&v)[4]) {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    }
+};
+template <> struct Quad<float> {
+    static __device__ __forceinline__ uint4 load(const void *p) { return *reinterpret_cast<const uint4 *>(p); }
+    static __device__ __forceinline__ void add(const uint4 &w, float (&v)[4]) {
+        v[0] += __uint_as_float(w.x); v[1] += __uint_as_float(w.y); v[2] += __uint_as_float(w.z); v[3] += __uint_as_float(w.w);
+    }
+    static __device__ __forceinline__ void store(void *p, const float (&v)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+};
+constexpr int kEpiRows = 8;   // a lane's rows of a 32-row chunk: its first, + 4, + 8, ...
+template <typename T> __device__ __forceinline__ void quad_load_rows(const void *p, int64_t o0, int64_t ld, int rows_left, uint4 (&w)[kEpiRows]) {
+    const T *src = reinterpret_cast<const T *>(p) + o0;
+#pragma unroll
+    for (int i = 0; i < kEpiRows; ++i, src += 4 * ld)
+        if (4 * i < rows_left) w[i] = Quad<T>::load(src);
+}
+template <typename T> __device__ __forceinline__ void quad_store_rows(void *p, int64_t o0, int64_t ld, int rows_left, const float (&v)[kEpiRows][4]) {
+    T *dst = reinterpret_cast<T *>(p) + o0;
+    if (rows_left >= 29) {   // 4 * 7 + 1: every row of the lane lies inside
+#pragma unroll
+        for (int i = 0; i < kEpiRows; ++i, dst += 4 * ld) Quad<T>::store(dst, v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kEpiRows; ++i, dst += 4 * ld)
+            if (4 * i < rows_left) Quad<T>::store(dst, v[i]);
+    }
+}
+template <typename T> __device__ __forceinline__ void quad_add_rows(const uint4 (&w)[kEpiRows], float (&v)[kEpiRows][4]) {
+#pragma unroll
+    for (int i = 0; i < kEpiRows; ++i) Quad<T>::add(w[i], v[i]);
+}
+
 // The same for HP_EPI.  The accumulators are staged as fp32 and everything element-wise happens on the way out, where a lane holds
 // four neighbouring columns of a row, the same columns in each of its eight rows: the bias is loaded once per 32-column chunk, the
 // residual, the pre-activation and the output are accessed in whole 32-byte sectors, and the result is rounded once.  The
 // residual's loads are issued before the accumulators are read, so that they return behind the tensor-memory load.  The lane's 32
-// values pass the activation together, under one branch: its exponentials and divisions then overlap each other.  Measured on 8192 x 14336
-// x 4096, bf16: SiLU 621 us, GELU 636, none 607, the plain product 601 (with four values under a branch and four warps SiLU took 994).
+// values pass every step together, under one branch on its kind: with two warps per scheduler the epilogue is bound by the number of
+// its instructions and what they wait for each other.  Measured on 8192 x 14336 x 4096, bf16: SiLU 621 us, GELU 636, none 607, the plain
+// product 601 (with four values under a branch and four warps SiLU took 994).
 template <int BLOCK_N, typename Release>
 __device__ __forceinline__ void epilogue_fused_block(const GemmParams &p, uint32_t taddr, bool have_acc, int64_t tile_row0, int64_t c_row_end, int n0,
                                                      uint8_t *stg, int lane, int c_begin, int c_end, Release release) {
-    constexpr int kRows = 8;   // a lane's rows of a chunk: row_in_pass, + 4, + 8, ...
     const int n_end = min(p.N, n0 + BLOCK_N);
     const int sub = lane & 7, row_in_pass = lane >> 3;
-    const int z_dtype = p.a_fmt ? PT_BF16 : PT_F16;
-    const int rows = (int) min((int64_t) 32, c_row_end - tile_row0);   // rows of this warp inside the matrix (may be negative)
+    const int rows_left = (int) min((int64_t) 32, c_row_end - tile_row0) - row_in_pass;   // the lane's row i lies inside while 4 i < rows_left
+    const int kind = p.c_dtype;
 #pragma unroll 1
     for (int c = c_begin; c < c_end; ++c) {
         const int gcol = n0 + c * 32 + sub * 4;
         const bool vec = p.vec_store_ok && gcol + 4 <= n_end;
         const int64_t o0 = (tile_row0 + row_in_pass) * p.ldc + gcol;
-        uint4 res[kRows];   // raw: converting here would wait for every load in turn
+        uint4 res[kEpiRows];   // raw: converting here would wait for every load in turn
         if (p.residual != nullptr && vec) {
-            if (p.c_dtype == PT_F32) {
-                const float *src = reinterpret_cast<const float *>(p.residual) + o0;
+            if (kind == PT_F32) quad_load_rows<float>(p.residual, o0, p.ldc, rows_left, res);
+            else quad_load_rows<__half>(p.residual, o0, p.ldc, rows_left, res);   // either 16-bit type
+        } else if (p.residual != nullptr) {   // element by element, one to a word
+            auto fetch = [&](auto *src) {
 #pragma unroll
-                for (int i = 0; i < kRows; ++i)
-                    if (i * 4 + row_in_pass < rows) res[i] = *reinterpret_cast<const uint4 *>(src + (int64_t) (4 * i) * p.ldc);
-            } else {
-                const uint16_t *src = reinterpret_cast<const uint16_t *>(p.residual) + o0;
-#pragma unroll
-                for (int i = 0; i < kRows; ++i)
-                    if (i * 4 + row_in_pass < rows) {
-                        const uint2 w = *reinterpret_cast<const uint2 *>(src + (int64_t) (4 * i) * p.ldc);
-                        res[i].x = w.x; res[i].y = w.y;
-                    }
-            }
+                for (int i = 0; i < kEpiRows; ++i) {
+                    if (4 * i >= rows_left) continue;
+                    const auto *row = src + o0 + (int64_t) (4 * i) * p.ldc;
+                    if (gcol < n_end) res[i].x = row[0];
+                    if (gcol + 1 < n_end) res[i].y = row[1];
+                    if (gcol + 2 < n_end) res[i].z = row[2];
+                    if (gcol + 3 < n_end) res[i].w = row[3];
+                }
+            };
+            if (kind == PT_F32) fetch(reinterpret_cast<const uint32_t *>(p.residual));
+            else fetch(reinterpret_cast<const uint16_t *>(p.residual));
         }
-        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        uint4 bias_raw = {};
         if (p.bias != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (gcol + i < n_end) bias[i] = load_as_f32(p.bias, p.bias_dtype, gcol + i);
+            if (p.bias_vec && gcol + 4 <= n_end) bias_raw = load4_raw(p.bias, p.bias_dtype, gcol);
+            else {
+                const int last = n_end - 1;   // columns past the end take its bias, and are not stored
+                auto fetch = [&](auto *src) {
+                    bias_raw.x = src[min(gcol, last)]; bias_raw.y = src[min(gcol + 1, last)]; bias_raw.z = src[min(gcol + 2, last)]; bias_raw.w = src[min(gcol + 3, last)];
+                };
+                if (p.bias_dtype == PT_F32) fetch(reinterpret_cast<const uint32_t *>(p.bias));
+                else {
+                    fetch(reinterpret_cast<const uint16_t *>(p.bias));
+                    bias_raw = make_uint4(bias_raw.x | bias_raw.y << 16, bias_raw.z | bias_raw.w << 16, 0u, 0u);   // as load4_raw has them
+                }
+            }
         }
         {
             uint32_t r[32];
@@ -349,47 +403,53 @@ __device__ __forceinline__ void epilogue_fused_block(const GemmParams &p, uint32
                 *reinterpret_cast<uint4 *>(my + 16 * (i ^ (lane & 7))) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
         }
         __syncwarp();
-        float v[kRows][4];
+        float v[kEpiRows][4];
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
+        for (int i = 0; i < kEpiRows; ++i) {
             const int rr = i * 4 + row_in_pass;
             const float4 acc = *reinterpret_cast<const float4 *>(stg + rr * 128 + (sub ^ (rr & 7)) * 16);
-            v[i][0] = acc.x + bias[0]; v[i][1] = acc.y + bias[1]; v[i][2] = acc.z + bias[2]; v[i][3] = acc.w + bias[3];
+            v[i][0] = acc.x; v[i][1] = acc.y; v[i][2] = acc.z; v[i][3] = acc.w;
+        }
+        if (p.bias != nullptr) {
+            float bias[4];
+            raw4_as_f32(bias_raw, p.bias_dtype, bias);
+#pragma unroll
+            for (int i = 0; i < kEpiRows; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i][e] += bias[e];
         }
         if (p.z != nullptr && vec) {
-#pragma unroll
-            for (int i = 0; i < kRows; ++i)
-                if (i * 4 + row_in_pass < rows) store4_from_f32(p.z, z_dtype, o0 + (int64_t) (4 * i) * p.ldc, v[i]);
+            if (p.a_fmt) quad_store_rows<__nv_bfloat16>(p.z, o0, p.ldc, rows_left, v);
+            else quad_store_rows<__half>(p.z, o0, p.ldc, rows_left, v);
         } else if (p.z != nullptr) {
 #pragma unroll
-            for (int i = 0; i < kRows; ++i)
+            for (int i = 0; i < kEpiRows; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (i * 4 + row_in_pass < rows && gcol + e < n_end) store_from_f32(p.z, z_dtype, o0 + (int64_t) (4 * i) * p.ldc + e, v[i][e]);
+                    if (4 * i < rows_left && gcol + e < n_end) store_from_f32(p.z, p.a_fmt ? PT_BF16 : PT_F16, o0 + (int64_t) (4 * i) * p.ldc + e, v[i][e]);
         }
-        act_any_all<kRows>(p.act, v);
+        act_any_all<kEpiRows>(p.act, v);
         if (vec) {
-#pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                if (i * 4 + row_in_pass >= rows) continue;
-                if (p.residual != nullptr) {
-                    float x[4];
-                    raw4_as_f32(res[i], p.c_dtype, x);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[i][e] += x[e];
-                }
-                store4_from_f32(p.C, p.c_dtype, o0 + (int64_t) (4 * i) * p.ldc, v[i]);
+            if (p.residual != nullptr) {
+                if (kind == PT_BF16) quad_add_rows<__nv_bfloat16>(res, v);
+                else if (kind == PT_F16) quad_add_rows<__half>(res, v);
+                else quad_add_rows<float>(res, v);
             }
+            if (kind == PT_BF16) quad_store_rows<__nv_bfloat16>(p.C, o0, p.ldc, rows_left, v);
+            else if (kind == PT_F16) quad_store_rows<__half>(p.C, o0, p.ldc, rows_left, v);
+            else quad_store_rows<float>(p.C, o0, p.ldc, rows_left, v);
         } else {
 #pragma unroll
-            for (int i = 0; i < kRows; ++i)
+            for (int i = 0; i < kEpiRows; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (i * 4 + row_in_pass >= rows || gcol + e >= n_end) continue;
-                    const int64_t o = o0 + (int64_t) (4 * i) * p.ldc + e;
+                    if (4 * i >= rows_left || gcol + e >= n_end) continue;
                     float y = v[i][e];
-                    if (p.residual != nullptr) y += load_as_f32(p.residual, p.c_dtype, o);
-                    store_from_f32(p.C, p.c_dtype, o, y);
+                    if (p.residual != nullptr) {
+                        const uint32_t w = e == 0 ? res[i].x : e == 1 ? res[i].y : e == 2 ? res[i].z : res[i].w;
+                        y += kind == PT_F32 ? __uint_as_float(w) : kind == PT_BF16 ? lo_f32<__nv_bfloat16>(w) : lo_f32<__half>(w);
+                    }
+                    store_from_f32(p.C, kind, o0 + (int64_t) (4 * i) * p.ldc + e, y);
                 }
         }
         __syncwarp();
@@ -942,6 +1002,7 @@ static int gemm_bias_act_host(const void *a, const void *b, int b_mn, int ab_dty
     p.b_mn = b_mn; p.bias = bias; p.bias_dtype = bias_dtype; p.residual = residual; p.z = z; p.act = act;
     const int esize = c_dtype == PT_F32 ? 4 : 2;
     p.vec_store_ok = N % 4 == 0 && aligned(c, 4 * esize) && aligned(residual, 4 * esize) && aligned(z, 8);
+    p.bias_vec = aligned(bias, bias_dtype == PT_F32 ? 16 : 8);
     p.a_fmt = p.b_fmt = ab_dtype == PT_BF16 ? 1 : 0;
     p.G = 1; p.b_group_rows = N; p.status = status;
     p.raster_m = raster_rows(M, 2 * K);

@@ -871,9 +871,14 @@ static int dispatch_block_n(int block_n, const void *a, int64_t a_rows, const vo
     }
     if (block_n == 0) block_n = default_block_n(MODE, p.N);
     const int64_t tiles = m_blocks_bound * ceil_div(p.N, block_n);
+    if constexpr (MODE != GEMM_HP_EPI) {   // 240 columns: the block-scaled modes' default; no call asks the fused epilogue for it
+        if (block_n == 240) return launch_gemm<240, MODE>(a, a_rows, b, b_rows, p, mx, max_ctas, tiles, st);
+    }
+    if constexpr (MODE != GEMM_HP_EPI) {   // 240 columns: the block-scaled modes' default; no call asks the fused epilogue for it
+        if (block_n == 240) return launch_gemm<240, MODE>(a, a_rows, b, b_rows, p, mx, max_ctas, tiles, st);
+    }
     switch (block_n) {
     case 128: return launch_gemm<128, MODE>(a, a_rows, b, b_rows, p, mx, max_ctas, tiles, st);
-    case 240: return launch_gemm<240, MODE>(a, a_rows, b, b_rows, p, mx, max_ctas, tiles, st);
     case 256: return launch_gemm<256, MODE>(a, a_rows, b, b_rows, p, mx, max_ctas, tiles, st);
     default: return set_error(PT_ERR_INVALID, "GEMM: BLOCK_N %d is not built (128, 240, 256)", block_n);
     }

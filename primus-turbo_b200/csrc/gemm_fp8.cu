@@ -874,9 +874,6 @@ static int dispatch_block_n(int block_n, const void *a, int64_t a_rows, const vo
     if constexpr (MODE != GEMM_HP_EPI) {   // 240 columns: the block-scaled modes' default; no call asks the fused epilogue for it
         if (block_n == 240) return launch_gemm<240, MODE>(a, a_rows, b, b_rows, p, mx, max_ctas, tiles, st);
     }
-    if constexpr (MODE != GEMM_HP_EPI) {   // 240 columns: the block-scaled modes' default; no call asks the fused epilogue for it
-        if (block_n == 240) return launch_gemm<240, MODE>(a, a_rows, b, b_rows, p, mx, max_ctas, tiles, st);
-    }
     switch (block_n) {
     case 128: return launch_gemm<128, MODE>(a, a_rows, b, b_rows, p, mx, max_ctas, tiles, st);
     case 256: return launch_gemm<256, MODE>(a, a_rows, b, b_rows, p, mx, max_ctas, tiles, st);

@@ -95,8 +95,8 @@ def gemm_bias_act_impl(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Op
         b = _k_major16(b, not trans_b)                   # [N, K]
     if a.data_ptr() % 16:                                # a view into a larger buffer; TMA reads from 16-byte boundaries
         a = a.clone()
-    out = torch.empty((M, N), dtype=out_dtype, device=device)
-    z = torch.empty((M, N), dtype=dtype, device=device) if want_z else None
+    out = a.new_empty((M, N)) if out_dtype == dtype else torch.empty((M, N), dtype=out_dtype, device=device)
+    z = a.new_empty((M, N)) if want_z else None
     bias = None if bias is None else bias.contiguous()
     residual = None if residual is None else residual.contiguous()
     with nv.on_device(device):

@@ -15,7 +15,7 @@ def moe_few_tokens_impl(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tens
     K = topk_indices.shape[1]
     if x.data_ptr() % 16:      # a view into a larger buffer; TMA reads from 16-byte boundaries
         x = x.clone()
-    out = torch.empty((T, H), dtype=x.dtype, device=x.device)
+    out = torch.empty_like(x)
     lib = nv.lib()
     nbytes = lib.pt_moe_few_tokens_scratch_bytes(T, K, I)
     scratch = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)

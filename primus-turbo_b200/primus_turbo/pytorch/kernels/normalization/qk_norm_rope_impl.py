@@ -27,8 +27,8 @@ def qk_norm_rope_fwd_impl(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tenso
     B, S = _extents(q)
     (Hq, D), Hk = q.shape[-2:], k.shape[-2]
     P, half = cos.shape
-    q_out = torch.empty(q.shape, dtype=dtype, device=device)
-    k_out = torch.empty(k.shape, dtype=dtype, device=device)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     status = nv.mapped_status(device)
     with nv.on_device(device):
         nv.check(nv.lib().pt_qk_norm_rope_fwd(q.data_ptr(), k.data_ptr(), nv.src_code(dtype), q_gamma.data_ptr(), k_gamma.data_ptr(),
@@ -46,8 +46,8 @@ def qk_norm_rope_bwd_impl(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     B, S = _extents(q)
     (Hq, D), Hk = q.shape[-2:], k.shape[-2]
     P, half = cos.shape
-    q_in = torch.empty(q.shape, dtype=dtype, device=device)
-    k_in = torch.empty(k.shape, dtype=dtype, device=device)
+    q_in = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_in = torch.empty_like(k, memory_format=torch.contiguous_format)
     dqg, dkg = torch.empty_like(q_gamma), torch.empty_like(k_gamma)
     lib = nv.lib()
     status = nv.mapped_status(device)

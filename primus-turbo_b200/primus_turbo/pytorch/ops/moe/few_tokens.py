@@ -38,7 +38,9 @@ def moe_few_tokens(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, t
     assert T <= MAX_TOKENS and 1 <= E <= MAX_EXPERTS and 1 <= K <= MAX_TOP_K and T * K <= MAX_SLOTS, \
         f"moe_few_tokens: takes at most {MAX_TOKENS} tokens, {MAX_EXPERTS} experts, {MAX_TOP_K} per token and {MAX_SLOTS} slots (got {T}, {E}, {K}); " \
         "longer inputs go through token_permute and grouped_gemm"
-    assert all(t.device == x.device for t in (gate_up, down, topk_indices, topk_probs)), "moe_few_tokens: all tensors must be on one device"
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate_up, down, topk_probs)):
+    index = x.get_device()
+    assert gate_up.get_device() == index and down.get_device() == index and topk_indices.get_device() == index and topk_probs.get_device() == index, \
+        "moe_few_tokens: all tensors must be on one device"
+    if torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad or down.requires_grad or topk_probs.requires_grad):
         raise RuntimeError("moe_few_tokens has no backward: call it under torch.no_grad(), or train through token_permute and grouped_gemm")
     return moe_few_tokens_impl(x.contiguous(), gate_up.contiguous(), down.contiguous(), topk_indices.contiguous(), topk_probs.contiguous(), act_type)

@@ -97,16 +97,17 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor, k_gamm
     (i, i + R / 2), or (2 i, 2 i + 1) when interleaved, by cos / sin of the token's position; elements from R on pass through.
     positions: int32 / int64 of the shape [..., tokens]; None: 0, 1, ... along the token dimension.  A position outside of
     [0, P) gives zeros for its token and an error at a following call.  Differentiable in q, k and the gains."""
-    tensors = (q, k, q_gamma, k_gamma, cos, sin) if positions is None else (q, k, q_gamma, k_gamma, cos, sin, positions)
-    device, dtype, D = q.device, q.dtype, q.shape[-1]
-    for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError("primus_turbo (B200) operators take CUDA tensors only; there is no CPU path")
-        assert t.device == device, "qk_norm_rope: all tensors must be on one device"
+    index, dtype, D = q.get_device(), q.dtype, q.shape[-1]
+    for t in (q, k, q_gamma, k_gamma, cos, sin) if positions is None else (q, k, q_gamma, k_gamma, cos, sin, positions):
+        if t.get_device() != index or index < 0:
+            if not t.is_cuda:
+                raise RuntimeError("primus_turbo (B200) operators take CUDA tensors only; there is no CPU path")
+            raise AssertionError("qk_norm_rope: all tensors must be on one device")
     assert dtype in (torch.bfloat16, torch.float16, torch.float32), f"qk_norm_rope: unsupported dtype {dtype}"
     assert k.dtype == dtype == q_gamma.dtype == k_gamma.dtype, "qk_norm_rope: q, k and the gains must have one dtype"
     assert q.dim() >= 3, f"qk_norm_rope: q must be [..., tokens, heads, D], got {tuple(q.shape)}"
-    assert k.dim() == q.dim() and k.shape[:-2] == q.shape[:-2] and k.shape[-1] == D, \
+    lead = q.shape[:-2]
+    assert k.dim() == q.dim() and k.shape[:-2] == lead and k.shape[-1] == D, \
         f"qk_norm_rope: q {tuple(q.shape)} and k {tuple(k.shape)} must agree but in their heads"
     assert q_gamma.shape == (D,) and k_gamma.shape == (D,), "qk_norm_rope: the gains must be [D]"
     assert cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape, \
@@ -114,7 +115,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor, k_gamm
     assert 2 * cos.shape[1] <= D, f"qk_norm_rope: the tables rotate {2 * cos.shape[1]} elements of heads of {D}"
     if positions is not None:
         assert positions.dtype in (torch.int32, torch.int64), "qk_norm_rope: positions must be int32 or int64"
-        assert positions.shape == q.shape[:-2], f"qk_norm_rope: positions {tuple(positions.shape)} must be [..., tokens] {tuple(q.shape[:-2])}"
+        assert positions.shape == lead, f"qk_norm_rope: positions {tuple(positions.shape)} must be [..., tokens] {tuple(q.shape[:-2])}"
         positions = positions.contiguous()
     else:
         assert q.shape[-3] <= cos.shape[0], f"qk_norm_rope: {q.shape[-3]} tokens need as many rows of cos / sin, got {cos.shape[0]}"

@@ -11,8 +11,8 @@
 // neighbouring lanes and never leaves their registers: a lane holds whole pairs (the vectors at i and at i + R / 2), so the
 // rotation needs no exchange and the norm one shuffle reduction.  A warp takes heads of one token only: the token's cosines and
 // sines and the gains are converted once for all of them.  Arithmetic in fp32, one rounding at the end.
-// Measured (B200): forward 8192 x 72 heads of 128, bf16, 64.6 us (4.7 TB/s); forward and backward of 8191 x 40 heads, fp16, half rotated, 104 us
-// (36, 64 and 4; 4.1 TB/s of the five passes).  Issue slots are 0.70 and 0.58 busy and loads in flight bound the rest.
+// Measured (B200): forward 8192 x 72 heads of 128, bf16, 61.7 us (4.9 TB/s); forward and backward of 8191 x 40 heads, fp16, half rotated, 99.6 us
+// (34, 62 and 4; 4.2 TB/s of the five passes).  Issue slots are 0.70 and 0.58 busy and loads in flight bound the rest.
 #include <algorithm>
 #include <type_traits>
 

@@ -95,6 +95,8 @@ def gemm_bias_act_impl(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Op
         b = _k_major16(b, not trans_b)                   # [N, K]
     if a.data_ptr() % 16:                                # a view into a larger buffer; TMA reads from 16-byte boundaries
         a = a.clone()
+    if b.data_ptr() % 16:
+        b = b.clone()
     out = a.new_empty((M, N)) if out_dtype == dtype else torch.empty((M, N), dtype=out_dtype, device=device)
     z = a.new_empty((M, N)) if want_z else None
     bias = None if bias is None else bias.contiguous()

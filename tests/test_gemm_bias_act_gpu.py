@@ -149,6 +149,53 @@ def test_gradients_without_bias_other_layouts_and_types():
     _check(200, 264, 128, bf, None, True, False, out_dtype=torch.float32, grad=True)
 
 
+@pytest.mark.parametrize("M", [4, 300])
+@pytest.mark.parametrize("trans_b", [True, False])
+@pytest.mark.parametrize("off", [1, 2, 4])
+def test_views_off_the_16_byte_boundary(M, trans_b, off):
+    """Every tensor a view that starts `off` elements into a buffer: the bits of aligned copies, forward and backward."""
+    from primus_turbo.pytorch.ops import gemm_bias_act
+    N, K, bf = 264, 96, torch.bfloat16
+    shapes = [(M, K), (N, K) if trans_b else (K, N), (N,), (M, N), (M, N)]
+
+    def run(shift):
+        ts = []
+        for i, s in enumerate(shapes):
+            buf = torch.zeros(math.prod(s) + 8, dtype=bf, device="cuda")
+            v = buf[shift:shift + math.prod(s)].view(s)
+            v.copy_(_make(s, bf, i + 1, 0.5))
+            ts.append(v)
+        a, b, bias, res = (t.requires_grad_() for t in ts[:4])
+        y = gemm_bias_act(a, b, bias=bias, activation="silu", residual=res, trans_b=trans_b)
+        return (y, *torch.autograd.grad(y, (a, b, bias, res), ts[4]))
+
+    for got, want in zip(run(off), run(0)):
+        assert torch.equal(got, want)
+
+
+def test_expanded_and_strided_inputs():
+    """Broadcast and transposed tensors are the values that they show; a broadcast leaf gets the sum over its copies."""
+    from primus_turbo.pytorch.ops import gemm_bias_act
+    M, N, K, bf = 40, 136, 64, torch.bfloat16
+    row, col, b0, r0 = _make((1, K), bf, 1), _make((N, 1), bf, 2), _make((1,), bf, 3), _make((M,), bf, 4)
+    a, b, bias, res = row.expand(M, K), col.expand(N, K), b0.expand(N), r0[:, None].expand(M, N)
+    plain = [t.contiguous() for t in (a, b, bias, res)]
+    assert torch.equal(gemm_bias_act(a, b, bias, "gelu", res, trans_b=True), gemm_bias_act(plain[0], plain[1], plain[2], "gelu", plain[3], trans_b=True))
+    w = _make((K, N), bf, 5)
+    assert torch.equal(gemm_bias_act(a, w.t(), bias, "gelu", res, trans_b=True), gemm_bias_act(plain[0], w.t().contiguous(), bias, "gelu", res, trans_b=True))
+    big = _make((2 * M, 2 * N), bf, 6)
+    assert torch.equal(gemm_bias_act(a, w, residual=big[::2, ::2]), gemm_bias_act(plain[0], w, residual=big[::2, ::2].contiguous()))
+    res_leaf = r0.clone().requires_grad_()
+    dy = _make((M, N), bf, 7)
+    gemm_bias_act(a, w, residual=res_leaf[:, None].expand(M, N)).backward(dy)
+    assert torch.equal(res_leaf.grad, dy.sum(1, keepdim=True)[:, 0])
+    x = plain[0].clone().requires_grad_()
+    gemm_bias_act(x, w, activation="silu").sum().backward()            # the gradient arrives with strides of zero
+    y = plain[0].clone().requires_grad_()
+    gemm_bias_act(y, w, activation="silu").backward(torch.ones(M, N, dtype=bf, device="cuda"))
+    assert torch.equal(x.grad, y.grad)
+
+
 def test_gradients_that_are_not_asked_for():
     from primus_turbo.pytorch.ops import gemm_bias_act
     a, b, bias = _make((40, 64), torch.bfloat16, 1), _make((96, 64), torch.bfloat16, 2), _make((96,), torch.bfloat16, 3)

@@ -6,10 +6,12 @@
 // its narrow one (N = 16 .. 256), so that a CTA streams 16 KiB weight blocks [128 features][64 of K] through a TMA ring and the
 // tensor core takes each of them in four instructions, far faster than it arrives.  Blocks of up to 128 tokens: two CTAs to an SM with
 // about 100 KiB each on their way, which covers the memory latency (148 SMs x 200 KiB = 29 MiB in flight) and lets one CTA's start and
-// write-out hide behind the other's stream.  Blocks of 192 and 256: one CTA with 200 KiB; there the stages out of L2 bound it.
+// write-out hide behind the other's stream.  Up to 192: one CTA with 200 KiB and more warps for the write-out.  Up to 256: pairs of CTAs whose
+// tensor cores multiply 256 features together (cta_group::2), each holding half of the tokens, because there what an SM takes in from L2
+// (about 108 GB/s) bounds it: 512 x 4096 x 4096 24.8 us by blocks of 192, 21.1 by pairs.
 //   The contraction is split over the CTAs of a cluster when the features alone would leave SMs idle: every CTA puts its partial
 // [tokens][128] block of fp32 sums into its own shared memory and the CTAs add each other's blocks for their share of the tokens
-// through distributed shared memory, in the order of their ranks.  So there is no workspace, no counter and no atomic: results do
+// through distributed shared memory, beginning with their own and going on by rank.  So there is no workspace, no counter and no atomic: results do
 // not depend on timing, and calls on different streams or in different graphs share nothing.
 //
 //   warp 0      producer (TMA; for experts also which tokens chose them)
@@ -18,7 +20,7 @@
 //   all         sum over the cluster, epilogue, write-out
 //
 // Measured (B200, bf16, replayed graphs, inputs beyond L2): 1 x 14336 x 4096 (rows, features, K) 22.0 us, 5.3 TB/s of weights; 1 x 64128 x 4096
-// 81 us, 6.5 TB/s; 333 x 4096 x 4096 20.9 us, 0.53 PFLOP/s.  One token through eight experts of 7168 x 2048 114 us, 6.2 TB/s; 64 tokens on 28
+// 81 us, 6.5 TB/s; 64 x 4096 x 4096 12.8 us; 129 x 4096 x 4096 13.6 us; 333 x 4096 x 4096 19.0 us, 0.59 PFLOP/s.  One token through eight experts of 7168 x 2048 114 us, 6.2 TB/s; 64 tokens on 28
 // of 32 such experts 388 us, 6.4 TB/s.
 //
 // Mixture, two kernels:
@@ -32,6 +34,7 @@
 //            fetched before the first kernel has finished (programmatic dependent launch): weights and routing do not depend
 //            on it.
 #include <algorithm>
+#include <cmath>
 
 #include "act_math.cuh"
 #include "common.cuh"
@@ -46,18 +49,20 @@ constexpr int kFrABytes = kFrFeat * 128;  // a weight block: 128 rows of 64 16-b
 constexpr int kFrMaxSlots = 2048;         // tokens x experts per token
 constexpr int kFrMaxTopK = 32;
 constexpr int kFrMaxSplit = 8;            // CTAs of a cluster
+constexpr int kFrPairTok = 256;           // the block that pairs of CTAs take
 
 enum FewRowsKind { FR_LINEAR = 0, FR_GATE_UP = 1, FR_DOWN = 2 };
 
 struct FewRowsArgs {
     int rows;                // LINEAR: M; else tokens
     int n, k;                // features of the output (GATE_UP: of one half), contraction length
-    int split;               // CTAs of a cluster
+    int split;               // CTAs (wide blocks: pairs of CTAs) of a cluster
     int fmt;                 // 0 = fp16, 1 = bf16 operands
     void *out;               // LINEAR / DOWN [rows, n]; GATE_UP [slots, n]
     int out_dtype;
     int act;
     // LINEAR
+    int block;               // tokens from one block to the next, at most TOK: a multiple of 16
     int w_mn;                // the weight is stored [k, n]: two boxes of 64 features x 64 contraction rows, read in place
     const void *bias, *residual;
     int bias_dtype;
@@ -72,13 +77,13 @@ struct FewRowsArgs {
     int *status;
 };
 
-template <int TOK> struct FrCfg {
-    static constexpr int kEpiWarps = TOK <= 32 ? 4 : 8;   // per quarter of the accumulator's rows: one, or two that share the tokens
+template <int TOK, bool PAIR> struct FrCfg {
+    static constexpr int kEpiWarps = TOK <= 32 ? 4 : TOK <= 128 ? 8 : 16;   // per quarter of the accumulator's rows: one, or two that share the tokens
     static constexpr int kThreads = 64 + 32 * kEpiWarps;
-    static constexpr int kBBytes = TOK * 128;
+    static constexpr int kBBytes = (PAIR ? TOK / 2 : TOK) * 128;
     static constexpr int kStageBytes = kFrABytes + kBBytes;
-    static constexpr int kCtas = TOK <= 128 ? 2 : 1;   // per SM
-    static constexpr int kStages = TOK <= 16 ? 6 : TOK <= 32 ? 5 : TOK <= 64 ? 4 : TOK <= 128 ? 3 : TOK <= 192 ? 5 : 4;
+    static constexpr int kCtas = TOK > 128 ? 1 : 2;           // per SM
+    static constexpr int kStages = TOK <= 16 ? 6 : TOK <= 32 ? 5 : TOK <= 64 ? 4 : TOK <= 128 ? 3 : PAIR ? 6 : 5;
     static constexpr int kRing = kStages * kStageBytes;
     static constexpr int kIdSlots = TOK * kFrMaxTopK < kFrMaxSlots ? TOK * kFrMaxTopK : kFrMaxSlots;
     static constexpr int kSmem = kRing + 1024 /* alignment */ + 2 * kIdSlots;
@@ -87,12 +92,46 @@ template <int TOK> struct FrCfg {
     static_assert(kCtas * (kSmem + 3584 /* static and reserved */) <= 228 * 1024, "CTAs per SM");
 };
 
-template <int TOK, int KIND>
-__global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
+// Four elements of each of ROWS rows, under predicates
+template <int ROWS> __device__ __forceinline__ void store4_rows(void *p, int dtype, int64_t at, int64_t pitch, const bool (&st)[ROWS], const float (&v)[ROWS][4]) {
+    if (dtype == PT_F32) {
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u)
+            if (st[u]) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + at + u * pitch) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u) {
+            const uint2 h = dtype == PT_BF16 ? make_uint2(pack2<__nv_bfloat16>(v[u][0], v[u][1]), pack2<__nv_bfloat16>(v[u][2], v[u][3]))
+                                             : make_uint2(pack2<__half>(v[u][0], v[u][1]), pack2<__half>(v[u][2], v[u][3]));
+            if (st[u]) *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p) + at + u * pitch) = h;
+        }
+    }
+}
+template <int ROWS> __device__ __forceinline__ void load4_rows(const void *p, int dtype, int64_t at, int64_t pitch, const bool (&st)[ROWS], uint4 (&raw)[ROWS]) {
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) raw[u] = make_uint4(0u, 0u, 0u, 0u);
+    if (dtype == PT_F32) {
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u)
+            if (st[u]) raw[u] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(p) + at + u * pitch);
+    } else {
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u)
+            if (st[u]) {
+                const uint2 h = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + at + u * pitch);
+                raw[u].x = h.x;
+                raw[u].y = h.y;
+            }
+    }
+}
+
+template <int TOK, int KIND, bool PAIR>
+__global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::kCtas)
     few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, FewRowsArgs a) {
-    using Cfg = FrCfg<TOK>;
+    using Cfg = FrCfg<TOK, PAIR>;
     constexpr int kStages = Cfg::kStages;
-    constexpr bool kMoe = KIND != FR_LINEAR;
+    constexpr bool kMoe = KIND != FR_LINEAR, kPair = PAIR;
+    static_assert(!kMoe || (TOK <= 128 && !PAIR), "wide blocks are for dense products");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     int16_t *s_ids = reinterpret_cast<int16_t *>(ring + Cfg::kRing);   // [tokens * top_k], -1: no expert of this call
@@ -104,9 +143,12 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
     __shared__ int s_row[KIND == FR_GATE_UP ? TOK : 1], s_slot[KIND == FR_GATE_UP ? TOK : 1];
     __shared__ float s_prob[KIND == FR_GATE_UP ? TOK : 1];
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = a.split > 1 ? (int) cluster_ctarank() : 0;
-    const int tile = (int) blockIdx.x / a.split;
+    const int warp = __shfl_sync(0xffffffffu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // the shuffle tells the compiler: uniform
+    // `rank`: which share of the contraction.  Wide blocks: CTAs 2 rank and 2 rank + 1 of the cluster are a pair.
+    const bool cluster = kPair || a.split > 1;
+    const int cta_rank = cluster ? (int) cluster_ctarank() : 0, half = kPair ? cta_rank & 1 : 0;
+    const int rank = kPair ? cta_rank >> 1 : cta_rank;
+    const int tile = kPair ? (int) blockIdx.x / (2 * a.split) * 2 + half : (int) blockIdx.x / a.split;
     const int T = a.rows;
 
     if (threadIdx.x == 0) {
@@ -115,16 +157,16 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
             mbar_init(&full_bar[s], kMoe ? 1 + 32 * Cfg::kEpiWarps : 1);   // the weights' bytes, and the copying threads
             mbar_init(&empty_bar[s], 1);
         }
-        mbar_init(&done_bar, 2);   // the MMA thread's own arrival (publishes s_touched) and its commit
+        mbar_init(&done_bar, 2);   // the MMA thread's commit, and an arrival of this CTA's warp 1 (publishes s_tmem and s_touched)
         fence_barrier_init();
         prefetch_tmap(&tmap_w);
         prefetch_tmap(&tmap_x);
     }
-    if (warp == 1) {
+    if (kMoe && warp == 1) {
         tmem_alloc(&s_tmem, Cfg::kTmemCols);
         tmem_relinquish();
     }
-    if (KIND == FR_LINEAR && threadIdx.x == 64 && blockIdx.y == 0) {
+    if (KIND == FR_LINEAR && threadIdx.x == 64 && blockIdx.y == 0 && tile * kFrFeat < a.n) {
         // The first weight blocks on their way into L2 while the kernel before this one finishes.  A prefetch is not a read: were the
         // weight being written, L2 would hold the new values all the same.
         const int chunks = (a.k + 63) / 64, l0 = chunks * rank / a.split, l1 = chunks * (rank + 1) / a.split;
@@ -143,7 +185,7 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
     }
 
     // ---- routing: which experts are chosen, and by whom
-    int cnt = KIND == FR_LINEAR ? min(TOK, T - (int) blockIdx.y * TOK) : 0;   // rows of this CTA
+    int cnt = KIND == FR_LINEAR ? min(a.block, T - (int) blockIdx.y * a.block) : 0;   // rows of this CTA
     int expert = 0, n_active = 0;
     if constexpr (kMoe) {
         if (threadIdx.x < 32) s_bits[threadIdx.x] = 0;
@@ -204,7 +246,9 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
         }
     }
     tc_fence_before_sync();
-    __syncthreads();
+    __syncwarp();
+    if constexpr (kPair) cluster_sync_all();   // the other CTA's barriers stand before anything arrives there
+    else __syncthreads();
     tc_fence_after_sync();
     if constexpr (KIND == FR_GATE_UP) cnt = s_count;
     if constexpr (KIND == FR_DOWN) cnt = T;
@@ -213,7 +257,16 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
     const int chunks = (a.k + 63) / 64;   // per expert
     const int64_t total = KIND == FR_DOWN ? (int64_t) n_active * chunks : chunks;
     const int l0 = (int) (total * rank / a.split), l1 = (int) (total * (rank + 1) / a.split);
-    const uint32_t tmem = s_tmem;
+    if (!kMoe && warp == 1) {   // only now: the producer does not wait for it (a pair's allocation takes about half a microsecond)
+        if constexpr (kPair) {
+            tmem_alloc_pair(&s_tmem, Cfg::kTmemCols);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(&s_tmem, Cfg::kTmemCols);
+            tmem_relinquish();
+        }
+        __syncwarp();
+    }
     volatile int *abort_flag = &s_abort;
     bool ok = true;
 
@@ -223,11 +276,26 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
         if constexpr (KIND != FR_DOWN) {
             if (elect_one()) {
                 const int expert_row = expert * 2 * a.n + tile * 64;
+                const int x_row = (int) blockIdx.y * a.block + half * 8 * ((cnt + 15) / 16);
+                const uint32_t x_bytes = kMoe ? 0 : (kPair ? a.block / 2 : a.block) * 128;
                 uint32_t stage = 0, phase = 0;
                 for (int l = l0; l < l1; ++l) {
                     if (!(ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag))) break;
                     uint8_t *A = ring + stage * Cfg::kStageBytes;
-                    mbar_arrive_expect_tx(&full_bar[stage], kFrABytes + (kMoe ? 0 : Cfg::kBBytes));
+                    if constexpr (kPair) {   // the bytes of both CTAs on the barrier of the first
+                        const uint32_t full = map_to_rank(&full_bar[stage], cta_rank & ~1);
+                        if (half == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * (kFrABytes + x_bytes));
+                        if (a.w_mn) {
+                            tma_load_2d_pair_hint(A, &tmap_w, full, tile * kFrFeat * 2, l * 64, stream_pol);
+                            tma_load_2d_pair_hint(A + kFrABytes / 2, &tmap_w, full, tile * kFrFeat * 2 + 128, l * 64, stream_pol);
+                        } else {
+                            tma_load_2d_pair_hint(A, &tmap_w, full, l * 128, tile * kFrFeat, stream_pol);
+                        }
+                        tma_load_2d_pair_hint(A + kFrABytes, &tmap_x, full, l * 128, x_row, keep_pol);
+                        if (++stage == kStages) { stage = 0; phase ^= 1; }
+                        continue;
+                    }
+                    mbar_arrive_expect_tx(&full_bar[stage], kFrABytes + x_bytes);
                     if (KIND == FR_GATE_UP) {
                         tma_load_2d_hint(A, &tmap_w, &full_bar[stage], l * 128, expert_row, stream_pol);
                         tma_load_2d_hint(A + kFrABytes / 2, &tmap_w, &full_bar[stage], l * 128, expert_row + a.n, stream_pol);
@@ -238,7 +306,7 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
                         } else {
                             tma_load_2d_hint(A, &tmap_w, &full_bar[stage], l * 128, tile * kFrFeat, stream_pol);
                         }
-                        tma_load_2d_hint(A + kFrABytes, &tmap_x, &full_bar[stage], l * 128, (int) blockIdx.y * TOK, keep_pol);
+                        tma_load_2d_hint(A + kFrABytes, &tmap_x, &full_bar[stage], l * 128, x_row, keep_pol);
                     }
                     if (++stage == kStages) { stage = 0; phase ^= 1; }
                 }
@@ -272,9 +340,13 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
         }
     } else if (warp == 1) {
         // ================================================================ MMA issuer
-        if (elect_one()) {
+        const uint32_t tmem = s_tmem;
+        if (half == 1) {
+            if (elect_one()) mbar_arrive(&done_bar);
+        } else if (elect_one()) {
             const bool w_mn = KIND == FR_LINEAR && a.w_mn;
-            const uint32_t idesc0 = idesc_f8(a.fmt, a.fmt, kFrFeat, 0) | ((uint32_t) w_mn << 15);
+            const uint16_t both = (uint16_t) (3u << cta_rank);   // the CTAs of the pair
+            const uint32_t idesc0 = idesc_f8(a.fmt, a.fmt, kPair ? 2 * kFrFeat : kFrFeat, 0) | ((uint32_t) w_mn << 15);
             const uint64_t w_step = w_mn ? (16 * 128) >> 4 : 32 >> 4;   // 16 contraction rows, or 32 bytes along a row
             uint32_t touched = 0;   // 16-token blocks that hold sums
             const uint32_t all = (1u << ((cnt + 15) / 16)) - 1;
@@ -296,18 +368,22 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
                     const uint32_t idesc = idesc0 | ((uint32_t) (2 * len) << 17);   // N = 16 len, in units of 8
                     const uint32_t acc0 = touched >> b0 & 1;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mma_f16(tmem + 16 * b0, a_desc + k * w_step, b_desc + 2 * k, idesc, acc0 | (uint32_t) (k > 0));
+                    for (int k = 0; k < 4; ++k) {
+                        if constexpr (kPair) mma_f16_pair(tmem, a_desc + k * w_step, b_desc + 2 * k, idesc, acc0 | (uint32_t) (k > 0));
+                        else mma_f16(tmem + 16 * b0, a_desc + k * w_step, b_desc + 2 * k, idesc, acc0 | (uint32_t) (k > 0));
+                    }
                     m &= ~(((1u << len) - 1) << b0);
                 }
                 touched |= used;
-                tc_commit(&empty_bar[stage]);
+                if constexpr (kPair) tc_commit_pair(&empty_bar[stage], both);
+                else tc_commit(&empty_bar[stage]);
                 if (++stage == kStages) { stage = 0; phase ^= 1; }
             }
             if (ok) {
                 s_touched = touched;
                 mbar_arrive(&done_bar);
-                tc_commit(&done_bar);
+                if constexpr (kPair) tc_commit_pair(&done_bar, both);
+                else tc_commit(&done_bar);
             }
         }
     }
@@ -373,12 +449,12 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
         const int q = warp & 3;   // tensor memory lanes this warp may read
         ok = mbar_wait_warp(&done_bar, 0, abort_flag);
         tc_fence_after_sync();
-        const uint32_t touched = ok ? s_touched : 0;
+        const uint32_t touched = !ok ? 0 : kPair ? (l1 > l0 ? (1u << blocks) - 1 : 0) : s_touched;
         // Two blocks of 16 tokens at a time, both loads in flight.  They are made whether or not the columns hold sums (a pair never
         // reaches past the allocation): between a load and its wait nothing may touch the registers, a branch's merge neither.
         for (int b = 2 * ((warp - 2) >> 2); b < blocks; b += Cfg::kEpiWarps / 2) {
             uint32_t r[2][16];
-            const uint32_t at = tmem + ((uint32_t) (q * 32) << 16) + 16 * b;
+            const uint32_t at = s_tmem + ((uint32_t) (q * 32) << 16) + 16 * b;
             tmem_ld16(at, r[0]);
             tmem_ld16(at + 16, r[1]);
             tmem_ld_wait();
@@ -397,11 +473,12 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
     }
     tc_fence_before_sync();
     __syncwarp();
-    if (a.split > 1) cluster_sync_all();
+    if (cluster) cluster_sync_all();
     else __syncthreads();
     if (warp == 1) {
         tc_fence_after_sync();
-        tmem_dealloc(tmem, Cfg::kTmemCols);
+        if constexpr (kPair) tmem_dealloc_pair(s_tmem, Cfg::kTmemCols);
+        else tmem_dealloc(s_tmem, Cfg::kTmemCols);
     }
     if constexpr (KIND == FR_DOWN) grid_dep_wait();
 
@@ -420,133 +497,142 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
             if (f < a.n) bias[i] = load_as_f32(a.bias, a.bias_dtype, f);
         }
     }
-    // A warp takes a token or two at once, the loads of several CTAs' blocks on their way before the first addition: one remote round trip
-    // for all of them.  The sums run in the order of the ranks.
-    constexpr int kAtOnce = TOK <= 16 ? 1 : 2;
+    // A warp takes up to kAtOnce tokens at once.  There are few warps, so this part is bound by the latency of its instructions, not
+    // their number: every step runs over all of the tokens before the next, under predicates instead of branches (128 x 4096 x 128: 7.6 us
+    // with two tokens at once and a branch around each step, now 5.6).  The sums begin with this CTA's own block and go on with the other ranks'
+    // after it, the loads of kOthers of them on their way before the first addition: a remote round trip takes about 0.6 us, and the
+    // instantiations below make one do.
     const int step = a.split * (Cfg::kThreads / 32);   // tokens between two of this warp's
+    auto write_out = [&](auto at_once, auto others) {
+    constexpr int kAtOnce = decltype(at_once)::value, kOthers = decltype(others)::value;
     for (int t0 = rank + a.split * warp; t0 < cnt; t0 += kAtOnce * step) {
         float v[kAtOnce][4];
-        auto load = [&](uint32_t src, bool remote, float (&w)[4]) {
-            if (vec) {
-                ld_cluster_f32x2(src, remote, w[0], w[1]);
-                ld_cluster_f32x2(src + (KIND == FR_GATE_UP ? 256 : 8), remote, w[2], w[3]);
+        bool in[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) in[u] = t0 + u * step < cnt;
+        auto load = [&](int u, uint32_t src, bool remote, float (&w)[4]) {
+            if (KIND == FR_GATE_UP) {
+                ld_cluster_f32x2(src, remote, in[u], w[0], w[1]);
+                ld_cluster_f32x2(src + 256, remote, in[u], w[2], w[3]);
+            } else if (vec) {
+                ld_cluster_f32x4(src, remote, in[u], w);
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = ld_cluster_f32(src + 128 * i, remote);
+                for (int i = 0; i < 4; ++i) ld_cluster_f32(src + 128 * i, remote, in[u], w[i]);
             }
         };
-        auto inside = [&](int u) { return u == 0 || t0 + u * step < cnt; };
         auto row_at = [&](int u) { return part_addr + (uint32_t) (t0 + u * step) * (kFrFeat * 4) + lane_at; };
-        if (a.split == 1) {
+        float w[kOthers > 0 ? kOthers : 1][kAtOnce][4];
 #pragma unroll
-            for (int u = 0; u < kAtOnce; ++u)
-                if (inside(u)) load(row_at(u), false, v[u]);
-        } else {
-            constexpr int kRanks = kAtOnce == 1 ? kFrMaxSplit : kFrMaxSplit / 2;
+        for (int s = 0; s < kOthers; ++s) {
+            const int other = (rank + 1 + s) & (a.split - 1);
 #pragma unroll
-            for (int u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[u][i] = 0.f;
-            for (int s0 = 0; s0 < a.split; s0 += kRanks) {
-                float w[kRanks][kAtOnce][4];
-#pragma unroll
-                for (int s = 0; s < kRanks; ++s)
-                    if (s0 + s < a.split) {
-#pragma unroll
-                        for (int u = 0; u < kAtOnce; ++u)
-                            if (inside(u)) load(map_addr_to_rank(row_at(u), s0 + s), true, w[s][u]);
-                    }
-#pragma unroll
-                for (int s = 0; s < kRanks; ++s)
-                    if (s0 + s < a.split) {
-#pragma unroll
-                        for (int u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) v[u][i] += w[s][u][i];
-                    }
-            }
+            for (int u = 0; u < kAtOnce; ++u) load(u, map_addr_to_rank(row_at(u), kPair ? 2 * other + half : other), true, w[s][u]);
         }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) load(u, row_at(u), false, v[u]);
+#pragma unroll
+        for (int s = 0; s < kOthers; ++s)
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[u][i] += w[s][u][i];
         if constexpr (KIND == FR_GATE_UP) {
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) {
                 const int t = t0 + u * step;
-                if (!inside(u) || f0 >= a.n) continue;
+                if (!in[u] || f0 >= a.n) continue;
                 const float p = s_prob[t];
                 const float h0 = act_any(a.act, v[u][0]) * v[u][2] * p, h1 = act_any(a.act, v[u][1]) * v[u][3] * p;
                 *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.out) + (int64_t) s_slot[t] * a.n + f0) =
                     a.fmt ? pack2<__nv_bfloat16>(h0, h1) : pack2<__half>(h0, h1);
             }
         } else if constexpr (KIND == FR_DOWN) {
+            bool st[kAtOnce];
 #pragma unroll
-            for (int u = 0; u < kAtOnce; ++u) {
-                const int t = t0 + u * step;
-                if (inside(u) && f0 < a.n) store4_from_f32(a.out, a.out_dtype, (int64_t) t * a.n + f0, v[u]);
-            }
+            for (int u = 0; u < kAtOnce; ++u) st[u] = in[u] && f0 < a.n;
+            store4_rows<kAtOnce>(a.out, a.out_dtype, (int64_t) t0 * a.n + f0, (int64_t) step * a.n, st, v);
         } else {
-            const int64_t o0 = ((int64_t) blockIdx.y * TOK + t0) * a.n + f0, o_step = (int64_t) step * a.n;
+            const int64_t o0 = ((int64_t) blockIdx.y * a.block + t0) * a.n + f0, o_step = (int64_t) step * a.n;
             const int zt = a.fmt ? PT_BF16 : PT_F16;
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[u][i] += bias[i];
             if (vec) {
-                if (f0 >= a.n) continue;
+                bool st[kAtOnce];
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) st[u] = in[u] && f0 < a.n;
                 uint4 res[kAtOnce];
+                if (a.residual != nullptr) load4_rows<kAtOnce>(a.residual, a.out_dtype, o0, o_step, st, res);
+                if (a.z != nullptr) store4_rows<kAtOnce>(a.z, zt, o0, o_step, st, v);
+                act_any_all<kAtOnce>(a.act, v);
                 if (a.residual != nullptr) {
 #pragma unroll
-                    for (int u = 0; u < kAtOnce; ++u)
-                        if (inside(u)) res[u] = load4_raw(a.residual, a.out_dtype, o0 + u * o_step);
-                }
-                if (a.z != nullptr) {
-#pragma unroll
-                    for (int u = 0; u < kAtOnce; ++u)
-                        if (inside(u)) store4_from_f32(a.z, zt, o0 + u * o_step, v[u]);
-                }
-                act_any_all<kAtOnce>(a.act, v);
-#pragma unroll
-                for (int u = 0; u < kAtOnce; ++u) {
-                    if (!inside(u)) continue;
-                    if (a.residual != nullptr) {
+                    for (int u = 0; u < kAtOnce; ++u) {
                         float x[4];
                         raw4_as_f32(res[u], a.out_dtype, x);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v[u][i] += x[i];
                     }
-                    store4_from_f32(a.out, a.out_dtype, o0 + u * o_step, v[u]);
                 }
+                store4_rows<kAtOnce>(a.out, a.out_dtype, o0, o_step, st, v);
             } else {
+                bool st[kAtOnce][4];
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) st[u][i] = in[u] && f0 + 32 * i < a.n;
                 uint32_t res[kAtOnce][4];   // raw, all on their way before the first is used
                 if (a.residual != nullptr) {
                     auto fetch = [&](auto *p) {
 #pragma unroll
                         for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (inside(u) && f0 + 32 * i < a.n) res[u][i] = p[o0 + u * o_step + 32 * i];
+                            for (int i = 0; i < 4; ++i) {
+                                res[u][i] = 0;
+                                if (st[u][i]) res[u][i] = p[o0 + u * o_step + 32 * i];
+                            }
                     };
                     if (a.out_dtype == PT_F32) fetch(reinterpret_cast<const uint32_t *>(a.residual));
                     else fetch(reinterpret_cast<const uint16_t *>(a.residual));
                 }
-                if (a.z != nullptr) {
+                auto put = [&](void *out, int dtype) {
+                    if (dtype == PT_F32) {
+#pragma unroll
+                        for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (st[u][i]) reinterpret_cast<float *>(out)[o0 + u * o_step + 32 * i] = v[u][i];
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t h = dtype == PT_BF16 ? pack2<__nv_bfloat16>(v[u][i], 0.f) : pack2<__half>(v[u][i], 0.f);
+                                if (st[u][i]) reinterpret_cast<uint16_t *>(out)[o0 + u * o_step + 32 * i] = (uint16_t) h;
+                            }
+                    }
+                };
+                if (a.z != nullptr) put(a.z, zt);
+                act_any_all<kAtOnce>(a.act, v);
+                if (a.residual != nullptr) {
 #pragma unroll
                     for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (inside(u) && f0 + 32 * i < a.n) store_from_f32(a.z, zt, o0 + u * o_step + 32 * i, v[u][i]);
-                }
-                act_any_all<kAtOnce>(a.act, v);
-#pragma unroll
-                for (int u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (!inside(u) || f0 + 32 * i >= a.n) continue;
-                        if (a.residual != nullptr)
                             v[u][i] += a.out_dtype == PT_F32 ? __uint_as_float(res[u][i]) : a.out_dtype == PT_BF16 ? lo_f32<__nv_bfloat16>(res[u][i]) : lo_f32<__half>(res[u][i]);
-                        store_from_f32(a.out, a.out_dtype, o0 + u * o_step + 32 * i, v[u][i]);
-                    }
+                }
+                put(a.out, a.out_dtype);
             }
         }
     }
+    };
+    using std::integral_constant;
+    if (a.split == 1) write_out(integral_constant<int, TOK <= 16 ? 1 : TOK <= 32 ? 2 : 4>(), integral_constant<int, 0>());
+    else if (a.split == 2) write_out(integral_constant<int, TOK <= 16 ? 2 : 4>(), integral_constant<int, 1>());
+    else if (a.split == 4) write_out(integral_constant<int, TOK <= 16 ? 1 : TOK <= 64 ? 2 : 3>(), integral_constant<int, 3>());
+    else if constexpr (!kPair) write_out(integral_constant<int, 1>(), integral_constant<int, kFrMaxSplit - 1>());
     if (a.split > 1) {
         __syncwarp();
         cluster_sync_all();   // no CTA leaves while another still reads its block
@@ -554,19 +640,21 @@ __global__ void __launch_bounds__(FrCfg<TOK>::kThreads, FrCfg<TOK>::kCtas)
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-template <int TOK, int KIND>
+template <int TOK, int KIND, bool PAIR = false>
 static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRowsArgs &a, int64_t tiles, int64_t grid_y, cudaStream_t st) {
-    using Cfg = FrCfg<TOK>;
-    auto kern = few_rows_kernel<TOK, KIND>;
+    using Cfg = FrCfg<TOK, PAIR>;
+    auto kern = few_rows_kernel<TOK, KIND, PAIR>;
     static bool attr_set[64] = {};   // per instantiation and device
     const int dev = current_device_slot();
     if (!attr_set[dev]) {
         PT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
         attr_set[dev] = true;
     }
-    PT_REQUIRE(tiles * a.split < (1ll << 31) && grid_y < 65536, "few-row product: grid too large");
+    const int cluster_ctas = PAIR ? 2 * a.split : a.split;
+    if (PAIR) tiles = ceil_div(tiles, 2);
+    PT_REQUIRE(tiles * cluster_ctas < (1ll << 31) && grid_y < 65536, "few-row product: grid too large");
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned) (tiles * a.split), (unsigned) grid_y);
+    cfg.gridDim = dim3((unsigned) (tiles * cluster_ctas), (unsigned) grid_y);
     cfg.blockDim = dim3(Cfg::kThreads);
     cfg.dynamicSmemBytes = Cfg::kSmem;
     cfg.stream = st;
@@ -574,40 +662,63 @@ static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRows
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned) a.split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-    const bool overlap = getenv("PT_NO_PDL") == nullptr, cluster = a.split > 1;   // as in launch_overlapped
+    attr[1].val.clusterDim.x = (unsigned) cluster_ctas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    const bool overlap = getenv("PT_NO_PDL") == nullptr, cluster = cluster_ctas > 1;   // as in launch_overlapped
     cfg.attrs = overlap ? attr : attr + 1;
     cfg.numAttrs = (overlap ? 1 : 0) + (cluster ? 1 : 0);
     PT_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, tw, tx, a));
     return PT_OK;
 }
 
-// Estimated time of a launch in us: `tiles` weight blocks wide, `blocks` times over them (blocks of `tok` tokens), `chunks` 64-wide steps of
-// the contraction, s CTAs per cluster.  4.5 us of launch, first bytes and write-out; the exchange of partial sums, longer with every CTA of
-// the cluster; and the longest of: a CTA's own steps, the weights out of memory (one 100 KiB ring per SM does not quite saturate it),
-// all stages out of L2 (13 TB/s).  CTAs beyond those resident at once start late, about 6 us per wave.  Measured against estimated (us):
-// 1 x 4096 x 14336 (rows, features, K), s = 1, 4, 8: 65.5 / 67, 24.6 / 25.3, 21.6 / 23.6; 64 x 4096 x 4096, s = 1, 2, 4, 8: 25.7 / 26.6, 17.0 /
-// 17.1, 13.8 / 14.3, 16.3 / 17.7; 333 x 4096 x 4096, 128 / 192 / 256 tokens per block and s = 2: 25.2 / 24.1, 21.3 / 20.3, 25.4 / 23.9.
-static double fr_cost(int tok, int64_t tiles, int64_t blocks, int64_t chunks, int s) {
-    const bool wide = tok > 128;   // one CTA per SM
-    const double ctas = (double) (tiles * blocks * s), resident = (wide ? 1.0 : 2.0) * sm_count();
-    const double steps = (double) ceil_div(chunks, s) * (wide ? 0.14 + 0.0012 * tok : 0.25 + 0.00125 * tok);
-    const double memory = (double) tiles * (double) chunks * kFrABytes / (!wide && ctas <= sm_count() ? 5.8e6 : 6.5e6);
-    const double l2 = (double) tiles * (double) (blocks * chunks) * (kFrABytes + tok * 128) / 13e6;
-    const double exchange = (tok <= 32 ? 0.008 : wide ? 0.0075 : 0.016) * tok * s;
-    return 4.5 + exchange + std::max(steps, std::max(memory, l2)) + 6.0 * std::max(0.0, ctas / resident - 1.0);
+// SMs that clusters of `ctas` CTAs can use at once with one CTA per SM (GPCs do not divide evenly; measured on 148 SMs: 33 clusters of four and 12 of
+// eight run together, 34 and 16 in two waves).  With two CTAs per SM no such loss was seen.  The driver's occupancy query is not asked: it
+// answers one CTA per SM for these kernels, and launches after it do run one per SM (333 x 4096 x 4096 in blocks of 128: 29.4 us, else 23.0).
+static double fr_resident(bool wide, int ctas) {
+    const double sms = sm_count();
+    return !wide ? 2.0 * sms : ctas <= 2 ? sms : ctas == 4 ? sms * 33 / 37 : sms * 2 / 3;
 }
-// Tokens per block and CTAs per cluster with the smallest estimate.
-struct FrPlan { int tok, split; double us; };
+
+// Estimated time of a launch in us: `tiles` weight blocks wide, `blocks` blocks of `block` tokens on the kernel for up to `tok`, `chunks` 64-wide
+// steps of the contraction, s CTAs or pairs per cluster.  A fixed part, and the longest of: a CTA's own steps (an SM takes in about 108 GB/s),
+// the bytes from and to memory (one 100 KiB ring per SM does not quite saturate it), all stages out of L2 (15 TB/s).  CTAs beyond those
+// resident at once are further waves.  Measured (us, SiLU epilogue; rows x features x K, kernel : block / s): 64 x 4096 x 4096 64 / 1, 2, 4, 8 24.8, 16.1,
+// 12.8, 13.0; 129 x 4096 x 4096 128 : 80 / 4 15.6, 192 : 144 / 2, 4 17.1, 13.6, 256 : 144 / 2, 4 16.7, 26.5 (two waves); 333 x 4096 x 4096 128 : 112 / 2
+// 23.3, 192 : 176 / 2 19.0, 256 : 176 / 2 19.0; 512 x 4096 x 4096 128 : 128 / 2 24.6, 192 : 128 / 1 24.8, 256 : 256 / 2 21.1; 512 x 4096 x 14336 192 : 176 / 1
+// 78, 256 : 256 / 2 47.7.  What the estimate picks was within 5 % of the best in 30 of the 36 sizes measured, within 15 % in all.
+static double fr_cost(int tok, int block, int64_t tiles, int64_t blocks, int64_t chunks, int s) {
+    const bool wide = tok > 128, pair = tok == kFrPairTok;
+    if (pair) tiles = (tiles + 1) / 2 * 2;
+    const double ctas = (double) (tiles * blocks * s), share = ctas / fr_resident(wide, pair ? 2 * s : s);
+    const double waves = std::max(1.0, wide ? std::ceil(share) : share);   // two CTAs per SM: a later one starts when either ends
+    const double x_bytes = (pair ? 64.0 : 128.0) * block;   // of tokens per step
+    double step = pair ? 0.18 + 0.0007 * block : wide ? 0.2 + 0.0005 * block : 0.25 + 0.00125 * block;
+    if (!wide && ctas > sm_count()) step = std::max(step, 2.0 * (kFrABytes + x_bytes) / 108e3);   // two CTAs share what an SM takes in
+    const double rows = (double) (blocks * block), k_bytes = 128.0 * (double) chunks;
+    const double memory = ((double) tiles * kFrFeat * (k_bytes + 2.0 * rows) + rows * k_bytes) / (!wide && ctas <= sm_count() ? 5.8e6 : 6.5e6);
+    const double l2 = (double) (tiles * blocks * chunks) * (kFrABytes + x_bytes) / 15e6;
+    double fixed;   // launch, first bytes, exchange of partial sums, write-out
+    if (pair) fixed = s == 1 ? 5.7 + 0.0025 * block : 7.2 + 0.0075 * block;
+    else if (wide) fixed = s == 1 ? 6.8 : 6.4 + 0.012 * block;
+    else if (tok > 32) fixed = (s == 1 ? 4.2 : 5.1 + (0.0065 + 0.006 * s) * block) + (tok > 64 && ctas > sm_count() ? 3.0 : 0.0);
+    else fixed = 4.5 + 0.008 * block * s;
+    return fixed + std::max(waves * step * (double) ceil_div(chunks, s), std::max(memory, l2)) + (waves - 1.0) * (tok > 64 ? fixed + 5.0 : 6.0);
+}
+// Kernel, tokens per block and CTAs (pairs) per cluster with the smallest estimate.
+struct FrPlan { int tok, block, split; double us; };
 static FrPlan fr_plan(int64_t rows, int64_t n, int64_t k) {
     const int64_t tiles = ceil_div(n, kFrFeat), chunks = ceil_div(k, 64);
-    FrPlan best{0, 1, 0.0};
-    for (int tok : {16, 32, 64, 128, 192, 256}) {
+    FrPlan best{0, 0, 1, 0.0};
+    for (int tok : {16, 32, 64, 128, 192, kFrPairTok}) {
         if ((tok < 128 && tok < rows) || (tok > 16 && tok <= 128 && tok / 2 >= rows) || (tok > 128 && rows <= 64)) continue;   // no room, or more than half of it empty
-        const int64_t blocks = ceil_div(rows, tok);
-        for (int s = 1; s <= kFrMaxSplit && (s == 1 || (tiles * blocks * s <= (tok > 128 ? 1 : 2) * (int64_t) sm_count() && chunks >= 2 * s)); s *= 2) {
-            const double us = fr_cost(tok, tiles, blocks, chunks, s);
-            if (best.tok == 0 || us < best.us) best = {tok, s, us};
+        for (int more = 0; more <= (tok >= 128 && rows > 64 ? 1 : 0); ++more) {   // as few blocks as possible, or one more
+            const int block = (int) ceil_div(ceil_div(rows, ceil_div(rows, tok) + more), 16) * 16;
+            const int64_t blocks = ceil_div(rows, block);
+            if (blocks > 65535) continue;   // the grid's second extent
+            const int max_split = tok == kFrPairTok ? kFrMaxSplit / 2 : kFrMaxSplit;
+            for (int s = 1; s <= max_split && (s == 1 || (tiles * blocks * s <= (tok > 128 ? 1 : 2) * (int64_t) sm_count() && chunks >= 2 * s)); s *= 2) {
+                const double us = fr_cost(tok, block, tiles, blocks, chunks, s);
+                if (best.tok == 0 || us < best.us) best = {tok, block, s, us};
+            }
         }
     }
     return best;
@@ -617,7 +728,7 @@ static FrPlan fr_plan(int64_t rows, int64_t n, int64_t k) {
 static int fr_split_experts(int tok, int64_t tiles, int64_t chunks) {
     int best = 1;
     for (int s = 2; s <= kFrMaxSplit && tiles * s <= 2 * (int64_t) sm_count() && chunks >= 2 * s; s *= 2)
-        if (fr_cost(tok, tiles, 1, chunks, s) < fr_cost(tok, tiles, 1, chunks, best)) best = s;
+        if (fr_cost(tok, tok, tiles, 1, chunks, s) < fr_cost(tok, tok, tiles, 1, chunks, best)) best = s;
     return best;
 }
 
@@ -631,7 +742,7 @@ static int fr_dispatch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRo
     }
     if constexpr (KIND == FR_LINEAR) {
         if (tok == 192) return fr_launch<192, KIND>(tw, tx, a, tiles, grid_y, st);
-        if (tok == 256) return fr_launch<256, KIND>(tw, tx, a, tiles, grid_y, st);
+        if (tok == 256) return fr_launch<256, KIND, true>(tw, tx, a, tiles, grid_y, st);
     }
     return set_error(PT_ERR_INVALID, "few-row product: no kernel for %d tokens per block", tok);
 }
@@ -646,13 +757,14 @@ int few_rows_linear(const void *a, const void *b, int b_mn, int ab_dtype, const 
     CUtensorMap tw, tx;
     int rc;
     if ((rc = b_mn ? make_tmap_bytes(&tw, b, K, 2 * N, 2 * N, 64) : make_tmap_bytes(&tw, b, N, 2 * K, 2 * K, kFrFeat)) != PT_OK) return rc;
-    if ((rc = make_tmap_bytes(&tx, a, M, 2 * K, 2 * K, tok)) != PT_OK) return rc;
+    if ((rc = make_tmap_bytes(&tx, a, M, 2 * K, 2 * K, tok == kFrPairTok ? plan.block / 2 : plan.block)) != PT_OK) return rc;
     FewRowsArgs r{};
+    r.block = plan.block;
     r.w_mn = b_mn; r.rows = (int) M; r.n = (int) N; r.k = (int) K; r.fmt = ab_dtype == PT_BF16 ? 1 : 0;
     r.out = c; r.out_dtype = c_dtype; r.act = act; r.bias = bias; r.bias_dtype = bias_dtype; r.residual = residual; r.z = z; r.status = status;
     const int esize = c_dtype == PT_F32 ? 4 : 2;
     r.vec_ok = N % 4 == 0 && aligned(c, 4 * esize) && aligned(residual, 4 * esize) && aligned(z, 8) && aligned(bias, bias_dtype == PT_F32 ? 16 : 8);
-    const int64_t tiles = ceil_div(N, kFrFeat), grid_y = ceil_div(M, tok);
+    const int64_t tiles = ceil_div(N, kFrFeat), grid_y = ceil_div(M, plan.block);
     r.split = plan.split;
     return fr_dispatch<FR_LINEAR>(tw, tx, r, tok, tiles, grid_y, st);
 }

@@ -335,16 +335,33 @@ __device__ __forceinline__ uint32_t map_addr_to_rank(uint32_t addr, uint32_t ran
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-// two floats from shared memory: of another CTA of the cluster (address from map_addr_to_rank), or this one's own
-__device__ __forceinline__ void ld_cluster_f32x2(uint32_t addr, bool remote, float &x, float &y) {
-    if (remote) asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x), "=f"(y) : "r"(addr) : "memory");
-    else asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(x), "=f"(y) : "r"(addr) : "memory");
+// Floats from shared memory, of another CTA of the cluster (address from map_addr_to_rank) or this one's own; zeros where `take` is not set
+// (a predicate, so that a run of such loads is issued without a branch).
+__device__ __forceinline__ void ld_cluster_f32x4(uint32_t addr, bool remote, bool take, float (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = 0.f;
+    if (remote)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@p ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n\t}"
+                     : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]) : "r"(addr), "r"((int) take) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@p ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n\t}"
+                     : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]) : "r"(addr), "r"((int) take) : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, bool remote) {
-    float x;
-    if (remote) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
-    else asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
-    return x;
+__device__ __forceinline__ void ld_cluster_f32x2(uint32_t addr, bool remote, bool take, float &x, float &y) {
+    x = y = 0.f;
+    if (remote)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t@p ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n\t}"
+                     : "+f"(x), "+f"(y) : "r"(addr), "r"((int) take) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t@p ld.shared.v2.f32 {%0, %1}, [%2];\n\t}"
+                     : "+f"(x), "+f"(y) : "r"(addr), "r"((int) take) : "memory");
+}
+__device__ __forceinline__ void ld_cluster_f32(uint32_t addr, bool remote, bool take, float &x) {
+    x = 0.f;
+    if (remote)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p ld.shared::cluster.f32 %0, [%1];\n\t}" : "+f"(x) : "r"(addr), "r"((int) take) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p ld.shared.f32 %0, [%1];\n\t}" : "+f"(x) : "r"(addr), "r"((int) take) : "memory");
 }
 // a tile into L2 only
 __device__ __forceinline__ void prefetch_l2_2d(const CUtensorMap *m, int c0, int c1) {

@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
         prefetch_tmap(&tmap_w);
         prefetch_tmap(&tmap_x);
     }
-    if (kMoe && warp == 1) {
+    if (TOK <= 128 && warp == 1) {   // while the kernel before this one finishes
         tmem_alloc(&s_tmem, Cfg::kTmemCols);
         tmem_relinquish();
     }
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
     const int chunks = (a.k + 63) / 64;   // per expert
     const int64_t total = KIND == FR_DOWN ? (int64_t) n_active * chunks : chunks;
     const int l0 = (int) (total * rank / a.split), l1 = (int) (total * (rank + 1) / a.split);
-    if (!kMoe && warp == 1) {   // only now: the producer does not wait for it (a pair's allocation takes about half a microsecond)
+    if (TOK > 128 && warp == 1) {   // one CTA per SM starts when the kernel before it is done: the first loads do not wait for this (0.5 us)
         if constexpr (kPair) {
             tmem_alloc_pair(&s_tmem, Cfg::kTmemCols);
             tmem_relinquish_pair();

@@ -103,6 +103,19 @@ def test_few_rows(dt, M, N, K):
         _check(M, N, K, dt, act, with_bias=i % 2 == 0, with_res=i % 3 != 1, seed=10 * i)
 
 
+@pytest.mark.parametrize("M,N,K", [(65, 100, 1024), (129, 100, 1024), (192, 520, 2056), (200, 2056, 1024), (513, 4101, 64), (500, 3976, 1544),
+                                   (300, 3976, 1544), (300, 4101, 1544), (222, 2049, 4104), (200, 2056, 4096), (130, 4096, 128), (700, 512, 200)])
+def test_wide_blocks(M, N, K):
+    """Blocks of more than 128 tokens, with one to eight shares of the contraction, single CTAs and pairs, even and odd numbers of weight
+    blocks, and the write-out of several tokens at once with everything that may join it."""
+    assert _few(M, N, K)
+    _check(M, N, K, torch.bfloat16, "gelu", True, True)
+    _check(M, N, K, torch.float16, "silu", False, True, out_dtype=torch.float32)
+    if N % 8 == 0:
+        _check(M, N, K, torch.bfloat16, None, True, False, trans_b=False)
+    _check(M, N, K, torch.float16, "gelu_tanh", True, True, grad=True)
+
+
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("M,N,K", [(33000, 130, 1032), (40000, 257, 2048), (9000, 1001, 1000)])
 def test_tiles(dt, M, N, K):

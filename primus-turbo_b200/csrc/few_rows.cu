@@ -56,6 +56,7 @@ enum FewRowsKind { FR_LINEAR = 0, FR_GATE_UP = 1, FR_DOWN = 2 };
 struct FewRowsArgs {
     int rows;                // LINEAR: M; else tokens
     int n, k;                // features of the output (GATE_UP: of one half), contraction length
+    int stages;              // of the ring
     int split;               // CTAs (wide blocks: pairs of CTAs) of a cluster
     int fmt;                 // 0 = fp16, 1 = bf16 operands
     void *out;               // LINEAR / DOWN [rows, n]; GATE_UP [slots, n]
@@ -84,12 +85,14 @@ template <int TOK, bool PAIR> struct FrCfg {
     static constexpr int kStageBytes = kFrABytes + kBBytes;
     static constexpr int kCtas = TOK > 128 ? 1 : 2;           // per SM
     static constexpr int kStages = TOK <= 16 ? 6 : TOK <= 32 ? 5 : TOK <= 64 ? 4 : TOK <= 128 ? 3 : PAIR ? 6 : 5;
+    static constexpr int kMaxStages = kCtas == 2 ? 2 * kStages : kStages;   // of a launch that leaves an SM to each CTA
     static constexpr int kRing = kStages * kStageBytes;
     static constexpr int kIdSlots = TOK * kFrMaxTopK < kFrMaxSlots ? TOK * kFrMaxTopK : kFrMaxSlots;
-    static constexpr int kSmem = kRing + 1024 /* alignment */ + 2 * kIdSlots;
+    static constexpr int smem_bytes(int stages) { return stages * kStageBytes + 1024 /* alignment */ + 2 * kIdSlots; }
     static constexpr int kTmemCols = TOK < 32 ? 32 : TOK > 128 ? 256 : TOK;
     static_assert(TOK * kFrFeat * 4 <= kRing, "the partial block must fit the ring");
-    static_assert(kCtas * (kSmem + 3584 /* static and reserved */) <= 228 * 1024, "CTAs per SM");
+    static_assert(kCtas * (smem_bytes(kStages) + 3584 /* static and reserved */) <= 228 * 1024, "CTAs per SM");
+    static_assert(smem_bytes(kMaxStages) + 3584 <= 228 * 1024, "one CTA per SM");
 };
 
 // Four elements of each of ROWS rows, under predicates
@@ -129,14 +132,15 @@ template <int TOK, int KIND, bool PAIR>
 __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::kCtas)
     few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, FewRowsArgs a) {
     using Cfg = FrCfg<TOK, PAIR>;
-    constexpr int kStages = Cfg::kStages;
+    constexpr int kMaxStages = Cfg::kMaxStages;
+    const int stages = a.stages;
     constexpr bool kMoe = KIND != FR_LINEAR, kPair = PAIR;
     static_assert(!kMoe || (TOK <= 128 && !PAIR), "wide blocks are for dense products");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    int16_t *s_ids = reinterpret_cast<int16_t *>(ring + Cfg::kRing);   // [tokens * top_k], -1: no expert of this call
-    __shared__ uint64_t full_bar[kStages], empty_bar[kStages], done_bar;
-    __shared__ uint32_t s_tmem, s_mask[kStages], s_touched;   // s_mask: DOWN, which 16-token blocks a stage holds
+    int16_t *s_ids = reinterpret_cast<int16_t *>(ring + stages * Cfg::kStageBytes);   // [tokens * top_k], -1: no expert of this call
+    __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], done_bar;
+    __shared__ uint32_t s_tmem, s_mask[kMaxStages], s_touched;   // s_mask: DOWN, which 16-token blocks a stage holds
     __shared__ int s_abort, s_count;
     __shared__ uint32_t s_bits[kMoe ? 32 : 1];
     __shared__ int16_t s_active[KIND == FR_DOWN ? kMaxGroups : 1];
@@ -153,7 +157,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
 
     if (threadIdx.x == 0) {
         s_abort = 0;
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbar_init(&full_bar[s], kMoe ? 1 + 32 * Cfg::kEpiWarps : 1);   // the weights' bytes, and the copying threads
             mbar_init(&empty_bar[s], 1);
         }
@@ -170,7 +174,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
         // The first weight blocks on their way into L2 while the kernel before this one finishes.  A prefetch is not a read: were the
         // weight being written, L2 would hold the new values all the same.
         const int chunks = (a.k + 63) / 64, l0 = chunks * rank / a.split, l1 = chunks * (rank + 1) / a.split;
-        for (int l = l0; l < min(l1, l0 + kStages); ++l) {
+        for (int l = l0; l < min(l1, l0 + stages); ++l) {
             if (a.w_mn) {
                 prefetch_l2_2d(&tmap_w, tile * kFrFeat * 2, l * 64);
                 prefetch_l2_2d(&tmap_w, tile * kFrFeat * 2 + 128, l * 64);
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
                             tma_load_2d_pair_hint(A, &tmap_w, full, l * 128, tile * kFrFeat, stream_pol);
                         }
                         tma_load_2d_pair_hint(A + kFrABytes, &tmap_x, full, l * 128, x_row, keep_pol);
-                        if (++stage == kStages) { stage = 0; phase ^= 1; }
+                        if (++stage == stages) { stage = 0; phase ^= 1; }
                         continue;
                     }
                     mbar_arrive_expect_tx(&full_bar[stage], kFrABytes + x_bytes);
@@ -308,7 +312,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
                         }
                         tma_load_2d_hint(A + kFrABytes, &tmap_x, &full_bar[stage], l * 128, x_row, keep_pol);
                     }
-                    if (++stage == kStages) { stage = 0; phase ^= 1; }
+                    if (++stage == stages) { stage = 0; phase ^= 1; }
                 }
             }
         } else {
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
                 }
                 if (!(ok = __shfl_sync(0xffffffffu, (int) ok, 0) != 0)) break;
                 if (++c == chunks) { c = 0; ++ai; }
-                if (++stage == kStages) { stage = 0; phase ^= 1; }
+                if (++stage == stages) { stage = 0; phase ^= 1; }
             }
         }
     } else if (warp == 1) {
@@ -377,7 +381,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
                 touched |= used;
                 if constexpr (kPair) tc_commit_pair(&empty_bar[stage], both);
                 else tc_commit(&empty_bar[stage]);
-                if (++stage == kStages) { stage = 0; phase ^= 1; }
+                if (++stage == stages) { stage = 0; phase ^= 1; }
             }
             if (ok) {
                 s_touched = touched;
@@ -438,7 +442,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
                 }
                 cp_async_arrive_noinc(&full_bar[stage]);
                 if (++c == chunks) { c = 0; ++ai; }
-                if (++stage == kStages) { stage = 0; phase ^= 1; }
+                if (++stage == stages) { stage = 0; phase ^= 1; }
             }
         }
     }
@@ -640,23 +644,36 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
 }
 
 // ------------------------------------------------------------------------------------------------ host side
+// CTAs that are resident at once in clusters of `ctas`, two or one (wide) per SM (GPCs do not divide evenly; measured on 148 SMs with one CTA per
+// SM: 33 clusters of four and 14 of eight run together, 34 and 16 in two waves).  With two CTAs per SM no such loss was seen.  The driver's occupancy query is not asked: it
+// answers one CTA per SM for these kernels, and launches after it do run one per SM (333 x 4096 x 4096 in blocks of 128: 29.4 us, else 23.0).
+static double fr_resident(bool wide, int ctas) {
+    const double sms = sm_count();
+    return !wide ? 2.0 * sms : ctas <= 2 ? sms : ctas == 4 ? sms * 33 / 37 : sms * 28 / 37;
+}
+// Whether a launch of `ctas` CTAs on a kernel for two per SM takes the ring of both: if each of them gets an SM for itself.  Measured (us): 64 x 4096 x
+// 4096 12.9 -> 12.0, 4000 x 512 x 512 11.9 -> 11.3; experts, 37 tokens in two of 60 of 1744 x 568 66.9 -> 63.9, but with 16 clusters of eight, of which two
+// would start late, 64 tokens in six of 64 of 2048 x 1408 215 -> 271.  Up to 16 tokens it gains nothing (1 x 1024 x 4096 6.5 -> 6.7).
+static bool fr_deep(int tok, int64_t ctas, int cluster) { return tok > 16 && tok <= 128 && (double) ctas <= fr_resident(true, cluster); }
+
 template <int TOK, int KIND, bool PAIR = false>
-static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRowsArgs &a, int64_t tiles, int64_t grid_y, cudaStream_t st) {
+static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, FewRowsArgs a, int64_t tiles, int64_t grid_y, cudaStream_t st) {
     using Cfg = FrCfg<TOK, PAIR>;
     auto kern = few_rows_kernel<TOK, KIND, PAIR>;
     static bool attr_set[64] = {};   // per instantiation and device
     const int dev = current_device_slot();
     if (!attr_set[dev]) {
-        PT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
+        PT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(Cfg::kMaxStages)));
         attr_set[dev] = true;
     }
     const int cluster_ctas = PAIR ? 2 * a.split : a.split;
     if (PAIR) tiles = ceil_div(tiles, 2);
     PT_REQUIRE(tiles * cluster_ctas < (1ll << 31) && grid_y < 65536, "few-row product: grid too large");
+    a.stages = fr_deep(TOK, tiles * cluster_ctas * grid_y, cluster_ctas) ? Cfg::kMaxStages : Cfg::kStages;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) (tiles * cluster_ctas), (unsigned) grid_y);
     cfg.blockDim = dim3(Cfg::kThreads);
-    cfg.dynamicSmemBytes = Cfg::kSmem;
+    cfg.dynamicSmemBytes = (size_t) Cfg::smem_bytes(a.stages);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -670,17 +687,9 @@ static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, const FewRows
     return PT_OK;
 }
 
-// SMs that clusters of `ctas` CTAs can use at once with one CTA per SM (GPCs do not divide evenly; measured on 148 SMs: 33 clusters of four and 12 of
-// eight run together, 34 and 16 in two waves).  With two CTAs per SM no such loss was seen.  The driver's occupancy query is not asked: it
-// answers one CTA per SM for these kernels, and launches after it do run one per SM (333 x 4096 x 4096 in blocks of 128: 29.4 us, else 23.0).
-static double fr_resident(bool wide, int ctas) {
-    const double sms = sm_count();
-    return !wide ? 2.0 * sms : ctas <= 2 ? sms : ctas == 4 ? sms * 33 / 37 : sms * 2 / 3;
-}
-
 // Estimated time of a launch in us: `tiles` weight blocks wide, `blocks` blocks of `block` tokens on the kernel for up to `tok`, `chunks` 64-wide
 // steps of the contraction, s CTAs or pairs per cluster.  A fixed part, and the longest of: a CTA's own steps (an SM takes in about 108 GB/s),
-// the bytes from and to memory (one 100 KiB ring per SM does not quite saturate it), all stages out of L2 (15 TB/s).  CTAs beyond those
+// the bytes from and to memory (one CTA per SM does not quite saturate it), all stages out of L2 (15 TB/s).  CTAs beyond those
 // resident at once are further waves.  Measured (us, SiLU epilogue; rows x features x K, kernel : block / s): 64 x 4096 x 4096 64 / 1, 2, 4, 8 24.8, 16.1,
 // 12.8, 13.0; 129 x 4096 x 4096 128 : 80 / 4 15.6, 192 : 144 / 2, 4 17.1, 13.6, 256 : 144 / 2, 4 16.7, 26.5 (two waves); 333 x 4096 x 4096 128 : 112 / 2
 // 23.3, 192 : 176 / 2 19.0, 256 : 176 / 2 19.0; 512 x 4096 x 4096 128 : 128 / 2 24.6, 192 : 128 / 1 24.8, 256 : 256 / 2 21.1; 512 x 4096 x 14336 192 : 176 / 1
@@ -691,10 +700,12 @@ static double fr_cost(int tok, int block, int64_t tiles, int64_t blocks, int64_t
     const double ctas = (double) (tiles * blocks * s), share = ctas / fr_resident(wide, pair ? 2 * s : s);
     const double waves = std::max(1.0, wide ? std::ceil(share) : share);   // two CTAs per SM: a later one starts when either ends
     const double x_bytes = (pair ? 64.0 : 128.0) * block;   // of tokens per step
-    double step = pair ? 0.18 + 0.0007 * block : wide ? 0.2 + 0.0005 * block : 0.25 + 0.00125 * block;
+    // (Counting the deeper ring for 128 tokens too chose it over the wide kernel, whose write-out is faster: 512 x 1536 x 1024 9.7 -> 11.9 us.)
+    const bool own_sm = wide || (tok <= 64 && fr_deep(tok, tiles * blocks * s, s));
+    double step = pair ? 0.18 + 0.0007 * block : own_sm ? 0.2 + 0.0005 * block : 0.25 + 0.00125 * block;
     if (!wide && ctas > sm_count()) step = std::max(step, 2.0 * (kFrABytes + x_bytes) / 108e3);   // two CTAs share what an SM takes in
     const double rows = (double) (blocks * block), k_bytes = 128.0 * (double) chunks;
-    const double memory = ((double) tiles * kFrFeat * (k_bytes + 2.0 * rows) + rows * k_bytes) / (!wide && ctas <= sm_count() ? 5.8e6 : 6.5e6);
+    const double memory = ((double) tiles * kFrFeat * (k_bytes + 2.0 * rows) + rows * k_bytes) / (!wide && ctas <= sm_count() ? 5.6e6 : 6.5e6);
     const double l2 = (double) (tiles * blocks * chunks) * (kFrABytes + x_bytes) / 15e6;
     double fixed;   // launch, first bytes, exchange of partial sums, write-out
     if (pair) fixed = s == 1 ? 5.7 + 0.0025 * block : 7.2 + 0.0075 * block;

@@ -49,6 +49,7 @@ constexpr int kFrABytes = kFrFeat * 128;  // a weight block: 128 rows of 64 16-b
 constexpr int kFrMaxSlots = 2048;         // tokens x experts per token
 constexpr int kFrMaxTopK = 32;
 constexpr int kFrMaxSplit = 8;            // CTAs of a cluster
+constexpr int kFrMaxStages = 12;          // of a ring
 constexpr int kFrPairTok = 256;           // the block that pairs of CTAs take
 
 enum FewRowsKind { FR_LINEAR = 0, FR_GATE_UP = 1, FR_DOWN = 2 };
@@ -56,7 +57,8 @@ enum FewRowsKind { FR_LINEAR = 0, FR_GATE_UP = 1, FR_DOWN = 2 };
 struct FewRowsArgs {
     int rows;                // LINEAR: M; else tokens
     int n, k;                // features of the output (GATE_UP: of one half), contraction length
-    int stages;              // of the ring
+    int ring_bytes;          // of shared memory for stages
+    int x_rows, stages;      // token rows of a stage, a multiple of 8; how many stages fit.  GATE_UP: by the expert's tokens, in the kernel
     int split;               // CTAs (wide blocks: pairs of CTAs) of a cluster
     int fmt;                 // 0 = fp16, 1 = bf16 operands
     void *out;               // LINEAR / DOWN [rows, n]; GATE_UP [slots, n]
@@ -81,18 +83,16 @@ struct FewRowsArgs {
 template <int TOK, bool PAIR> struct FrCfg {
     static constexpr int kEpiWarps = TOK <= 32 ? 4 : TOK <= 128 ? 8 : 16;   // per quarter of the accumulator's rows: one, or two that share the tokens
     static constexpr int kThreads = 64 + 32 * kEpiWarps;
-    static constexpr int kBBytes = (PAIR ? TOK / 2 : TOK) * 128;
-    static constexpr int kStageBytes = kFrABytes + kBBytes;
     static constexpr int kCtas = TOK > 128 ? 1 : 2;           // per SM
-    static constexpr int kStages = TOK <= 16 ? 6 : TOK <= 32 ? 5 : TOK <= 64 ? 4 : TOK <= 128 ? 3 : PAIR ? 6 : 5;
-    static constexpr int kMaxStages = kCtas == 2 ? 2 * kStages : kStages;   // of a launch that leaves an SM to each CTA
-    static constexpr int kRing = kStages * kStageBytes;
+    // Six, five, four and three full stages of two CTAs per SM; five of single CTAs, six of pairs.  Smaller stages fit more often.
+    static constexpr int kRing = (TOK <= 16 ? 6 : TOK <= 32 ? 5 : TOK <= 64 ? 4 : TOK <= 128 ? 3 : PAIR ? 6 : 5) * (kFrABytes + (PAIR ? TOK / 2 : TOK) * 128);
+    static constexpr int kMaxRing = kCtas * kRing;            // of a launch that leaves an SM to each CTA
     static constexpr int kIdSlots = TOK * kFrMaxTopK < kFrMaxSlots ? TOK * kFrMaxTopK : kFrMaxSlots;
-    static constexpr int smem_bytes(int stages) { return stages * kStageBytes + 1024 /* alignment */ + 2 * kIdSlots; }
+    static constexpr int smem_bytes(int ring) { return ring + 1024 /* alignment */ + 2 * kIdSlots; }
     static constexpr int kTmemCols = TOK < 32 ? 32 : TOK > 128 ? 256 : TOK;
     static_assert(TOK * kFrFeat * 4 <= kRing, "the partial block must fit the ring");
-    static_assert(kCtas * (smem_bytes(kStages) + 3584 /* static and reserved */) <= 228 * 1024, "CTAs per SM");
-    static_assert(smem_bytes(kMaxStages) + 3584 <= 228 * 1024, "one CTA per SM");
+    static_assert(kCtas * (smem_bytes(kRing) + 3584 /* static and reserved */) <= 228 * 1024, "CTAs per SM");
+    static_assert(smem_bytes(kMaxRing) + 3584 <= 228 * 1024, "one CTA per SM");
 };
 
 // Four elements of each of ROWS rows, under predicates
@@ -132,15 +132,13 @@ template <int TOK, int KIND, bool PAIR>
 __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::kCtas)
     few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, FewRowsArgs a) {
     using Cfg = FrCfg<TOK, PAIR>;
-    constexpr int kMaxStages = Cfg::kMaxStages;
-    const int stages = a.stages;
     constexpr bool kMoe = KIND != FR_LINEAR, kPair = PAIR;
     static_assert(!kMoe || (TOK <= 128 && !PAIR), "wide blocks are for dense products");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    int16_t *s_ids = reinterpret_cast<int16_t *>(ring + stages * Cfg::kStageBytes);   // [tokens * top_k], -1: no expert of this call
-    __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], done_bar;
-    __shared__ uint32_t s_tmem, s_mask[kMaxStages], s_touched;   // s_mask: DOWN, which 16-token blocks a stage holds
+    int16_t *s_ids = reinterpret_cast<int16_t *>(ring + a.ring_bytes);   // [tokens * top_k], -1: no expert of this call
+    __shared__ uint64_t full_bar[kFrMaxStages], empty_bar[kFrMaxStages], done_bar;
+    __shared__ uint32_t s_tmem, s_mask[kFrMaxStages], s_touched;   // s_mask: DOWN, which 16-token blocks a stage holds
     __shared__ int s_abort, s_count;
     __shared__ uint32_t s_bits[kMoe ? 32 : 1];
     __shared__ int16_t s_active[KIND == FR_DOWN ? kMaxGroups : 1];
@@ -157,7 +155,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
 
     if (threadIdx.x == 0) {
         s_abort = 0;
-        for (int s = 0; s < stages; ++s) {
+        for (int s = 0; s < (KIND == FR_GATE_UP ? kFrMaxStages : a.stages); ++s) {
             mbar_init(&full_bar[s], kMoe ? 1 + 32 * Cfg::kEpiWarps : 1);   // the weights' bytes, and the copying threads
             mbar_init(&empty_bar[s], 1);
         }
@@ -173,8 +171,9 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
     if (KIND == FR_LINEAR && threadIdx.x == 64 && blockIdx.y == 0 && tile * kFrFeat < a.n) {
         // The first weight blocks on their way into L2 while the kernel before this one finishes.  A prefetch is not a read: were the
         // weight being written, L2 would hold the new values all the same.
+        constexpr int kPrefetch = 6;
         const int chunks = (a.k + 63) / 64, l0 = chunks * rank / a.split, l1 = chunks * (rank + 1) / a.split;
-        for (int l = l0; l < min(l1, l0 + stages); ++l) {
+        for (int l = l0; l < min(l1, l0 + kPrefetch); ++l) {
             if (a.w_mn) {
                 prefetch_l2_2d(&tmap_w, tile * kFrFeat * 2, l * 64);
                 prefetch_l2_2d(&tmap_w, tile * kFrFeat * 2 + 128, l * 64);
@@ -257,7 +256,9 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
     if constexpr (KIND == FR_GATE_UP) cnt = s_count;
     if constexpr (KIND == FR_DOWN) cnt = T;
 
-    // ---- this CTA's share of the contraction
+    // ---- the stages and this CTA's share of the contraction
+    const int stage_bytes = kFrABytes + (KIND == FR_GATE_UP ? (cnt + 15) / 16 * 16 : a.x_rows) * 128;
+    const int stages = KIND == FR_GATE_UP ? min(kFrMaxStages, a.ring_bytes / stage_bytes) : a.stages;
     const int chunks = (a.k + 63) / 64;   // per expert
     const int64_t total = KIND == FR_DOWN ? (int64_t) n_active * chunks : chunks;
     const int l0 = (int) (total * rank / a.split), l1 = (int) (total * (rank + 1) / a.split);
@@ -281,11 +282,11 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
             if (elect_one()) {
                 const int expert_row = expert * 2 * a.n + tile * 64;
                 const int x_row = (int) blockIdx.y * a.block + half * 8 * ((cnt + 15) / 16);
-                const uint32_t x_bytes = kMoe ? 0 : (kPair ? a.block / 2 : a.block) * 128;
+                const uint32_t x_bytes = kMoe ? 0 : a.x_rows * 128;
                 uint32_t stage = 0, phase = 0;
                 for (int l = l0; l < l1; ++l) {
                     if (!(ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag))) break;
-                    uint8_t *A = ring + stage * Cfg::kStageBytes;
+                    uint8_t *A = ring + stage * stage_bytes;
                     if constexpr (kPair) {   // the bytes of both CTAs on the barrier of the first
                         const uint32_t full = map_to_rank(&full_bar[stage], cta_rank & ~1);
                         if (half == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * (kFrABytes + x_bytes));
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
                 if (lane == 0 && (ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag))) {
                     s_mask[stage] = blocks;
                     mbar_arrive_expect_tx(&full_bar[stage], kFrABytes);
-                    tma_load_2d_hint(ring + stage * Cfg::kStageBytes, &tmap_w, &full_bar[stage], c * 128, s_active[ai] * a.n + tile * kFrFeat, stream_pol);
+                    tma_load_2d_hint(ring + stage * stage_bytes, &tmap_w, &full_bar[stage], c * 128, s_active[ai] * a.n + tile * kFrFeat, stream_pol);
                 }
                 if (!(ok = __shfl_sync(0xffffffffu, (int) ok, 0) != 0)) break;
                 if (++c == chunks) { c = 0; ++ai; }
@@ -359,7 +360,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
                 if (!(ok = mbar_wait(&full_bar[stage], phase, abort_flag))) break;
                 if constexpr (kMoe) fence_proxy_async_smem();   // the copied rows were written through the generic proxy
                 tc_fence_after_sync();
-                const uint32_t A = smem_u32(ring + stage * Cfg::kStageBytes);
+                const uint32_t A = smem_u32(ring + stage * stage_bytes);
                 const uint64_t a_desc = w_mn ? smem_desc_sw128_mn(A, kFrABytes / 2) : smem_desc_sw128(A);
                 uint32_t m = KIND == FR_DOWN ? s_mask[stage] : all;
                 const uint32_t used = m;
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
                     const bool inside = k0 + c16 < a.x_pitch;
 #pragma unroll
                     for (int i = 0; i < kCopies; ++i)
-                        cp_async_16_or_zero(ring + stage * Cfg::kStageBytes + dst[i], src[i] != nullptr && inside ? src[i] + k0 : reinterpret_cast<const uint8_t *>(a.x),
+                        cp_async_16_or_zero(ring + stage * stage_bytes + dst[i], src[i] != nullptr && inside ? src[i] + k0 : reinterpret_cast<const uint8_t *>(a.x),
                                             src[i] != nullptr && inside);
                 }
                 cp_async_arrive_noinc(&full_bar[stage]);
@@ -663,17 +664,19 @@ static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, FewRowsArgs a
     static bool attr_set[64] = {};   // per instantiation and device
     const int dev = current_device_slot();
     if (!attr_set[dev]) {
-        PT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(Cfg::kMaxStages)));
+        PT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(Cfg::kMaxRing)));
         attr_set[dev] = true;
     }
     const int cluster_ctas = PAIR ? 2 * a.split : a.split;
     if (PAIR) tiles = ceil_div(tiles, 2);
     PT_REQUIRE(tiles * cluster_ctas < (1ll << 31) && grid_y < 65536, "few-row product: grid too large");
-    a.stages = fr_deep(TOK, tiles * cluster_ctas * grid_y, cluster_ctas) ? Cfg::kMaxStages : Cfg::kStages;
+    a.ring_bytes = fr_deep(TOK, tiles * cluster_ctas * grid_y, cluster_ctas) ? Cfg::kMaxRing : Cfg::kRing;
+    a.x_rows = KIND != FR_LINEAR ? TOK : PAIR ? a.block / 2 : a.block;
+    a.stages = std::min(kFrMaxStages, a.ring_bytes / (kFrABytes + a.x_rows * 128));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) (tiles * cluster_ctas), (unsigned) grid_y);
     cfg.blockDim = dim3(Cfg::kThreads);
-    cfg.dynamicSmemBytes = (size_t) Cfg::smem_bytes(a.stages);
+    cfg.dynamicSmemBytes = (size_t) Cfg::smem_bytes(a.ring_bytes);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
     }
     if (KIND != FR_DOWN) {   // DOWN waits later: what it reads up to there is not written by the kernel before it
         grid_dep_wait();
-        grid_dep_launch();
+        if (TOK <= 128 && warp == 1) grid_dep_launch();   // after this warp's allocation: what is launched then cannot wait for us holding its columns
     }
 
     // ---- routing: which experts are chosen, and by whom
@@ -270,6 +270,7 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
             tmem_alloc(&s_tmem, Cfg::kTmemCols);
             tmem_relinquish();
         }
+        grid_dep_launch();
         __syncwarp();
     }
     volatile int *abort_flag = &s_abort;

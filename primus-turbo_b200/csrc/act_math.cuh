@@ -50,16 +50,7 @@ __device__ __forceinline__ float gelu_epilogue(float z) {
     return (z > 0.0f ? z : 0.0f * z) - 0.5f * x * poly * __expf(-0.5f * x * x);   // 0 z: a NaN stays one
 }
 
-// The activation chosen at run time (uniform over the launch), and the same for a lane's values under one branch.
-__device__ __forceinline__ float act_any(int act, float v) {
-    switch (act) {
-    case PT_ACT_SILU: return act_value<PT_ACT_SILU>(v);
-    case PT_ACT_GELU: return gelu_epilogue(v);
-    case PT_ACT_RELU: return act_value<PT_ACT_RELU>(v);
-    case PT_ACT_GELU_TANH: return act_value<PT_ACT_GELU_TANH>(v);
-    default: return v;
-    }
-}
+// The activation chosen at run time (uniform over the launch), for a lane's values under one branch.
 template <int ROWS> __device__ __forceinline__ void act_any_all(int act, float (&v)[ROWS][4]) {
     auto all = [&](auto f) {
 #pragma unroll

@@ -510,129 +510,141 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
     // instantiations below make one do.
     const int step = a.split * (Cfg::kThreads / 32);   // tokens between two of this warp's
     auto write_out = [&](auto at_once, auto others) {
-    constexpr int kAtOnce = decltype(at_once)::value, kOthers = decltype(others)::value;
-    for (int t0 = rank + a.split * warp; t0 < cnt; t0 += kAtOnce * step) {
-        float v[kAtOnce][4];
-        bool in[kAtOnce];
+        constexpr int kAtOnce = decltype(at_once)::value, kOthers = decltype(others)::value;
+        for (int t0 = rank + a.split * warp; t0 < cnt; t0 += kAtOnce * step) {
+            float v[kAtOnce][4];
+            bool in[kAtOnce];
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) in[u] = t0 + u * step < cnt;
-        auto load = [&](int u, uint32_t src, bool remote, float (&w)[4]) {
-            if (KIND == FR_GATE_UP) {
-                ld_cluster_f32x2(src, remote, in[u], w[0], w[1]);
-                ld_cluster_f32x2(src + 256, remote, in[u], w[2], w[3]);
-            } else if (vec) {
-                ld_cluster_f32x4(src, remote, in[u], w);
-            } else {
+            for (int u = 0; u < kAtOnce; ++u) in[u] = t0 + u * step < cnt;
+            auto load = [&](int u, uint32_t src, bool remote, float (&w)[4]) {
+                if (KIND == FR_GATE_UP) {
+                    ld_cluster_f32x2(src, remote, in[u], w[0], w[1]);
+                    ld_cluster_f32x2(src + 256, remote, in[u], w[2], w[3]);
+                } else if (vec) {
+                    ld_cluster_f32x4(src, remote, in[u], w);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) ld_cluster_f32(src + 128 * i, remote, in[u], w[i]);
-            }
-        };
-        auto row_at = [&](int u) { return part_addr + (uint32_t) (t0 + u * step) * (kFrFeat * 4) + lane_at; };
-        float w[kOthers > 0 ? kOthers : 1][kAtOnce][4];
-#pragma unroll
-        for (int s = 0; s < kOthers; ++s) {
-            const int other = (rank + 1 + s) & (a.split - 1);
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u) load(u, map_addr_to_rank(row_at(u), kPair ? 2 * other + half : other), true, w[s][u]);
-        }
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) load(u, row_at(u), false, v[u]);
-#pragma unroll
-        for (int s = 0; s < kOthers; ++s)
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[u][i] += w[s][u][i];
-        if constexpr (KIND == FR_GATE_UP) {
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u) {
-                const int t = t0 + u * step;
-                if (!in[u] || f0 >= a.n) continue;
-                const float p = s_prob[t];
-                const float h0 = act_any(a.act, v[u][0]) * v[u][2] * p, h1 = act_any(a.act, v[u][1]) * v[u][3] * p;
-                *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.out) + (int64_t) s_slot[t] * a.n + f0) =
-                    a.fmt ? pack2<__nv_bfloat16>(h0, h1) : pack2<__half>(h0, h1);
-            }
-        } else if constexpr (KIND == FR_DOWN) {
-            bool st[kAtOnce];
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u) st[u] = in[u] && f0 < a.n;
-            store4_rows<kAtOnce>(a.out, a.out_dtype, (int64_t) t0 * a.n + f0, (int64_t) step * a.n, st, v);
-        } else {
-            const int64_t o0 = ((int64_t) blockIdx.y * a.block + t0) * a.n + f0, o_step = (int64_t) step * a.n;
-            const int zt = a.fmt ? PT_BF16 : PT_F16;
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[u][i] += bias[i];
-            if (vec) {
-                bool st[kAtOnce];
-#pragma unroll
-                for (int u = 0; u < kAtOnce; ++u) st[u] = in[u] && f0 < a.n;
-                uint4 res[kAtOnce];
-                if (a.residual != nullptr) load4_rows<kAtOnce>(a.residual, a.out_dtype, o0, o_step, st, res);
-                if (a.z != nullptr) store4_rows<kAtOnce>(a.z, zt, o0, o_step, st, v);
-                act_any_all<kAtOnce>(a.act, v);
-                if (a.residual != nullptr) {
-#pragma unroll
-                    for (int u = 0; u < kAtOnce; ++u) {
-                        float x[4];
-                        raw4_as_f32(res[u], a.out_dtype, x);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[u][i] += x[i];
-                    }
+                    for (int i = 0; i < 4; ++i) ld_cluster_f32(src + 128 * i, remote, in[u], w[i]);
                 }
-                store4_rows<kAtOnce>(a.out, a.out_dtype, o0, o_step, st, v);
-            } else {
-                bool st[kAtOnce][4];
+            };
+            auto row_at = [&](int u) { return part_addr + (uint32_t) (t0 + u * step) * (kFrFeat * 4) + lane_at; };
+            float w[kOthers > 0 ? kOthers : 1][kAtOnce][4];
+#pragma unroll
+            for (int s = 0; s < kOthers; ++s) {
+                const int other = (rank + 1 + s) & (a.split - 1);
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) load(u, map_addr_to_rank(row_at(u), kPair ? 2 * other + half : other), true, w[s][u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) load(u, row_at(u), false, v[u]);
+#pragma unroll
+            for (int s = 0; s < kOthers; ++s)
 #pragma unroll
                 for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) st[u][i] = in[u] && f0 + 32 * i < a.n;
-                uint32_t res[kAtOnce][4];   // raw, all on their way before the first is used
-                if (a.residual != nullptr) {
-                    auto fetch = [&](auto *p) {
+                    for (int i = 0; i < 4; ++i) v[u][i] += w[s][u][i];
+            if constexpr (KIND == FR_GATE_UP) {
+                float p[kAtOnce];
+                int slot[kAtOnce];
 #pragma unroll
-                        for (int u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                res[u][i] = 0;
-                                if (st[u][i]) res[u][i] = p[o0 + u * o_step + 32 * i];
-                            }
-                    };
-                    if (a.out_dtype == PT_F32) fetch(reinterpret_cast<const uint32_t *>(a.residual));
-                    else fetch(reinterpret_cast<const uint16_t *>(a.residual));
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const int t = in[u] ? t0 + u * step : 0;
+                    p[u] = s_prob[t];
+                    slot[u] = s_slot[t];
                 }
-                auto put = [&](void *out, int dtype) {
-                    if (dtype == PT_F32) {
+                auto gated = [&](auto f) {
+#pragma unroll
+                    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) v[u][i] = f(v[u][i]) * v[u][2 + i] * p[u];
+                };
+                if (a.act == PT_ACT_SILU) gated([](float x) { return act_value<PT_ACT_SILU>(x); });
+                else gated([](float x) { return gelu_epilogue(x); });
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const uint32_t h = a.fmt ? pack2<__nv_bfloat16>(v[u][0], v[u][1]) : pack2<__half>(v[u][0], v[u][1]);
+                    if (in[u] && f0 < a.n) *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.out) + (int64_t) slot[u] * a.n + f0) = h;
+                }
+            } else if constexpr (KIND == FR_DOWN) {
+                bool st[kAtOnce];
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) st[u] = in[u] && f0 < a.n;
+                store4_rows<kAtOnce>(a.out, a.out_dtype, (int64_t) t0 * a.n + f0, (int64_t) step * a.n, st, v);
+            } else {
+                const int64_t o0 = ((int64_t) blockIdx.y * a.block + t0) * a.n + f0, o_step = (int64_t) step * a.n;
+                const int zt = a.fmt ? PT_BF16 : PT_F16;
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[u][i] += bias[i];
+                if (vec) {
+                    bool st[kAtOnce];
+#pragma unroll
+                    for (int u = 0; u < kAtOnce; ++u) st[u] = in[u] && f0 < a.n;
+                    uint4 res[kAtOnce];
+                    if (a.residual != nullptr) load4_rows<kAtOnce>(a.residual, a.out_dtype, o0, o_step, st, res);
+                    if (a.z != nullptr) store4_rows<kAtOnce>(a.z, zt, o0, o_step, st, v);
+                    act_any_all<kAtOnce>(a.act, v);
+                    if (a.residual != nullptr) {
+#pragma unroll
+                        for (int u = 0; u < kAtOnce; ++u) {
+                            float x[4];
+                            raw4_as_f32(res[u], a.out_dtype, x);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[u][i] += x[i];
+                        }
+                    }
+                    store4_rows<kAtOnce>(a.out, a.out_dtype, o0, o_step, st, v);
+                } else {
+                    bool st[kAtOnce][4];
+#pragma unroll
+                    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) st[u][i] = in[u] && f0 + 32 * i < a.n;
+                    uint32_t res[kAtOnce][4];   // raw, all on their way before the first is used
+                    if (a.residual != nullptr) {
+                        auto fetch = [&](auto *p) {
+#pragma unroll
+                            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    res[u][i] = 0;
+                                    if (st[u][i]) res[u][i] = p[o0 + u * o_step + 32 * i];
+                                }
+                        };
+                        if (a.out_dtype == PT_F32) fetch(reinterpret_cast<const uint32_t *>(a.residual));
+                        else fetch(reinterpret_cast<const uint16_t *>(a.residual));
+                    }
+                    auto put = [&](void *out, int dtype) {
+                        if (dtype == PT_F32) {
+#pragma unroll
+                            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (st[u][i]) reinterpret_cast<float *>(out)[o0 + u * o_step + 32 * i] = v[u][i];
+                        } else {
+#pragma unroll
+                            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const uint32_t h = dtype == PT_BF16 ? pack2<__nv_bfloat16>(v[u][i], 0.f) : pack2<__half>(v[u][i], 0.f);
+                                    if (st[u][i]) reinterpret_cast<uint16_t *>(out)[o0 + u * o_step + 32 * i] = (uint16_t) h;
+                                }
+                        }
+                    };
+                    if (a.z != nullptr) put(a.z, zt);
+                    act_any_all<kAtOnce>(a.act, v);
+                    if (a.residual != nullptr) {
 #pragma unroll
                         for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                if (st[u][i]) reinterpret_cast<float *>(out)[o0 + u * o_step + 32 * i] = v[u][i];
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t h = dtype == PT_BF16 ? pack2<__nv_bfloat16>(v[u][i], 0.f) : pack2<__half>(v[u][i], 0.f);
-                                if (st[u][i]) reinterpret_cast<uint16_t *>(out)[o0 + u * o_step + 32 * i] = (uint16_t) h;
-                            }
+                                v[u][i] += a.out_dtype == PT_F32 ? __uint_as_float(res[u][i]) : a.out_dtype == PT_BF16 ? lo_f32<__nv_bfloat16>(res[u][i]) : lo_f32<__half>(res[u][i]);
                     }
-                };
-                if (a.z != nullptr) put(a.z, zt);
-                act_any_all<kAtOnce>(a.act, v);
-                if (a.residual != nullptr) {
-#pragma unroll
-                    for (int u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            v[u][i] += a.out_dtype == PT_F32 ? __uint_as_float(res[u][i]) : a.out_dtype == PT_BF16 ? lo_f32<__nv_bfloat16>(res[u][i]) : lo_f32<__half>(res[u][i]);
+                    put(a.out, a.out_dtype);
                 }
-                put(a.out, a.out_dtype);
             }
         }
-    }
     };
     using std::integral_constant;
     if (a.split == 1) write_out(integral_constant<int, TOK <= 16 ? 1 : TOK <= 32 ? 2 : 4>(), integral_constant<int, 0>());

@@ -87,12 +87,6 @@ __device__ __forceinline__ uint4 load4_raw(const void *p, int dtype, int64_t i) 
     const uint2 h = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + i);
     return make_uint4(h.x, h.y, 0u, 0u);
 }
-__device__ __forceinline__ void store4_from_f32(void *p, int dtype, int64_t i, const float (&v)[4]) {
-    if (dtype == PT_F32) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
-    else if (dtype == PT_BF16)
-        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p) + i) = make_uint2(pack2<__nv_bfloat16>(v[0], v[1]), pack2<__nv_bfloat16>(v[2], v[3]));
-    else *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p) + i) = make_uint2(pack2<__half>(v[0], v[1]), pack2<__half>(v[2], v[3]));
-}
 
 // few_rows.cu: y = act(a . b^T + bias) + residual for few rows of a
 int few_rows_linear(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype,

@@ -20,8 +20,8 @@
 //   all         sum over the cluster, epilogue, write-out
 //
 // Measured (B200, bf16, replayed graphs, inputs beyond L2): 1 x 14336 x 4096 (rows, features, K) 22.0 us, 5.3 TB/s of weights; 1 x 64128 x 4096
-// 81 us, 6.5 TB/s; 64 x 4096 x 4096 12.8 us; 129 x 4096 x 4096 13.6 us; 333 x 4096 x 4096 19.0 us, 0.59 PFLOP/s.  One token through eight experts of 7168 x 2048 114 us, 6.2 TB/s; 64 tokens on 28
-// of 32 such experts 388 us, 6.4 TB/s.
+// 81 us, 6.5 TB/s; 64 x 4096 x 4096 11.7 us; 129 x 4096 x 4096 13.6 us; 333 x 4096 x 4096 19.0 us, 0.59 PFLOP/s.  One token through eight
+// experts of 7168 x 2048 114 us, 6.2 TB/s; 64 tokens on 28 of 32 such experts 375 to 388 us, 6.5 TB/s.
 //
 // Mixture, two kernels:
 //   GATE_UP  grid (blocks of 64 features x split, chosen experts): the block is 64 gate rows and the 64 up rows that belong to them.
@@ -708,8 +708,8 @@ static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, FewRowsArgs a
 // the bytes from and to memory (one CTA per SM does not quite saturate it), all stages out of L2 (15 TB/s).  CTAs beyond those
 // resident at once are further waves.  Measured (us, SiLU epilogue; rows x features x K, kernel : block / s): 64 x 4096 x 4096 64 / 1, 2, 4, 8 24.8, 16.1,
 // 12.8, 13.0; 129 x 4096 x 4096 128 : 80 / 4 15.6, 192 : 144 / 2, 4 17.1, 13.6, 256 : 144 / 2, 4 16.7, 26.5 (two waves); 333 x 4096 x 4096 128 : 112 / 2
-// 23.3, 192 : 176 / 2 19.0, 256 : 176 / 2 19.0; 512 x 4096 x 4096 128 : 128 / 2 24.6, 192 : 128 / 1 24.8, 256 : 256 / 2 21.1; 512 x 4096 x 14336 192 : 176 / 1
-// 78, 256 : 256 / 2 47.7.  What the estimate picks was within 5 % of the best in 30 of the 36 sizes measured, within 15 % in all.
+// 23.3, 192 : 176 / 2 19.0, 256 : 176 / 2 19.0; 512 x 4096 x 4096 128 : 128 / 2 24.6, 192 : 128 / 1 24.8, 256 : 256 / 2 21.1.  What the estimates
+// pick, the tiles of gemm_bias_act included, was within 5 % of the best in 39 of 45 sizes measured, 16 % from it at worst (513 x 512 x 1024).
 static double fr_cost(int tok, int block, int64_t tiles, int64_t blocks, int64_t chunks, int s) {
     const bool wide = tok > 128, pair = tok == kFrPairTok;
     if (pair) tiles = (tiles + 1) / 2 * 2;

@@ -20,6 +20,9 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 OUT = os.path.join(HERE, "_ref")
 LIB = os.path.join(OUT, "libref_tile_scale.so")
+# the files of the reference tree that are read
+SOURCES = ("csrc/include/primus_turbo/quantization.h", "csrc/kernels/quantization/quantization_mxfp8.cu",
+           "csrc/kernels/quantization/quantization_mxfp4.cu", "csrc/include/primus_turbo/device/utils.cuh")
 
 SHIM_HEAD = r'''
 #include <cstdint>
@@ -63,17 +66,18 @@ def _slice(text, start_pat, end_pat, what):
 
 
 def build(ref_root="/root/reference"):
-    """Returns the library path, or None when the reference tree is absent (the GPU box: prebuilt files travel)."""
-    if not os.path.isdir(ref_root):
+    """Returns the library path, or None when the reference tree is absent (no directory, or one without the sources; prebuilt
+    files travel)."""
+    if not os.path.isfile(os.path.join(ref_root, SOURCES[0])):
         return LIB if os.path.exists(LIB) else None
     rd = lambda rel: open(os.path.join(ref_root, rel)).read()
-    consts = _slice(rd("csrc/include/primus_turbo/quantization.h"), r"constexpr int FP32_MANTISSA_BITS", r"constexpr int E8M0_EXPONENT_BIAS = 127;",
+    consts = _slice(rd(SOURCES[0]), r"constexpr int FP32_MANTISSA_BITS", r"constexpr int E8M0_EXPONENT_BIAS = 127;",
                     "the format constants")
-    fn8 = _slice(rd("csrc/kernels/quantization/quantization_mxfp8.cu"), r"template <typename DType>\s*__device__ __forceinline__ void compute_tile_scale",
+    fn8 = _slice(rd(SOURCES[1]), r"template <typename DType>\s*__device__ __forceinline__ void compute_tile_scale",
                  r"\n}\n", "compute_tile_scale (fp8)")
-    fn4 = _slice(rd("csrc/kernels/quantization/quantization_mxfp4.cu"), r"__device__ __forceinline__ void compute_tile_scale", r"\n}\n",
+    fn4 = _slice(rd(SOURCES[2]), r"__device__ __forceinline__ void compute_tile_scale", r"\n}\n",
                  "compute_tile_scale (fp4)")
-    e8 = _slice(rd("csrc/include/primus_turbo/device/utils.cuh"), r"PRIMUS_TURBO_DEVICE float e8m0_to_scale", r"\n}\n", "e8m0_to_scale")
+    e8 = _slice(rd(SOURCES[3]), r"PRIMUS_TURBO_DEVICE float e8m0_to_scale", r"\n}\n", "e8m0_to_scale")
     os.makedirs(OUT, exist_ok=True)
     src = os.path.join(OUT, "ref_tile_scale.cpp")
     with open(src, "w") as f:

@@ -149,7 +149,8 @@ def moe_few_tokens_impl(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tens
 
 @moe_few_tokens_impl.register_fake
 def _(x, gate_up, down, topk_indices, topk_probs, act_type):
-    return torch.empty_like(x)
+    _few.check_moe_few_tokens(x, gate_up, down, topk_indices, topk_probs, act_type)
+    return x.new_empty(x.shape)
 
 
 # ------------------------------------------------------------------------------------------------ grouped GEMMs

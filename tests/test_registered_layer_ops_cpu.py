@@ -1,0 +1,51 @@
+"""torch.ops.primus_turbo forms of the operators around a decoder layer's products: they refuse what `ops` refuses.  Fake CUDA tensors
+reach the refusals on a machine without a GPU; the implementations make the same checks before anything is launched."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+bf16, f16, f32, i64 = torch.bfloat16, torch.float16, torch.float32, torch.int64
+
+
+def _e(*shape, dt=bf16):
+    return torch.empty(shape, dtype=dt, device="cuda")
+
+
+def _op(name):
+    import primus_turbo.pytorch  # noqa: F401
+    return getattr(torch.ops.primus_turbo, name)
+
+
+def _refused(call, match):
+    with FakeTensorMode(), pytest.raises(AssertionError, match=match):
+        call()
+
+
+# ------------------------------------------------------------------------------------------------ moe_few_tokens
+def _moe(**change):
+    a = dict(x=_e(3, 64), gate_up=_e(4, 32, 64), down=_e(4, 64, 16), topk_indices=_e(3, 2, dt=i64), topk_probs=_e(3, 2, dt=f32), act_type="silu")
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change,match", [
+    (lambda: dict(act_type="relu"), "Unsupported act_type"),
+    (lambda: dict(x=_e(3, 72)), "do not fit"),
+    (lambda: dict(gate_up=_e(4, 16, 64)), "do not fit"),
+    (lambda: dict(gate_up=_e(3, 32, 64)), "do not fit"),
+    (lambda: dict(x=_e(3, 64, dt=f16)), "bf16 or fp16"),
+    (lambda: dict(topk_indices=_e(2, 2, dt=i64)), "must be .T, K."),
+    (lambda: dict(topk_probs=_e(3, 1, dt=f32)), "must be .T, K."),
+    (lambda: dict(topk_probs=_e(3, 2)), "float32"),
+    (lambda: dict(topk_indices=_e(3, 2, dt=torch.int16)), "int32 or int64"),
+    (lambda: dict(topk_probs=torch.empty(3, 2, device="cpu")), "one device"),
+])
+def test_moe_few_tokens_refuses(change, match):
+    from primus_turbo.pytorch.kernels.moe.few_tokens_impl import moe_few_tokens_impl
+    _refused(lambda: _op("moe_few_tokens_impl")(**_moe(**change())), match)
+    _refused(lambda: moe_few_tokens_impl(*_moe(**change()).values()), match)
+
+
+def test_moe_few_tokens_output_is_contiguous():
+    with FakeTensorMode():
+        assert _op("moe_few_tokens_impl")(**_moe(x=_e(64, 3).t())).is_contiguous()

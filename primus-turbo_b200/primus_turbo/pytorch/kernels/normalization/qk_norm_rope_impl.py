@@ -1,5 +1,6 @@
-"""Per-head RMS norm and position rotation of queries and keys over the C ABI.  Tensors come as [S, heads, D] or [B, S, heads, D]
-views with a contiguous last dimension; the kernels take their strides."""
+"""Per-head RMS norm and position rotation of queries and keys over the C ABI.  qk_norm_rope_args checks a call's tensors and lays them
+out as the two functions below it take them: [S, heads, D] or [B, S, heads, D] views with a contiguous last dimension, whose strides the
+kernels read, and contiguous gains, tables and positions."""
 import struct
 from typing import Optional, Tuple
 
@@ -17,6 +18,41 @@ def _strides(t):
 
 def _extents(q):
     return q.shape[:2] if q.dim() == 4 else (1, q.shape[0])
+
+
+def _as_heads(x):
+    """x [..., tokens, heads, D] with three or four dimensions and a contiguous last one, without a copy where its strides allow it."""
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+    return x if x.dim() <= 4 else x.flatten(0, -4)
+
+
+def qk_norm_rope_args(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor, k_gamma: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                      positions: Optional[torch.Tensor]) -> Tuple[Optional[torch.Tensor], ...]:
+    """The same seven tensors as qk_norm_rope_fwd_impl and qk_norm_rope_bwd_impl take them; refuses what does not fit together."""
+    index, dtype, D = q.get_device(), q.dtype, q.shape[-1]
+    for t in (q, k, q_gamma, k_gamma, cos, sin) if positions is None else (q, k, q_gamma, k_gamma, cos, sin, positions):
+        if t.get_device() != index or index < 0:
+            if not t.is_cuda:
+                raise RuntimeError("primus_turbo (B200) operators take CUDA tensors only; there is no CPU path")
+            raise AssertionError("qk_norm_rope: all tensors must be on one device")
+    assert dtype in (torch.bfloat16, torch.float16, torch.float32), f"qk_norm_rope: unsupported dtype {dtype}"
+    assert k.dtype == dtype == q_gamma.dtype == k_gamma.dtype, "qk_norm_rope: q, k and the gains must have one dtype"
+    assert q.dim() >= 3, f"qk_norm_rope: q must be [..., tokens, heads, D], got {tuple(q.shape)}"
+    lead = q.shape[:-2]
+    assert k.dim() == q.dim() and k.shape[:-2] == lead and k.shape[-1] == D, \
+        f"qk_norm_rope: q {tuple(q.shape)} and k {tuple(k.shape)} must agree but in their heads"
+    assert q_gamma.shape == (D,) and k_gamma.shape == (D,), "qk_norm_rope: the gains must be [D]"
+    assert cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape, \
+        "qk_norm_rope: cos and sin must be float32 [positions, R / 2]"
+    assert 2 * cos.shape[1] <= D, f"qk_norm_rope: the tables rotate {2 * cos.shape[1]} elements of heads of {D}"
+    if positions is not None:
+        assert positions.dtype in (torch.int32, torch.int64), "qk_norm_rope: positions must be int32 or int64"
+        assert positions.shape == lead, f"qk_norm_rope: positions {tuple(positions.shape)} must be [..., tokens] {tuple(q.shape[:-2])}"
+        positions = positions.contiguous()
+    else:
+        assert q.shape[-3] <= cos.shape[0], f"qk_norm_rope: {q.shape[-3]} tokens need as many rows of cos / sin, got {cos.shape[0]}"
+    return _as_heads(q), _as_heads(k), q_gamma.contiguous(), k_gamma.contiguous(), cos.contiguous(), sin.contiguous(), positions
 
 
 def qk_norm_rope_fwd_impl(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor, k_gamma: torch.Tensor, cos: torch.Tensor,

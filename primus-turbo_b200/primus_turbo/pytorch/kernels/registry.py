@@ -133,11 +133,14 @@ def _(a, b, trans_b, bias, activation, residual, out_dtype):
 def qk_norm_rope_fwd_impl(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor, k_gamma: torch.Tensor, cos: torch.Tensor,
                           sin: torch.Tensor, positions: Optional[torch.Tensor], eps: float, interleaved: bool,
                           zero_centered: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    return _qk.qk_norm_rope_fwd_impl(q, k, q_gamma, k_gamma, cos, sin, positions, eps, interleaved, zero_centered)
+    args = _qk.qk_norm_rope_args(q, k, q_gamma, k_gamma, cos, sin, positions)
+    q_out, k_out = _qk.qk_norm_rope_fwd_impl(*args, eps, interleaved, zero_centered)
+    return (q_out, k_out) if q.dim() <= 4 else (q_out.view(q.shape), k_out.view(k.shape))
 
 
 @qk_norm_rope_fwd_impl.register_fake
 def _(q, k, q_gamma, k_gamma, cos, sin, positions, eps, interleaved, zero_centered):
+    _qk.qk_norm_rope_args(q, k, q_gamma, k_gamma, cos, sin, positions)
     return torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
 
 

@@ -5,7 +5,7 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from ..kernels.normalization.qk_norm_rope_impl import qk_norm_rope_bwd_impl, qk_norm_rope_fwd_impl
+from ..kernels.normalization.qk_norm_rope_impl import qk_norm_rope_args, qk_norm_rope_bwd_impl, qk_norm_rope_fwd_impl
 
 from ..kernels.normalization.rmsnorm_impl import (
     rmsnorm_bwd_impl,
@@ -79,13 +79,6 @@ class _QKNormRopeFunction(torch.autograd.Function):
         return (*qk_norm_rope_bwd_impl(dq, dk, q, k, q_gamma, k_gamma, cos, sin, positions, *ctx.options),) + (None,) * 6
 
 
-def _as_heads(x):
-    """x [..., tokens, heads, D] with three or four dimensions and a contiguous last one, without a copy where its strides allow it."""
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
-        x = x.contiguous()
-    return x if x.dim() <= 4 else x.flatten(0, -4)
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor, k_gamma: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                  positions: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
                  zero_centered: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -97,30 +90,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor, k_gamm
     (i, i + R / 2), or (2 i, 2 i + 1) when interleaved, by cos / sin of the token's position; elements from R on pass through.
     positions: int32 / int64 of the shape [..., tokens]; None: 0, 1, ... along the token dimension.  A position outside of
     [0, P) gives zeros for its token and an error at a following call.  Differentiable in q, k and the gains."""
-    index, dtype, D = q.get_device(), q.dtype, q.shape[-1]
-    for t in (q, k, q_gamma, k_gamma, cos, sin) if positions is None else (q, k, q_gamma, k_gamma, cos, sin, positions):
-        if t.get_device() != index or index < 0:
-            if not t.is_cuda:
-                raise RuntimeError("primus_turbo (B200) operators take CUDA tensors only; there is no CPU path")
-            raise AssertionError("qk_norm_rope: all tensors must be on one device")
-    assert dtype in (torch.bfloat16, torch.float16, torch.float32), f"qk_norm_rope: unsupported dtype {dtype}"
-    assert k.dtype == dtype == q_gamma.dtype == k_gamma.dtype, "qk_norm_rope: q, k and the gains must have one dtype"
-    assert q.dim() >= 3, f"qk_norm_rope: q must be [..., tokens, heads, D], got {tuple(q.shape)}"
-    lead = q.shape[:-2]
-    assert k.dim() == q.dim() and k.shape[:-2] == lead and k.shape[-1] == D, \
-        f"qk_norm_rope: q {tuple(q.shape)} and k {tuple(k.shape)} must agree but in their heads"
-    assert q_gamma.shape == (D,) and k_gamma.shape == (D,), "qk_norm_rope: the gains must be [D]"
-    assert cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape, \
-        "qk_norm_rope: cos and sin must be float32 [positions, R / 2]"
-    assert 2 * cos.shape[1] <= D, f"qk_norm_rope: the tables rotate {2 * cos.shape[1]} elements of heads of {D}"
-    if positions is not None:
-        assert positions.dtype in (torch.int32, torch.int64), "qk_norm_rope: positions must be int32 or int64"
-        assert positions.shape == lead, f"qk_norm_rope: positions {tuple(positions.shape)} must be [..., tokens] {tuple(q.shape[:-2])}"
-        positions = positions.contiguous()
-    else:
-        assert q.shape[-3] <= cos.shape[0], f"qk_norm_rope: {q.shape[-3]} tokens need as many rows of cos / sin, got {cos.shape[0]}"
-    args = (_as_heads(q), _as_heads(k), q_gamma.contiguous(), k_gamma.contiguous(), cos.contiguous(), sin.contiguous(), positions, eps,
-            interleaved, zero_centered)
+    args = (*qk_norm_rope_args(q, k, q_gamma, k_gamma, cos, sin, positions), eps, interleaved, zero_centered)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_gamma.requires_grad or k_gamma.requires_grad or
                                     cos.requires_grad or sin.requires_grad):
         assert not (cos.requires_grad or sin.requires_grad), "qk_norm_rope: the tables are not differentiated"

@@ -49,3 +49,30 @@ def test_moe_few_tokens_refuses(change, match):
 def test_moe_few_tokens_output_is_contiguous():
     with FakeTensorMode():
         assert _op("moe_few_tokens_impl")(**_moe(x=_e(64, 3).t())).is_contiguous()
+
+
+# ------------------------------------------------------------------------------------------------ qk_norm_rope
+def _qk(**change):
+    a = dict(q=_e(5, 4, 64), k=_e(5, 2, 64), q_gamma=_e(64), k_gamma=_e(64), cos=_e(16, 32, dt=f32), sin=_e(16, 32, dt=f32), positions=None,
+             eps=1e-6, interleaved=False, zero_centered=False)
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change,match", [
+    (lambda: dict(k=_e(4, 2, 64)), "agree but in their heads"),
+    (lambda: dict(k=_e(5, 2, 32)), "agree but in their heads"),
+    (lambda: dict(k_gamma=_e(32)), "gains must be"),
+    (lambda: dict(q_gamma=_e(64, dt=f32)), "one dtype"),
+    (lambda: dict(cos=_e(16, 32)), "float32"),
+    (lambda: dict(sin=_e(8, 32, dt=f32)), "float32"),
+    (lambda: dict(cos=_e(16, 40, dt=f32), sin=_e(16, 40, dt=f32)), "tables rotate"),
+    (lambda: dict(cos=_e(4, 32, dt=f32), sin=_e(4, 32, dt=f32)), "as many rows"),
+    (lambda: dict(positions=_e(4, dt=i64)), "must be"),
+    (lambda: dict(positions=_e(5, dt=torch.int16)), "int32 or int64"),
+    (lambda: dict(q=_e(5, 64), k=_e(5, 64)), "heads, D"),
+    (lambda: dict(q_gamma=torch.empty(64, dtype=bf16, device="cpu")), "CUDA tensors only"),
+])
+def test_qk_norm_rope_refuses(change, match):
+    with FakeTensorMode(), pytest.raises((AssertionError, RuntimeError), match=match):
+        _op("qk_norm_rope_fwd_impl")(**_qk(**change()))

@@ -29,3 +29,21 @@ def test_moe_few_tokens_with_strides():
                  (x, gu, dn, ids, wide[:, ::2]), (_turned(x), _turned(gu, 1, 2), _turned(dn, 0, 2), _turned(ids).int(), _turned(p))):
         got = torch.ops.primus_turbo.moe_few_tokens_impl(*args, "silu")
         assert got.is_contiguous() and torch.equal(got, want) and torch.equal(ops.moe_few_tokens(*args), want)
+
+
+def test_qk_norm_rope_with_strides_and_more_dimensions():
+    from primus_turbo.pytorch import ops
+    T, Hq, Hk, D, R = 6, 4, 2, 32, 24
+    q, k, qg, kg = _rand((T, Hq, D), 1), _rand((T, Hk, D), 2), _rand((D,), 3), _rand((D,), 4)
+    cos, sin = _rand((16, R // 2), 5, dt=torch.float32), _rand((16, R // 2), 6, dt=torch.float32)
+    pos = torch.tensor([3, 0, 15, 2, 2, 9], device="cuda")
+    reg = torch.ops.primus_turbo.qk_norm_rope_fwd_impl
+    want = ops.qk_norm_rope(q, k, qg, kg, cos, sin, positions=pos)
+    gap = lambda t: torch.stack([t, torch.zeros_like(t)], -1).flatten(-2)[..., ::2]      # the values of t, every second element
+    for args in ((_turned(q, 1, 2), k, qg, kg, cos, sin, pos), (q, _turned(k, 0, 2), qg, kg, cos, sin, pos), (q, k, gap(qg), kg, cos, sin, pos),
+                 (q, k, qg, gap(kg), _turned(cos), sin, pos), (q, k, qg, kg, cos, gap(sin), gap(pos)), (gap(q), gap(k), qg, kg, cos, sin, pos.int())):
+        for got in (reg(*args, 1e-6, False, False), ops.qk_norm_rope(*args)):
+            assert all(torch.equal(g, w) and g.is_contiguous() for g, w in zip(got, want))
+    many = lambda t: t.view(1, 3, 1, 2, *t.shape[1:])
+    got = reg(many(q), many(k), qg, kg, cos, sin, pos.view(1, 3, 1, 2), 1e-6, False, False)
+    assert all(g.shape == many(t).shape and torch.equal(g, many(w)) for g, t, w in zip(got, (q, k), want))

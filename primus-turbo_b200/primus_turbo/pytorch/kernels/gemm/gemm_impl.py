@@ -82,6 +82,26 @@ def gemm_accum_impl(a: torch.Tensor, trans_a: bool, b: torch.Tensor, trans_b: bo
 EPILOGUE_ACTS = {"silu": 0, "gelu": 1, None: 2, "relu": 3, "gelu_tanh": 4}
 
 
+def check_gemm_bias_act(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Optional[torch.Tensor], act: Optional[str],
+                        residual: Optional[torch.Tensor], out_dtype: torch.dtype) -> None:
+    """Refuses what gemm_bias_act_impl, which trusts its arguments but for their strides, does not take."""
+    assert a.dim() == 2 and b.dim() == 2, "Only 2D GEMM is supported"
+    dtype, index, (M, K) = a.dtype, a.get_device(), a.shape
+    assert b.dtype == dtype and dtype in (torch.bfloat16, torch.float16), "a and b must both be bf16 or fp16"
+    assert act in EPILOGUE_ACTS, f"Unsupported activation: {act}. Supported: {list(EPILOGUE_ACTS)}"
+    N, Kb = b.shape if trans_b else b.shape[::-1]
+    assert Kb == K, f"contraction mismatch: {tuple(a.shape)} vs {tuple(b.shape)} (trans_b={trans_b})"
+    assert K > 0, "gemm_bias_act: the contraction must not be empty"
+    assert out_dtype in (torch.bfloat16, torch.float16, torch.float32), f"gemm_bias_act: unsupported out_dtype {out_dtype}"
+    assert b.get_device() == index, "gemm_bias_act: all tensors must be on one device"
+    if bias is not None:
+        assert bias.shape == (N,) and bias.dtype in (dtype, torch.float32), f"gemm_bias_act: bias must be [{N}] in a's dtype or float32"
+        assert bias.get_device() == index, "gemm_bias_act: all tensors must be on one device"
+    if residual is not None:
+        assert residual.shape == (M, N) and residual.dtype == out_dtype, f"gemm_bias_act: residual must be [{M}, {N}] in {out_dtype}"
+        assert residual.get_device() == index, "gemm_bias_act: all tensors must be on one device"
+
+
 def gemm_bias_act_impl(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Optional[torch.Tensor], act: Optional[str],
                        residual: Optional[torch.Tensor], out_dtype: torch.dtype, want_z: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(act(a . op(b) + bias) + residual, the pre-activation in a's type or None) in one kernel."""

@@ -117,15 +117,17 @@ def _(a, trans_a, b, trans_b, out_dtype, trans_c, out, default_backend):
 
 
 # ------------------------------------------------------------------------------------------------ around a decoder layer's products
-# (no counterpart in the reference; `ops` checks the arguments before it calls the same functions)
+# (no counterpart in the reference; the checks are those of `ops`)
 @_op("primus_turbo::gemm_bias_act_impl", mutates_args=(), device_types="cuda")
 def gemm_bias_act_impl(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Optional[torch.Tensor], activation: Optional[str],
                        residual: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    _g16.check_gemm_bias_act(a, b, trans_b, bias, activation, residual, out_dtype)
     return _g16.gemm_bias_act_impl(a, b, trans_b, bias, activation, residual, out_dtype, False)[0]
 
 
 @gemm_bias_act_impl.register_fake
 def _(a, b, trans_b, bias, activation, residual, out_dtype):
+    _g16.check_gemm_bias_act(a, b, trans_b, bias, activation, residual, out_dtype)
     return _out2d(a, b, False, trans_b, False, out_dtype)
 
 

@@ -9,10 +9,10 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ..kernels.gemm.gemm_impl import (
-    EPILOGUE_ACTS,
     act_bias_bwd_impl,
     bias_act_dgrad_impl,
     bias_act_wgrad_impl,
+    check_gemm_bias_act,
     gemm_accum_impl,
     gemm_bias_act_impl,
     gemm_impl,
@@ -94,25 +94,9 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     (a's dtype by default).  Few rows (a decoding batch) run on a kernel that streams the weight over all SMs.  A contraction that is
     not a multiple of 8 is padded first (copies of a and b), as in gemm.  Differentiable in
     a, b, bias and residual; the pre-activation is kept in a's dtype for the backward when an activation needs it."""
-    assert a.dim() == 2 and b.dim() == 2, "Only 2D GEMM is supported"
-    dtype, index, (M, K) = a.dtype, a.get_device(), a.shape
-    assert b.dtype == dtype and dtype in (torch.bfloat16, torch.float16), "a and b must both be bf16 or fp16"
-    assert activation in EPILOGUE_ACTS, f"Unsupported activation: {activation}. Supported: {list(EPILOGUE_ACTS)}"
-    N, Kb = b.shape if trans_b else b.shape[::-1]
-    assert Kb == K, f"contraction mismatch: {tuple(a.shape)} vs {tuple(b.shape)} (trans_b={trans_b})"
-    assert K > 0, "gemm_bias_act: the contraction must not be empty"
-    out_dtype = dtype if out_dtype is None else out_dtype
-    assert out_dtype in (torch.bfloat16, torch.float16, torch.float32), f"gemm_bias_act: unsupported out_dtype {out_dtype}"
-    assert b.get_device() == index, "gemm_bias_act: all tensors must be on one device"
-    grad = a.requires_grad or b.requires_grad
-    if bias is not None:
-        assert bias.shape == (N,) and bias.dtype in (dtype, torch.float32), f"gemm_bias_act: bias must be [{N}] in a's dtype or float32"
-        assert bias.get_device() == index, "gemm_bias_act: all tensors must be on one device"
-        grad = grad or bias.requires_grad
-    if residual is not None:
-        assert residual.shape == (M, N) and residual.dtype == out_dtype, f"gemm_bias_act: residual must be [{M}, {N}] in {out_dtype}"
-        assert residual.get_device() == index, "gemm_bias_act: all tensors must be on one device"
-        grad = grad or residual.requires_grad
+    out_dtype = a.dtype if out_dtype is None else out_dtype
+    check_gemm_bias_act(a, b, trans_b, bias, activation, residual, out_dtype)
+    grad = a.requires_grad or b.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad)
     if grad and torch.is_grad_enabled():
         return GemmBiasActFunction.apply(a, b, bias, residual, trans_b, activation, out_dtype, fuse_bgrad_accum_pattern)
     return gemm_bias_act_impl(a, b, trans_b, bias, activation, residual, out_dtype, False)[0]

@@ -76,3 +76,23 @@ def _qk(**change):
 def test_qk_norm_rope_refuses(change, match):
     with FakeTensorMode(), pytest.raises((AssertionError, RuntimeError), match=match):
         _op("qk_norm_rope_fwd_impl")(**_qk(**change()))
+
+
+# ------------------------------------------------------------------------------------------------ gemm_bias_act
+@pytest.mark.parametrize("change,match", [
+    (lambda: dict(a=_e(4, 63)), "contraction mismatch"),
+    (lambda: dict(trans_b=False), "contraction mismatch"),
+    (lambda: dict(a=_e(2, 4, 64)), "Only 2D"),
+    (lambda: dict(a=_e(4, 64, dt=f16)), "both be bf16 or fp16"),
+    (lambda: dict(a=_e(4, 0), b=_e(32, 0)), "must not be empty"),
+    (lambda: dict(activation="swish"), "Unsupported activation"),
+    (lambda: dict(bias=_e(31)), "bias must be"),
+    (lambda: dict(bias=_e(32, dt=f16)), "bias must be"),
+    (lambda: dict(residual=_e(4, 31)), "residual must be"),
+    (lambda: dict(residual=_e(4, 32), out_dtype=f32), "residual must be"),
+    (lambda: dict(out_dtype=torch.float64), "unsupported out_dtype"),
+    (lambda: dict(bias=torch.empty(32, dtype=bf16, device="cpu")), "one device"),
+])
+def test_gemm_bias_act_refuses(change, match):
+    _refused(lambda: _op("gemm_bias_act_impl")(**{**dict(a=_e(4, 64), b=_e(32, 64), trans_b=True, bias=None, activation=None, residual=None, out_dtype=bf16),
+                                                  **change()}), match)

@@ -47,3 +47,24 @@ def test_qk_norm_rope_with_strides_and_more_dimensions():
     many = lambda t: t.view(1, 3, 1, 2, *t.shape[1:])
     got = reg(many(q), many(k), qg, kg, cos, sin, pos.view(1, 3, 1, 2), 1e-6, False, False)
     assert all(g.shape == many(t).shape and torch.equal(g, many(w)) for g, t, w in zip(got, (q, k), want))
+
+
+def test_gemm_bias_act_with_strides():
+    from primus_turbo.pytorch import ops
+    M, N, K = 9, 40, 24
+    a, b, bias, res = _rand((M, K), 1), _rand((N, K), 2), _rand((2 * N,), 3)[::2], _rand((N, M), 4).t()
+    want = ops.gemm_bias_act(a, b, bias.contiguous(), "silu", res.contiguous(), trans_b=True)
+    for args in ((_turned(a), b), (a, _turned(b)), (_turned(a), _turned(b))):
+        assert torch.equal(torch.ops.primus_turbo.gemm_bias_act_impl(*args, True, bias, "silu", res, BF), want)
+
+
+def test_a_misfit_is_refused_before_any_launch():
+    t = torch.ops.primus_turbo
+    a, b = _rand((4, 64), 1), _rand((32, 64), 2)
+    with pytest.raises(AssertionError, match="bias must be"):
+        t.gemm_bias_act_impl(a, b, True, b[0, :16], None, None, BF)
+    with pytest.raises(AssertionError, match="gains must be"):
+        t.qk_norm_rope_fwd_impl(a.view(4, 1, 64), a.view(4, 1, 64), b[0], b[0, :32], torch.ones(4, 32, device="cuda"), torch.ones(4, 32, device="cuda"), None, 1e-6,
+                                False, False)
+    with pytest.raises(AssertionError, match="must be float32"):
+        t.moe_few_tokens_impl(a, b.view(2, 16, 64), _rand((2, 64, 8), 3), torch.zeros(4, 1, dtype=torch.int64, device="cuda"), a[:, :1], "silu")

@@ -627,7 +627,7 @@ static int qk_check(const QkArgs &a, int dtype, int64_t B) {
                "qk_norm_rope: the head size must lie in [1, %d] and the rotated part be even and no larger (got %d, %d)", kQkMaxD, a.D, a.R);
     PT_REQUIRE(a.T < (1ll << 31) && a.T * (a.heads[0] + (int64_t) a.heads[1]) < (1ll << 31), "qk_norm_rope: tokens x heads exceed 32-bit indices");
     PT_REQUIRE(a.pos_bytes == 0 || a.pos_bytes == 4 || a.pos_bytes == 8, "qk_norm_rope: positions must be int32 or int64");
-    PT_REQUIRE((a.pos_bytes == 0) == (a.positions == nullptr), "qk_norm_rope: positions and their size go together");
+    PT_REQUIRE(a.T == 0 || (a.pos_bytes == 0) == (a.positions == nullptr), "qk_norm_rope: positions and their size go together");   // an empty tensor is a null pointer
     for (int r = 0; r < 2; ++r)
         PT_REQUIRE(a.T == 0 || a.heads[r] == 0 || (a.x[r] && a.out[r] && a.gamma[r]), "qk_norm_rope: null pointer");
     PT_REQUIRE(a.T == 0 || a.R == 0 || (a.cos && a.sin), "qk_norm_rope: null table");

@@ -1,0 +1,19 @@
+"""Edges of the operators around a decoder layer's products that need no launch: they reach the C ABI or the Python checks without a GPU."""
+import ctypes
+
+import pytest
+
+
+@pytest.mark.parametrize("pos_bytes", [0, 4, 8])
+@pytest.mark.parametrize("B,S", [(1, 0), (0, 5), (3, 0)])
+def test_qk_norm_rope_takes_no_tokens_with_positions(pos_bytes, B, S):
+    """An empty positions tensor is a null pointer of a known element size."""
+    from primus_turbo import _clib
+    lib = _clib.load()
+    st = (ctypes.c_int64 * 3)(0, 0, 0)
+    assert lib.pt_qk_norm_rope_fwd(None, None, 0, None, None, None, None, None, pos_bytes, B, S, 8, 2, 1, 64, 64, st, st, 1e-6, 0, 0, None, None, None,
+                                   None) == 0, lib.pt_last_error()
+    # the backward goes on to its own buffers, which are missing here
+    rc = lib.pt_qk_norm_rope_bwd(None, None, None, None, 0, None, None, None, None, None, pos_bytes, B, S, 8, 2, 1, 64, 64, st, st, st, st, 1e-6, 0, 0, None,
+                                 None, None, None, None, 0, None, None)
+    assert rc == -1 and b"dgamma buffers" in lib.pt_last_error()

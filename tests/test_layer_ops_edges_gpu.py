@@ -1,0 +1,31 @@
+"""Edges of the operators around a decoder layer's products: empty inputs, values at the ends of the types' ranges, tails of the
+activations, sizes at which a block of tokens holds next to nothing."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+U = 2.0 ** -24
+
+
+def _rand(shape, seed, std=1.0, dt=BF):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.empty(shape, dtype=torch.float32, device="cuda").normal_(0, std, generator=g).to(dt)
+
+
+# ------------------------------------------------------------------------------------------------ qk_norm_rope
+@pytest.mark.parametrize("idt", [None, torch.int32, torch.int64])
+@pytest.mark.parametrize("lead", [(0,), (2, 0), (0, 3)])
+def test_qk_norm_rope_without_tokens(idt, lead):
+    """Empty outputs and gradients of zero for the gains, with positions and without."""
+    from primus_turbo.pytorch.ops import qk_norm_rope
+    q, k = (torch.empty((*lead, h, 64), dtype=BF, device="cuda", requires_grad=True) for h in (4, 2))
+    qg, kg = _rand((64,), 1).requires_grad_(), _rand((64,), 2).requires_grad_()
+    cos = sin = torch.ones(8, 32, device="cuda")
+    pos = None if idt is None else torch.empty(lead, dtype=idt, device="cuda")
+    q_out, k_out = qk_norm_rope(q, k, qg, kg, cos, sin, positions=pos)
+    assert q_out.shape == q.shape and k_out.shape == k.shape
+    dq, dk, dqg, dkg = torch.autograd.grad([q_out, k_out], [q, k, qg, kg], [torch.empty_like(q_out), torch.empty_like(k_out)])
+    assert dq.shape == q.shape and dk.shape == k.shape and not dqg.any() and not dkg.any()

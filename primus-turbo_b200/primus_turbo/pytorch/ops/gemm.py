@@ -17,7 +17,7 @@ from ..kernels.gemm.gemm_impl import (
     gemm_bias_act_impl,
     gemm_impl,
 )
-from .utils import _get_dummy_wgrad, _setup_fused_grad_accum
+from .utils import _forward_ad_active, _get_dummy_wgrad, _setup_fused_grad_accum
 
 __all__ = ["gemm", "gemm_bias_act"]
 
@@ -97,6 +97,6 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     out_dtype = a.dtype if out_dtype is None else out_dtype
     check_gemm_bias_act(a, b, trans_b, bias, activation, residual, out_dtype)
     grad = a.requires_grad or b.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad)
-    if grad and torch.is_grad_enabled():
+    if (grad and torch.is_grad_enabled()) or _forward_ad_active():
         return GemmBiasActFunction.apply(a, b, bias, residual, trans_b, activation, out_dtype, fuse_bgrad_accum_pattern)
     return gemm_bias_act_impl(a, b, trans_b, bias, activation, residual, out_dtype, False)[0]

@@ -6,8 +6,10 @@ prompts.  For a decoding batch those steps cost more than reading the weights; h
 experts' weights once.
 """
 import torch
+from torch.autograd import forward_ad
 
 from ...kernels.moe.few_tokens_impl import moe_few_tokens_impl
+from ..utils import _forward_ad_active
 
 __all__ = ["moe_few_tokens"]
 
@@ -24,4 +26,6 @@ def moe_few_tokens(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, t
     (erf form)."""
     if torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad or down.requires_grad or topk_probs.requires_grad):
         raise RuntimeError("moe_few_tokens has no backward: call it under torch.no_grad(), or train through token_permute and grouped_gemm")
+    if _forward_ad_active() and any(forward_ad.unpack_dual(t).tangent is not None for t in (x, gate_up, down, topk_probs)):
+        raise RuntimeError("moe_few_tokens has no forward-mode derivative either")
     return moe_few_tokens_impl(x, gate_up, down, topk_indices, topk_probs, act_type)

@@ -13,6 +13,7 @@ from ..kernels.normalization.rmsnorm_impl import (
     rmsnorm_fwd_impl,
     rmsnorm_fwd_residual_impl,
 )
+from .utils import _forward_ad_active
 
 __all__ = ["rmsnorm", "rmsnorm_residual", "qk_norm_rope"]
 
@@ -91,8 +92,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor, k_gamm
     positions: int32 / int64 of the shape [..., tokens]; None: 0, 1, ... along the token dimension.  A position outside of
     [0, P) gives zeros for its token and an error at a following call.  Differentiable in q, k and the gains."""
     args = (*qk_norm_rope_args(q, k, q_gamma, k_gamma, cos, sin, positions), eps, interleaved, zero_centered)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_gamma.requires_grad or k_gamma.requires_grad or
-                                    cos.requires_grad or sin.requires_grad):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_gamma.requires_grad or k_gamma.requires_grad or
+                                     cos.requires_grad or sin.requires_grad)) or _forward_ad_active():
         assert not (cos.requires_grad or sin.requires_grad), "qk_norm_rope: the tables are not differentiated"
         q_out, k_out = _QKNormRopeFunction.apply(*args)
     else:

@@ -2,6 +2,7 @@
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from ..core.low_precision import Format, float8_e4m3, float8_e5m2
 
@@ -28,6 +29,12 @@ def _setup_fused_grad_accum(b, fuse_bgrad_accum_pattern: Optional[str]):
         "b.main_grad must be a tensor with the same shape as b"
     b.grad_added_to_main_grad = True
     return True, b.main_grad
+
+
+def _forward_ad_active() -> bool:
+    """Whether tensors may carry forward-mode tangents, which requires_grad does not show.  An operator that calls its kernels directly
+    where no gradient is asked for goes through its autograd function then: it has no forward-mode formula and says so."""
+    return forward_ad._current_level >= 0
 
 
 _dummy_wgrads = {}

@@ -17,3 +17,16 @@ def test_qk_norm_rope_takes_no_tokens_with_positions(pos_bytes, B, S):
     rc = lib.pt_qk_norm_rope_bwd(None, None, None, None, 0, None, None, None, None, None, pos_bytes, B, S, 8, 2, 1, 64, 64, st, st, st, st, 1e-6, 0, 0, None,
                                  None, None, None, None, 0, None, None)
     assert rc == -1 and b"dgamma buffers" in lib.pt_last_error()
+
+
+def test_moe_few_tokens_refuses_a_tangent():
+    import torch
+    from torch.autograd import forward_ad
+    from primus_turbo.pytorch.ops import moe_few_tokens
+    z = lambda *s: torch.zeros(s, dtype=torch.bfloat16)
+    x, rest = z(3, 64), (z(4, 32, 64), z(4, 64, 16), torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2))
+    with forward_ad.dual_level(), torch.no_grad():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            moe_few_tokens(forward_ad.make_dual(x, x.clone()), *rest)
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            moe_few_tokens(x, *rest)

@@ -29,3 +29,26 @@ def test_qk_norm_rope_without_tokens(idt, lead):
     assert q_out.shape == q.shape and k_out.shape == k.shape
     dq, dk, dqg, dkg = torch.autograd.grad([q_out, k_out], [q, k, qg, kg], [torch.empty_like(q_out), torch.empty_like(k_out)])
     assert dq.shape == q.shape and dk.shape == k.shape and not dqg.any() and not dkg.any()
+
+
+# ------------------------------------------------------------------------------------------------ forward-mode derivatives
+@pytest.mark.parametrize("enabled", [True, False])
+def test_forward_mode_derivatives_are_refused(enabled):
+    """None of the operators has them: a tangent is refused, not dropped, under torch.no_grad too; without one nothing changes."""
+    from torch.autograd import forward_ad
+    from primus_turbo.pytorch import ops
+    x, w, h, g, t = _rand((4, 64), 1), _rand((16, 64), 2), _rand((4, 2, 32), 3), _rand((32,), 4), torch.ones(4, 16, device="cuda")
+    gu, dn, ids, p = _rand((2, 16, 64), 5), _rand((2, 64, 8), 6), torch.zeros(4, 1, dtype=torch.int64, device="cuda"), torch.ones(4, 1, device="cuda")
+    calls = [(lambda a, b: ops.gemm_bias_act(a, b, trans_b=True), (x, w)), (lambda a, b: ops.gemm_bias_act(x, w, bias=a, residual=b, trans_b=True), (w[:, 0], _rand((4, 16), 7))),
+             (lambda a, b: ops.qk_norm_rope(a, h, b, g, t, t)[0], (h, g)), (lambda a, b: ops.qk_norm_rope(h, a, g, g, b, t)[1], (h, t)),
+             (lambda a, b: ops.moe_few_tokens(a, gu, dn, ids, b), (x, p)), (lambda a, b: ops.moe_few_tokens(x, a, b, ids, p), (gu, dn))]
+    with torch.set_grad_enabled(enabled):
+        for call, args in calls:
+            want = call(*args)
+            with forward_ad.dual_level():
+                assert torch.equal(call(*args), want)
+                for i in range(2):
+                    dual = [forward_ad.make_dual(a, torch.ones_like(a)) if i == j else a for j, a in enumerate(args)]
+                    with pytest.raises((NotImplementedError, RuntimeError), match="forward"):
+                        call(*dual)
+            assert torch.equal(call(*args), want)

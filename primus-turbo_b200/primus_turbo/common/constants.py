@@ -20,4 +20,4 @@ ENV_PT_GEMM_PAIR = "PT_GEMM_PAIR"                    # 0: single-CTA GEMM tiles 
 ENV_PT_BW_GEMM_PAIR = "PT_BW_GEMM_PAIR"              # 1: CTA-pair form of the block-scaled GEMM
 ENV_PT_MX_QUANT_NO_TMA = "PT_MX_QUANT_NO_TMA"        # MX quantizer: one-CTA-per-tile kernel
 ENV_PT_MX_QUANT_NO_SPLIT = "PT_MX_QUANT_NO_SPLIT"    # MX quantizer: single-role consumer warps instead of the warp-split kernel
-ENV_PT_CHECK_STATUS = "PT_CHECK_STATUS"              # 1: read the kernels' status word after every GEMM call (synchronises)
+ENV_PT_CHECK_STATUS = "PT_CHECK_STATUS"              # 1: read the kernels' status words after every call that may report an error (synchronises)

@@ -89,8 +89,9 @@ def status_word(device) -> torch.Tensor:
 def mapped_status(device):
     """Address of the device's status word in pinned host memory, which the kernels of gemm_bias_act, qk_norm_rope and
     moe_few_tokens write directly (mapped, so the address is the device's too).  Raises if a kernel launched earlier has reported
-    an error into it: nothing is waited for, the error of a launch surfaces at a following call, or at check_status().  One host
-    load: a copy and an event per call, as poll_status makes, would cost an operator on one token as much as its kernel."""
+    an error into it: nothing is waited for, the error of a launch surfaces at a following call, at check_status(), or with
+    PT_CHECK_STATUS=1 at the launch itself (launched()).  One host load: a copy and an event per call, as poll_status makes, would cost
+    an operator on one token as much as its kernel."""
     w = _host_status.get(device.index)
     if w is None:
         t = torch.zeros(1, dtype=torch.int32).pin_memory()
@@ -101,6 +102,16 @@ def mapped_status(device):
     return w[2]
 
 
+# os.environ's own table: a look-up through os.environ takes 0.8 us, a twentieth of a whole call on one token
+_environ = getattr(os.environ, "_data", os.environb)
+
+
+def launched(device):
+    """After a launch that was given mapped_status: the synchronising check of PT_CHECK_STATUS=1, as poll_status makes it."""
+    if _environ.get(b"PT_CHECK_STATUS") == b"1" and not torch.cuda.is_current_stream_capturing():
+        check_status(device)
+
+
 def _raise(code):
     if code == PT_ERR_INVALID:
         raise RuntimeError("a kernel was given an index outside of its table (a position beyond the cos / sin rows); the rows of that "
@@ -109,7 +120,7 @@ def _raise(code):
 
 
 def check_status(device):
-    """Synchronises and raises if a kernel reported an expired wait since the last check."""
+    """Synchronises and raises if a kernel reported an expired wait or an index outside of its table since the last check."""
     s = status_word(device)
     code = int(s.item())
     if code != 0:

@@ -42,7 +42,9 @@ def _launch(a, a_mn, b, b_mn, out, beta, mapped_status=False):
     with nv.on_device(out.device):
         nv.check(nv.lib().pt_gemm_mn(nv.ptr(a), int(a_mn), nv.ptr(b), int(b_mn), nv.src_code(a.dtype), nv.ptr(out), nv.src_code(out.dtype), M, N, K,
                                      float(beta), st, nv.stream(out.device)), "gemm")
-    if not mapped_status:
+    if mapped_status:
+        nv.launched(out.device)
+    else:
         nv.poll_status(out.device)
     return out
 
@@ -126,6 +128,7 @@ def gemm_bias_act_impl(a: torch.Tensor, b: torch.Tensor, trans_b: bool, bias: Op
                                            0 if bias is None else nv.src_code(bias.dtype), nv.ptr(residual), out.data_ptr(),
                                            nv.src_code(out_dtype), nv.ptr(z), EPILOGUE_ACTS[act], M, N, (K + 7) // 8 * 8,
                                            nv.mapped_status(device), nv.stream(device)), "gemm_bias_act")
+    nv.launched(device)
     return out, z
 
 

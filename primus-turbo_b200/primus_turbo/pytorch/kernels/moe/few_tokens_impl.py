@@ -50,4 +50,5 @@ def moe_few_tokens_impl(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tens
         nv.check(lib.pt_moe_few_tokens(nv.ptr(x), nv.ptr(gate_up), nv.ptr(down), nv.src_code(x.dtype), nv.ptr(topk_indices),
                                        topk_indices.element_size(), nv.ptr(topk_probs), T, E, K, H, I, ACT_CODES[act], nv.ptr(scratch), nbytes,
                                        nv.ptr(out), nv.mapped_status(x.device), nv.stream(x.device)), "moe_few_tokens")
+    nv.launched(x.device)
     return out

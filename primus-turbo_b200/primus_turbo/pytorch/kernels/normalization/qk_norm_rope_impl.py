@@ -71,6 +71,7 @@ def qk_norm_rope_fwd_impl(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tenso
                                               cos.data_ptr(), sin.data_ptr(), nv.ptr(positions), 0 if positions is None else positions.element_size(),
                                               B, S, P, Hq, Hk, D, 2 * half, _strides(q), _strides(k), eps, interleaved, zero_centered,
                                               q_out.data_ptr(), k_out.data_ptr(), status, nv.stream(device)), "qk_norm_rope_fwd")
+    nv.launched(device)
     return q_out, k_out
 
 
@@ -96,4 +97,5 @@ def qk_norm_rope_bwd_impl(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
                                          _strides(dk), _strides(q), _strides(k), eps, interleaved, zero_centered, q_in.data_ptr(),
                                          k_in.data_ptr(), dqg.data_ptr(), dkg.data_ptr(), partial.data_ptr(), parts,
                                          status, nv.stream(device)), "qk_norm_rope_bwd")
+    nv.launched(device)
     return q_in, k_in, dqg, dkg

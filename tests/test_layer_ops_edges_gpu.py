@@ -52,3 +52,60 @@ def test_forward_mode_derivatives_are_refused(enabled):
                     with pytest.raises((NotImplementedError, RuntimeError), match="forward"):
                         call(*dual)
             assert torch.equal(call(*args), want)
+
+
+# ------------------------------------------------------------------------------------------------ PT_CHECK_STATUS
+def test_check_status_variable_raises_at_the_launch(monkeypatch):
+    """With PT_CHECK_STATUS=1 the call whose kernel reports raises, forward and backward; without it a following call does."""
+    from primus_turbo.pytorch import ops
+    from primus_turbo.pytorch.kernels import _native as nv
+    q, g, t = _rand((3, 2, 32), 1).requires_grad_(), _rand((32,), 2), torch.ones(4, 16, device="cuda")
+    good, bad = torch.tensor([0, 1, 3], device="cuda"), torch.tensor([0, 4, 1], device="cuda")
+    call = lambda pos: ops.qk_norm_rope(q, q, g, g, t, t, positions=pos)
+    nv.check_status(q.device)
+    monkeypatch.setenv("PT_CHECK_STATUS", "1")
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="outside of its table"):
+            call(bad)
+        call(good)
+    pos = good.clone()
+    y = call(pos)
+    pos.data.copy_(bad)
+    with pytest.raises(RuntimeError, match="outside of its table"):
+        torch.autograd.grad(y[0].float().sum(), q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):      # nothing waits inside a capture
+        call(good)
+    graph.replay()
+    monkeypatch.setenv("PT_CHECK_STATUS", "0")
+    call(bad)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="outside of its table"):
+        call(good)
+    nv.check_status(q.device)
+
+
+@pytest.mark.parametrize("name", ["gemm_bias_act", "moe_few_tokens", "backward"])
+def test_check_status_variable_reaches_every_operator(monkeypatch, name):
+    """A code that stands in the mapped word when the launch is over, put there by the host after the call has looked at it."""
+    from primus_turbo.pytorch import ops
+    from primus_turbo.pytorch.kernels import _native as nv
+    x, w = _rand((4, 64), 1), _rand((16, 64), 2)
+    gu, dn, ids, p = _rand((2, 16, 64), 3), _rand((2, 64, 8), 4), torch.zeros(4, 1, dtype=torch.int64, device="cuda"), torch.ones(4, 1, device="cuda")
+    calls = {"gemm_bias_act": lambda: ops.gemm_bias_act(x, w, trans_b=True), "moe_few_tokens": lambda: ops.moe_few_tokens(x, gu, dn, ids, p)}
+    y = ops.gemm_bias_act(x.requires_grad_(name == "backward"), w, trans_b=True)
+    calls["backward"] = lambda: y.backward(torch.ones_like(y))
+    word, look = nv._host_status[x.device.index][1], nv.mapped_status
+    if name == "moe_few_tokens":
+        calls[name]()
+    monkeypatch.setenv("PT_CHECK_STATUS", "1")
+
+    def leave_a_code(device):
+        address = look(device)
+        word.value = -4      # PT_ERR_TIMEOUT
+        return address
+    monkeypatch.setattr(nv, "mapped_status", leave_a_code)
+    monkeypatch.setattr(nv, "check_status", lambda device: look(device))
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        calls[name]()
+    assert word.value == 0

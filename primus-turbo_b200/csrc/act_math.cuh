@@ -38,6 +38,12 @@ template <int ACT> __device__ __forceinline__ float act_grad(float a) {
         return 0.3989422803f * a * __expf(-(0.7071067811f * a) * (0.7071067811f * a)) + 0.5f * erff(0.7071067811f * a) + 0.5f;
     }
 }
+// The slope at a pre-activation that was saved in 16 bits.  Beyond 65504 fp16 holds an infinity, and the square of a large bf16 value is one;
+// either would meet a factor that has become zero.  At +-100 every slope has long reached its limit in fp32, 0 or 1, so further values
+// take that (a NaN stays one).
+template <int ACT> __device__ __forceinline__ float act_grad_saved(float z) {
+    return act_grad<ACT>(fabsf(z) > 100.0f ? copysignf(100.0f, z) : z);
+}
 template <int ACT> __device__ __forceinline__ float glu_value(float a, float b, float p) { return act_value<ACT>(a) * b * p; }
 
 // GELU (erf form) of the epilogues: z Phi(z) = max(z, 0) - |z| / 2 erfc(|z| / sqrt 2), with erfc by the rational approximation 7.1.26 of

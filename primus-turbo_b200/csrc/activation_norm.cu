@@ -531,10 +531,10 @@ __global__ void __launch_bounds__(32 * kAbWarps, 4) act_bias_bwd_kernel(const Dy
                     for (int i = 0; i < V; ++i) g[i] *= f(x[i]);
                 };
                 switch (act) {
-                case PT_ACT_SILU: scale([](float v) { return act_grad<PT_ACT_SILU>(v); }); break;
-                case PT_ACT_GELU: scale([](float v) { return act_grad<PT_ACT_GELU>(v); }); break;
-                case PT_ACT_RELU: scale([](float v) { return act_grad<PT_ACT_RELU>(v); }); break;
-                default: scale([](float v) { return act_grad<PT_ACT_GELU_TANH>(v); }); break;
+                case PT_ACT_SILU: scale([](float v) { return act_grad_saved<PT_ACT_SILU>(v); }); break;
+                case PT_ACT_GELU: scale([](float v) { return act_grad_saved<PT_ACT_GELU>(v); }); break;
+                case PT_ACT_RELU: scale([](float v) { return act_grad_saved<PT_ACT_RELU>(v); }); break;
+                default: scale([](float v) { return act_grad_saved<PT_ACT_GELU_TANH>(v); }); break;
                 }
             }
             if (o != nullptr) {

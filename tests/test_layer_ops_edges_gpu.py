@@ -109,3 +109,33 @@ def test_check_status_variable_reaches_every_operator(monkeypatch, name):
     with pytest.raises(RuntimeError, match="gave up waiting"):
         calls[name]()
     assert word.value == 0
+
+
+# ------------------------------------------------------------------------------------------------ gemm_bias_act at the ends of the range
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("dt,av,bv", [(F16, 200.0, 100.0), (BF, 2.0 ** 50, 2.0 ** 20)])
+def test_slopes_of_large_pre_activations(dt, av, bv, act):
+    """Pre-activations of +-8 av bv: beyond fp16's range, or with a square beyond fp32's.  Every slope is 1 or 0 there, and all sums are
+    exact in the operands' type."""
+    from primus_turbo.pytorch.ops import gemm_bias_act
+    M, N, K = 3, 24, 8
+    a = torch.full((M, K), av, dtype=dt, device="cuda").requires_grad_()
+    sign = torch.where(torch.arange(N, device="cuda") % 3 == 0, -1.0, 1.0)
+    b = (bv * sign)[:, None].expand(N, K).to(dt).contiguous().requires_grad_()
+    bias = torch.zeros(N, dtype=dt, device="cuda").requires_grad_()
+    y = gemm_bias_act(a, b, bias=bias, activation=act, trans_b=True, out_dtype=F32)
+    assert torch.equal(y, (8 * av * bv * sign.clamp(min=0)).float().expand(M, N))
+    da, db, dbias = torch.autograd.grad(y, (a, b, bias), torch.ones_like(y))
+    open_ = sign.clamp(min=0)
+    assert torch.equal(da.float(), torch.full((M, K), 16 * bv, device="cuda"))
+    assert torch.equal(db.float(), (M * av * open_)[:, None].expand(N, K)) and torch.equal(dbias.float(), M * open_)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_gradients_of_nan_stay_nan(act):
+    from primus_turbo.pytorch.ops import gemm_bias_act
+    a, b = _rand((3, 16), 1), _rand((24, 16), 2)
+    a[1, 3] = float("nan")
+    a.requires_grad_()
+    (da,) = torch.autograd.grad(gemm_bias_act(a, b, activation=act, trans_b=True).sum(), a)
+    assert da[1].isnan().all() and da[[0, 2]].isfinite().all()

@@ -139,3 +139,24 @@ def test_gradients_of_nan_stay_nan(act):
     a.requires_grad_()
     (da,) = torch.autograd.grad(gemm_bias_act(a, b, activation=act, trans_b=True).sum(), a)
     assert da[1].isnan().all() and da[[0, 2]].isfinite().all()
+
+
+# ------------------------------------------------------------------------------------------------ the GELU of the epilogues
+@pytest.mark.parametrize("M,N", [(2000, 8), (2000, 5), (40000, 260), (40000, 257), (9000, 1028), (9000, 1001)])
+def test_gelu_in_fp32_is_right_in_its_tail(M, N):
+    """Exact pre-activations (one product of an fp16 value with a power of two) through both kernels, vector and ragged write-out.  The
+    result is max(z, 0) - x R exp(-x^2 / 2), x = |z|; in half steps u of fp32 the second term may be off by 3 for the fit of R, 8 + 8 for the
+    polynomial's roundings and its argument (conditioned by at most 2), 4 for the hardware exponential, 1.5 x^2 for the three roundings of its
+    argument, 5 for the products: (45 + 1.5 x^2) u; the difference adds one more."""
+    from primus_turbo.pytorch.kernels import _native as nv
+    from primus_turbo.pytorch.ops import gemm_bias_act
+    assert bool(nv.lib().pt_gemm_bias_act_few_rows(M, N, 8)) == (M == 2000)
+    a, b = torch.zeros(M, 8, dtype=F16, device="cuda"), torch.zeros(N, 8, dtype=F16, device="cuda")
+    a[:, 3] = torch.linspace(-12.5, 6.0, M, device="cuda").to(F16)
+    b[:, 3] = 2.0 ** -(torch.arange(N, device="cuda") % 5).to(F16)
+    z = a[:, 3:4].double() * b[:, 3].double()
+    y = gemm_bias_act(a, b, activation="gelu", trans_b=True, out_dtype=F32).double()
+    tail = 0.5 * z.abs() * torch.erfc(z.abs() / math.sqrt(2))
+    err = (y - (z.clamp(min=0) - tail)).abs()
+    tol = (45 + 1.5 * z * z) * U * tail + U * y.abs() + 1e-44
+    assert (err <= tol).all(), f"worst {float((err / tol).max()):.2f} x tolerance"

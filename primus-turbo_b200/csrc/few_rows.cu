@@ -823,7 +823,8 @@ int pt_moe_few_tokens(const void *x, const void *gate_up, const void *down, int 
     if (T == 0) return PT_OK;
     PT_REQUIRE(x && gate_up && down && ids && probs && scratch && out, "moe_few_tokens: null pointer");
     PT_REQUIRE(scratch_bytes >= pt_moe_few_tokens_scratch_bytes(T, top_k, I) && aligned(scratch, 16), "moe_few_tokens: scratch too small or unaligned");
-    PT_REQUIRE(aligned(x, 16) && aligned(out, 8), "moe_few_tokens: x must be 16-byte and out 8-byte aligned");
+    PT_REQUIRE(aligned(x, 16) && aligned(gate_up, 16) && aligned(down, 16) && aligned(out, 8),
+               "moe_few_tokens: x and the weights must start on 16-byte boundaries, out on an 8-byte one");
     cudaStream_t st = (cudaStream_t) stream;
     const int tok = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
     const int64_t slots = T * top_k, most = std::min<int64_t>(E, slots);   // experts that can be chosen

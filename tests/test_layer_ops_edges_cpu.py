@@ -30,3 +30,13 @@ def test_moe_few_tokens_refuses_a_tangent():
             moe_few_tokens(forward_ad.make_dual(x, x.clone()), *rest)
         with pytest.raises(RuntimeError, match="CUDA tensors only"):
             moe_few_tokens(x, *rest)
+
+
+@pytest.mark.parametrize("which", ["x", "gate_up", "down", "out"])
+def test_moe_few_tokens_abi_refuses_pointers_off_their_boundary(which):
+    from primus_turbo import _clib
+    lib = _clib.load()
+    at = dict(x=1 << 20, gate_up=2 << 20, down=3 << 20, out=4 << 20)
+    at[which] += 8 if which != "out" else 4
+    rc = lib.pt_moe_few_tokens(at["x"], at["gate_up"], at["down"], 0, 5 << 20, 8, 6 << 20, 3, 4, 2, 64, 16, 0, 7 << 20, 1 << 16, at["out"], None, None)
+    assert rc == -1 and b"boundar" in lib.pt_last_error()

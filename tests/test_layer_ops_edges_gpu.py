@@ -160,3 +160,16 @@ def test_gelu_in_fp32_is_right_in_its_tail(M, N):
     err = (y - (z.clamp(min=0) - tail)).abs()
     tol = (45 + 1.5 * z * z) * U * tail + U * y.abs() + 1e-44
     assert (err <= tol).all(), f"worst {float((err / tol).max()):.2f} x tolerance"
+
+
+# ------------------------------------------------------------------------------------------------ moe_few_tokens
+@pytest.mark.parametrize("which", ["gate_up", "down"])
+def test_moe_few_tokens_refuses_weights_off_the_16_byte_boundary(which):
+    from primus_turbo.pytorch.ops import moe_few_tokens
+    shapes = dict(gate_up=(4, 48, 64), down=(4, 64, 24))
+    w = {n: _rand((math.prod(s) + 8,), i, 0.1)[4 if n == which else 0:][:math.prod(s)].view(s) for i, (n, s) in enumerate(shapes.items())}
+    x, ids, p = _rand((3, 64), 5), torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.ones(3, 1, device="cuda")
+    with pytest.raises((RuntimeError, ValueError), match="16-byte boundaries"):
+        moe_few_tokens(x, w["gate_up"], w["down"], ids, p)
+    w[which] = w[which].clone()
+    assert moe_few_tokens(x, w["gate_up"], w["down"], ids, p).isfinite().all()

@@ -465,8 +465,9 @@ int pt_qk_norm_rope_bwd(const void *dq, const void *dk, const void *q, const voi
  * bases; ids [T, top_k] int32 / int64 (id_bytes 4 / 8), probs fp32 [T, top_k].  An id outside [0, E) (an expert of another shard,
  * a dropped slot) adds nothing; a token without any comes out as zeros.  act 0 = SiLU, 1 = GELU (erf).  H, I multiples of 8;
  * T at most PT_MOE_FEW_TOKENS_MAX, E at most 1024, top_k at most 32, T * top_k at most 2048.  p * act(g) * u is rounded to the
- * dtype between the two products.  Two launches; the same bits every run.  status: device or mapped host int, receives
- * PT_ERR_TIMEOUT if a bounded wait expires.  scratch: pt_moe_few_tokens_scratch_bytes bytes, 16-byte aligned.
+ * dtype between the two products (fp16: infinite beyond 65504).  Weights must be finite: tokens of other experts meet them as zeros.
+ * Two launches; the same bits every run.  status: device or mapped host int, receives PT_ERR_TIMEOUT if a bounded wait expires.
+ * scratch: pt_moe_few_tokens_scratch_bytes bytes, 16-byte aligned.
  * (The reference composes this from token_permute, grouped_gemm, swiglu_with_probs and token_unpermute.) */
 #define PT_MOE_FEW_TOKENS_MAX 128
 size_t pt_moe_few_tokens_scratch_bytes(int64_t T, int top_k, int64_t I);
@@ -474,15 +475,16 @@ int pt_moe_few_tokens(const void *x, const void *gate_up, const void *down, int 
                       int E, int top_k, int64_t H, int64_t I, int act, void *scratch, size_t scratch_bytes, void *out, int *status, void *stream);
 
 /* ---- matrix product with bias, activation and residual in its epilogue (csrc/gemm_fp8.cu, csrc/few_rows.cu) ----------
- * c [M, N] = act(a . b^T + bias) + residual, fp32 accumulate, rounded once: a [M, K], b [N, K], or [K, N] with b_mn (N a multiple of
- * 8 then); PT_BF16 / PT_F16, K a multiple of 8, 16-byte aligned bases; bias [N] of any of the three types or null, residual [M, N] of c's type or null.  act 0 = SiLU, 1 = GELU
- * (erf), 2 = none, 3 = ReLU, 4 = GELU (tanh).  z: null, or [M, N] in the operands' type, receives a . b^T + bias (the backward's
- * input).  residual may be c itself.  status: device or mapped host int, as in pt_gemm.  pt_gemm_bias_act_few_rows tells which kernels a
- * size runs on (1: the weight-streaming ones for few rows, 0: the tiles of pt_gemm), for measurements.  (The reference runs gemm and leaves bias, activation and residual to separate torch kernels:
+ * c [M, N] = act(a . b^T + bias) + residual, fp32 accumulate, rounded once: a [M, K], b [N, K], or [K, N] with b_mn (N a multiple of 8
+ * then); PT_BF16 / PT_F16, K a multiple of 8, 16-byte aligned bases; bias [N] of any of the three types or null, residual [M, N] of
+ * c's type or null.  act 0 = SiLU, 1 = GELU (erf), 2 = none, 3 = ReLU, 4 = GELU (tanh).  z: null, or [M, N] in the operands' type,
+ * receives a . b^T + bias (the backward's input).  residual may be c itself.  status: device or mapped host int, as in pt_gemm.
+ * pt_gemm_bias_act_few_rows tells which kernels a size runs on (1: the weight-streaming ones for few rows, 0: the tiles of pt_gemm),
+ * for measurements.  (The reference runs gemm and leaves bias, activation and residual to separate torch kernels:
  * primus_turbo/pytorch/ops/gemm.py.) */
 int pt_gemm_bias_act_few_rows(int64_t M, int64_t N, int64_t K);
-int pt_gemm_bias_act(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c, int c_dtype, void *z,
-                     int act, int64_t M, int64_t N, int64_t K, int *status, void *stream);
+int pt_gemm_bias_act(const void *a, const void *b, int b_mn, int ab_dtype, const void *bias, int bias_dtype, const void *residual, void *c,
+                     int c_dtype, void *z, int act, int64_t M, int64_t N, int64_t K, int *status, void *stream);
 /* Its element-wise backward: dz [M, N] = dy * act'(z) in the operands' type `dtype` (null: not written), dbias [N] = column sums of
  * the unrounded dz (null: none).  dy of type `dtype` or fp32; z may be null with act 2.  partial fp32 [parts, N] with
  * parts = pt_act_bias_bwd_parts(M, N) when dbias is given (null with one part).  Same bits every run. */

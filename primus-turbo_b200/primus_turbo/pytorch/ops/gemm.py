@@ -92,8 +92,10 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
 
     activation: None, "relu", "silu", "gelu" (erf form) or "gelu_tanh".  bias [N] in a's dtype or fp32; residual [M, N] in out_dtype
     (a's dtype by default).  Few rows (a decoding batch) run on a kernel that streams the weight over all SMs.  A contraction that is
-    not a multiple of 8 is padded first (copies of a and b), as in gemm.  Differentiable in
-    a, b, bias and residual; the pre-activation is kept in a's dtype for the backward when an activation needs it."""
+    not a multiple of 8 is padded first (copies of a and b), as in gemm.  Differentiable in a, b, bias and residual.  When an activation
+    needs it the pre-activation is kept for the backward in a's dtype, half of fp32's memory: the slope is taken at the rounded value (in
+    fp16 a positive one below 2^-25 is kept as zero, where ReLU's slope is zero), and the gradient behind the activation is rounded once to
+    a's dtype, the operand type of the two products that follow."""
     out_dtype = a.dtype if out_dtype is None else out_dtype
     check_gemm_bias_act(a, b, trans_b, bias, activation, residual, out_dtype)
     grad = a.requires_grad or b.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad)

@@ -18,13 +18,14 @@ def moe_few_tokens(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, t
                    act_type: str = "silu") -> torch.Tensor:
     """out[t] = sum over j of topk_probs[t, j] * down[e] . (act(gate[e] . x[t]) * (up[e] . x[t])) with e = topk_indices[t, j].
 
-    x [T, H], gate_up [E, 2 I, H] (gate rows first), down [E, H, I], bf16 or fp16, the weights starting on 16-byte boundaries (views into a
-    larger buffer that do not are refused; copying all experts would cost more than the layer); topk_indices int32 / int64 and topk_probs fp32
-    [T, K].  An index outside of [0, E), such as -1 for an expert of another shard, adds nothing.  H and I are multiples of 8;
-    T at most 128, E 1024, K 32, T * K 2048: longer inputs go through token_permute and grouped_gemm.  Forward only (no gradient);
-    act(gate) * up * prob is rounded to x's dtype between the two products.  The weights must be finite: the down product multiplies
-    the rows of an expert's weight with zeros for tokens that did not choose it, and an infinity would reach them.  act_type: "silu" or "gelu"
-    (erf form)."""
+    x [T, H], gate_up [E, 2 I, H] (gate rows first), down [E, H, I], bf16 or fp16, the weights starting on 16-byte boundaries (views into
+    a larger buffer that do not are refused; copying all experts would cost more than the layer); topk_indices int32 / int64 and
+    topk_probs fp32 [T, K].  An index outside of [0, E), such as -1 for an expert of another shard, adds nothing.  H and I are multiples
+    of 8; T at most 128, E 1024, K 32, T * K 2048: longer inputs go through token_permute and grouped_gemm.  Forward only (no gradient).
+    act(gate) * up * prob is rounded to x's dtype between the two products, as swiglu_with_probs rounds it: the second product's operand
+    type.  In fp16 a value of it beyond 65504 is therefore an infinity, also where the layer's output would be finite.  The weights must be
+    finite: the down product multiplies the rows of an expert's weight with zeros for tokens that did not choose it, and an infinity
+    would reach them.  act_type: "silu" or "gelu" (erf form)."""
     if torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad or down.requires_grad or topk_probs.requires_grad):
         raise RuntimeError("moe_few_tokens has no backward: call it under torch.no_grad(), or train through token_permute and grouped_gemm")
     if _forward_ad_active() and any(forward_ad.unpack_dual(t).tangent is not None for t in (x, gate_up, down, topk_probs)):

@@ -194,7 +194,13 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
         if (threadIdx.x < 32) s_bits[threadIdx.x] = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < T * a.top_k; i += Cfg::kThreads) {
-            const int64_t id = a.id_bytes == 8 ? reinterpret_cast<const int64_t *>(a.ids)[i] : (int64_t) reinterpret_cast<const int *>(a.ids)[i];
+            int64_t id;
+            if constexpr (KIND == FR_DOWN) {   // before its wait for the kernel ahead: from L2, where what was written earlier stands, not from L1
+                id = a.id_bytes == 8 ? (int64_t) __ldcg(reinterpret_cast<const long long *>(a.ids) + i)
+                                     : (int64_t) __ldcg(reinterpret_cast<const int *>(a.ids) + i);
+            } else {
+                id = a.id_bytes == 8 ? reinterpret_cast<const int64_t *>(a.ids)[i] : (int64_t) reinterpret_cast<const int *>(a.ids)[i];
+            }
             const bool valid = id >= 0 && id < a.experts;
             s_ids[i] = valid ? (int16_t) id : (int16_t) -1;
             if (valid) atomicOr(&s_bits[id >> 5], 1u << (id & 31));

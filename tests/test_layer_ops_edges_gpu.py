@@ -173,3 +173,38 @@ def test_moe_few_tokens_refuses_weights_off_the_16_byte_boundary(which):
         moe_few_tokens(x, w["gate_up"], w["down"], ids, p)
     w[which] = w[which].clone()
     assert moe_few_tokens(x, w["gate_up"], w["down"], ids, p).isfinite().all()
+
+
+@pytest.mark.parametrize("idt", [torch.int32, torch.int64])
+def test_moe_few_tokens_reads_the_routing_of_this_call(idt):
+    """The routing is rewritten in place by the kernel just ahead of every call, eagerly and in a replayed graph: the second product, which
+    starts before the first has finished, must see the new one."""
+    from primus_turbo.pytorch.ops import moe_few_tokens
+    T, E, K, H, I, rounds = 6, 8, 2, 512, 264, 24
+    x, gu, dn, p = _rand((T, H), 1), _rand((E, 2 * I, H), 2, 0.05), _rand((E, H, I), 3, 0.06), torch.rand(T, K, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(4)
+    tables = torch.rand((rounds, T, E), generator=g, device="cuda").topk(K, dim=2).indices.to(idt)
+    want = []
+    for t in tables:
+        torch.cuda.synchronize()
+        want.append(moe_few_tokens(x, gu, dn, t.clone(), p))
+    torch.cuda.synchronize()
+    ids, got = tables[0].clone(), []
+
+    def steps():
+        for t in tables:
+            ids.copy_(t)
+            got.append(moe_few_tokens(x, gu, dn, ids, p))
+    steps()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got.clear()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        steps()
+    for _ in range(3):
+        for y in got:
+            y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

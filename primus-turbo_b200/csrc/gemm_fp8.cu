@@ -667,14 +667,13 @@ __global__ void __launch_bounds__((GemmCfg<BLOCK_N, mode_is_mx(MODE), MODE == GE
             tc_fence_after_sync();
             const uint32_t taddr = tmem_base + ((uint32_t) (q * 32) << 16) + acc_stage * BLOCK_N;
             auto release = [&]() { mbar_arrive(&tmem_empty_bar[acc_stage]); };
-            if constexpr (MODE == GEMM_HP_EPI)
-                {
+            if constexpr (MODE == GEMM_HP_EPI) {
                 constexpr int kChunks = (BLOCK_N + 31) / 32;
                 const int half = (warp - kEpiWarp0) >> 2;
                 epilogue_fused_block<BLOCK_N>(p, taddr, have_acc, tile_row0, c_row_end, n0, stg, lane, half ? kChunks / 2 : 0, half ? kChunks : kChunks / 2, release);
-            }
-            else
+            } else {
                 epilogue_store_block<BLOCK_N, MODE>(p, taddr, have_acc, tile_row0, c_row_end, n0, gi, stg, lane, 0, (BLOCK_N + 31) / 32, release);
+            }
             if (have_acc && ++acc_stage == kAccStages) { acc_stage = 0; acc_phase ^= 1; }
         }
     }

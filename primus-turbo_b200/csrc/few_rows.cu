@@ -6,22 +6,22 @@
 // its narrow one (N = 16 .. 256), so that a CTA streams 16 KiB weight blocks [128 features][64 of K] through a TMA ring and the
 // tensor core takes each of them in four instructions, far faster than it arrives.  Blocks of up to 128 tokens: two CTAs to an SM with
 // about 100 KiB each on their way, which covers the memory latency (148 SMs x 200 KiB = 29 MiB in flight) and lets one CTA's start and
-// write-out hide behind the other's stream.  Up to 192: one CTA with 200 KiB and more warps for the write-out.  Up to 256: pairs of CTAs whose
-// tensor cores multiply 256 features together (cta_group::2), each holding half of the tokens, because there what an SM takes in from L2
-// (about 108 GB/s) bounds it: 512 x 4096 x 4096 24.8 us by blocks of 192, 21.1 by pairs.
+// write-out hide behind the other's stream.  Up to 192: one CTA with 200 KiB and more warps for the write-out.  Up to 256: pairs of CTAs
+// whose tensor cores multiply 256 features together (cta_group::2), each holding half of the tokens, because there what an SM takes in
+// from L2 (about 108 GB/s) bounds it: 512 x 4096 x 4096 24.8 us by blocks of 192, 20.8 by pairs.
 //   The contraction is split over the CTAs of a cluster when the features alone would leave SMs idle: every CTA puts its partial
 // [tokens][128] block of fp32 sums into its own shared memory and the CTAs add each other's blocks for their share of the tokens
-// through distributed shared memory, beginning with their own and going on by rank.  So there is no workspace, no counter and no atomic: results do
-// not depend on timing, and calls on different streams or in different graphs share nothing.
+// through distributed shared memory, beginning with their own and going on by rank.  So there is no workspace, no counter and no
+// atomic: results do not depend on timing, and calls on different streams or in different graphs share nothing.
 //
 //   warp 0      producer (TMA; for experts also which tokens chose them)
 //   warp 1      one thread issues the MMAs; owns the tensor memory
 //   the others  for experts: copy the tokens' rows into the stages; then tensor memory -> shared memory
 //   all         sum over the cluster, epilogue, write-out
 //
-// Measured (B200, bf16, replayed graphs, inputs beyond L2): 1 x 14336 x 4096 (rows, features, K) 22.0 us, 5.3 TB/s of weights; 1 x 64128 x 4096
-// 81 us, 6.5 TB/s; 64 x 4096 x 4096 11.7 us; 129 x 4096 x 4096 13.6 us; 333 x 4096 x 4096 19.0 us, 0.59 PFLOP/s.  One token through eight
-// experts of 7168 x 2048 114 us, 6.2 TB/s; 64 tokens on 28 of 32 such experts 375 to 388 us, 6.5 TB/s.
+// Measured (B200, bf16, replayed graphs, inputs beyond L2): 1 x 14336 x 4096 (rows, features, K) 21.6 us, 5.4 TB/s of weights; 1 x
+// 64128 x 4096 81 us, 6.5 TB/s; 64 x 4096 x 4096 11.3 us; 129 x 4096 x 4096 13.4 us; 333 x 4096 x 4096 18.2 us, 0.61 PFLOP/s.  One
+// token through eight experts of 7168 x 2048 112.5 us, 6.3 TB/s; 64 tokens on 28 of 32 such experts 375 to 393 us, 6.3 to 6.5 TB/s.
 //
 // Mixture, two kernels:
 //   GATE_UP  grid (blocks of 64 features x split, chosen experts): the block is 64 gate rows and the 64 up rows that belong to them.
@@ -81,7 +81,8 @@ struct FewRowsArgs {
 };
 
 template <int TOK, bool PAIR> struct FrCfg {
-    static constexpr int kEpiWarps = TOK <= 32 ? 4 : TOK <= 128 ? 8 : 16;   // per quarter of the accumulator's rows: one, or two that share the tokens
+    // per quarter of the accumulator's rows: one, two or four that share the tokens
+    static constexpr int kEpiWarps = TOK <= 32 ? 4 : TOK <= 128 ? 8 : 16;
     static constexpr int kThreads = 64 + 32 * kEpiWarps;
     static constexpr int kCtas = TOK > 128 ? 1 : 2;           // per SM
     // Six, five, four and three full stages of two CTAs per SM; five of single CTAs, six of pairs.  Smaller stages fit more often.
@@ -184,7 +185,8 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
     }
     if (KIND != FR_DOWN) {   // DOWN waits later: what it reads up to there is not written by the kernel before it
         grid_dep_wait();
-        if (TOK <= 128 && warp == 1) grid_dep_launch();   // after this warp's allocation: what is launched then cannot wait for us holding its columns
+        // after this warp's allocation: what is launched then cannot wait for us holding its columns
+        if (TOK <= 128 && warp == 1) grid_dep_launch();
     }
 
     // ---- routing: which experts are chosen, and by whom
@@ -664,16 +666,16 @@ __global__ void __launch_bounds__(FrCfg<TOK, PAIR>::kThreads, FrCfg<TOK, PAIR>::
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-// CTAs that are resident at once in clusters of `ctas`, two or one (wide) per SM (GPCs do not divide evenly; measured on 148 SMs with one CTA per
-// SM: 33 clusters of four and 14 of eight run together, 34 and 16 in two waves).  With two CTAs per SM no such loss was seen.  The driver's occupancy query is not asked: it
-// answers one CTA per SM for these kernels, and launches after it do run one per SM (333 x 4096 x 4096 in blocks of 128: 29.4 us, else 23.0).
+// CTAs that are resident at once in clusters of `ctas`, two or one (wide) per SM.  GPCs do not divide evenly: on 148 SMs with one CTA per SM, 33
+// clusters of four and 14 of eight ran together, 34 and 16 in two waves.  With two CTAs per SM no such loss was seen.
 static double fr_resident(bool wide, int ctas) {
     const double sms = sm_count();
     return !wide ? 2.0 * sms : ctas <= 2 ? sms : ctas == 4 ? sms * 33 / 37 : sms * 28 / 37;
 }
-// Whether a launch of `ctas` CTAs on a kernel for two per SM takes the ring of both: if each of them gets an SM for itself.  Measured (us): 64 x 4096 x
-// 4096 12.9 -> 12.0, 4000 x 512 x 512 11.9 -> 11.3; experts, 37 tokens in two of 60 of 1744 x 568 66.9 -> 63.9, but with 16 clusters of eight, of which two
-// would start late, 64 tokens in six of 64 of 2048 x 1408 215 -> 271.  Up to 16 tokens it gains nothing (1 x 1024 x 4096 6.5 -> 6.7).
+// Whether a launch of `ctas` CTAs on a kernel for two per SM takes the ring of both: if each of them gets an SM for itself.  Measured (us): 64 x
+// 4096 x 4096 12.9 -> 12.0, 4000 x 512 x 512 11.9 -> 11.3; experts, 37 tokens in two of 60 of 1744 x 568 66.9 -> 63.9, but with 16 clusters of
+// eight, of which two would start late, 64 tokens in six of 64 of 2048 x 1408 215 -> 271.  Up to 16 tokens it gains nothing (1 x 1024 x 4096 6.5
+// -> 6.7).
 static bool fr_deep(int tok, int64_t ctas, int cluster) { return tok > 16 && tok <= 128 && (double) ctas <= fr_resident(true, cluster); }
 
 template <int TOK, int KIND, bool PAIR = false>
@@ -709,13 +711,14 @@ static int fr_launch(const CUtensorMap &tw, const CUtensorMap &tx, FewRowsArgs a
     return PT_OK;
 }
 
-// Estimated time of a launch in us: `tiles` weight blocks wide, `blocks` blocks of `block` tokens on the kernel for up to `tok`, `chunks` 64-wide
-// steps of the contraction, s CTAs or pairs per cluster.  A fixed part, and the longest of: a CTA's own steps (an SM takes in about 108 GB/s),
-// the bytes from and to memory (one CTA per SM does not quite saturate it), all stages out of L2 (15 TB/s).  CTAs beyond those
-// resident at once are further waves.  Measured (us, SiLU epilogue; rows x features x K, kernel : block / s): 64 x 4096 x 4096 64 / 1, 2, 4, 8 24.8, 16.1,
-// 12.8, 13.0; 129 x 4096 x 4096 128 : 80 / 4 15.6, 192 : 144 / 2, 4 17.1, 13.6, 256 : 144 / 2, 4 16.7, 26.5 (two waves); 333 x 4096 x 4096 128 : 112 / 2
-// 23.3, 192 : 176 / 2 19.0, 256 : 176 / 2 19.0; 512 x 4096 x 4096 128 : 128 / 2 24.6, 192 : 128 / 1 24.8, 256 : 256 / 2 21.1.  What the estimates
-// pick, the tiles of gemm_bias_act included, was within 5 % of the best in 39 of 45 sizes measured, 16 % from it at worst (513 x 512 x 1024).
+// Estimated time of a launch in us: `tiles` weight blocks wide, `blocks` blocks of `block` tokens on the kernel for up to `tok`, `chunks`
+// 64-wide steps of the contraction, s CTAs or pairs per cluster.  A fixed part, and the longest of: a CTA's own steps (an SM takes in about 108
+// GB/s), the bytes from and to memory (one CTA per SM does not quite saturate it), all stages out of L2 (15 TB/s).  CTAs beyond those resident
+// at once are further waves.  Measured (us, SiLU epilogue; rows x features x K, kernel : block / s): 64 x 4096 x 4096 64 / 1, 2, 4, 8 24.8,
+// 16.1, 12.8, 13.0; 129 x 4096 x 4096 128 : 80 / 4 15.6, 192 : 144 / 2, 4 17.1, 13.6, 256 : 144 / 2, 4 16.7, 26.5 (two waves); 333 x 4096 x 4096
+// 128 : 112 / 2 23.3, 192 : 176 / 2 19.0, 256 : 176 / 2 19.0; 512 x 4096 x 4096 128 : 128 / 2 24.6, 192 : 128 / 1 24.8, 256 : 256 / 2 21.1.
+// What the estimates pick, the tiles of gemm_bias_act included, is within 5 % of the best plan in 41 of 54 sizes of 65 to 1030 rows and 22 %
+// from it at worst (1030 x 4096 x 14336, 141 us); the misses are mostly products of 6 to 12 us.
 static double fr_cost(int tok, int block, int64_t tiles, int64_t blocks, int64_t chunks, int s) {
     const bool wide = tok > 128, pair = tok == kFrPairTok;
     if (pair) tiles = (tiles + 1) / 2 * 2;
@@ -742,7 +745,8 @@ static FrPlan fr_plan(int64_t rows, int64_t n, int64_t k) {
     const int64_t tiles = ceil_div(n, kFrFeat), chunks = ceil_div(k, 64);
     FrPlan best{0, 0, 1, 0.0};
     for (int tok : {16, 32, 64, 128, 192, kFrPairTok}) {
-        if ((tok < 128 && tok < rows) || (tok > 16 && tok <= 128 && tok / 2 >= rows) || (tok > 128 && rows <= 64)) continue;   // no room, or more than half of it empty
+        // no room, or more than half of it empty
+        if ((tok < 128 && tok < rows) || (tok > 16 && tok <= 128 && tok / 2 >= rows) || (tok > 128 && rows <= 64)) continue;
         for (int more = 0; more <= (tok >= 128 && rows > 64 ? 1 : 0); ++more) {   // as few blocks as possible, or one more
             const int block = (int) ceil_div(ceil_div(rows, ceil_div(rows, tok) + more), 16) * 16;
             const int64_t blocks = ceil_div(rows, block);

@@ -974,11 +974,11 @@ int gemm_hp_host(const void *a, const void *b, int ab_dtype, void *c, int c_dtyp
     return dispatch_block_n<GEMM_HP>(0, a, a_rows_total, b, b_rows, p, mx, max_ctas, (cudaStream_t) stream);
 }
 
-// Which kernels a product runs on: the weight-streaming ones of few_rows.cu or the tiles above (CTA pairs), whichever the estimate
-// makes faster.  The pairs take about 10 us and, per wave of 256 x 256 tiles, 4.8 us per 1024 of K plus 3 us of epilogue between waves.
-// Measured (us, SiLU epilogue) few rows / pairs: 129 x 4096 x 128 (M, N, K) 5.6 / 9.9; 129 x 4096 x 4096 13.6 / 29.1, 512 x 4096 x 4096 21.2 / 29.6, 768 x
-// 4096 x 4096 27.3 / 30.7, 1024 x 4096 x 4096 31.0 / 30.4; 192 x 14336 x 4096 30.9 / 35.6, 333 x 14336 x 4096 56.6 / 52.6, 512 x 14336 x 4096 64.5 / 54.0;
-// 512 x 4096 x 14336 47.7 / 78.0, 768 x 4096 x 14336 73.6 / 80.
+// Which kernels a product runs on: the weight-streaming ones of few_rows.cu or the tiles above (CTA pairs), whichever the estimate makes faster.
+// The pairs take about 10 us and, per wave of 256 x 256 tiles, 4.8 us per 1024 of K plus 3 us of epilogue between waves.  Measured (us, SiLU
+// epilogue) few rows / pairs: 129 x 4096 x 128 (M, N, K) 5.6 / 9.9; 129 x 4096 x 4096 13.6 / 29.1, 512 x 4096 x 4096 21.2 / 29.6, 768 x 4096 x
+// 4096 27.3 / 30.7, 1024 x 4096 x 4096 31.0 / 30.4; 192 x 14336 x 4096 30.9 / 35.6, 333 x 14336 x 4096 56.6 / 52.6, 512 x 14336 x 4096 64.5 /
+// 54.0; 512 x 4096 x 14336 47.7 / 78.0, 768 x 4096 x 14336 73.6 / 80.
 static bool few_rows_better(int64_t M, int64_t N, int64_t K) {
     if (M <= 64) return true;
     if (M > (int64_t) 65535 * 128) return false;   // blocks of tokens are the grid's second extent

@@ -11,8 +11,10 @@
 // neighbouring lanes and never leaves their registers: a lane holds whole pairs (the vectors at i and at i + R / 2), so the
 // rotation needs no exchange and the norm one shuffle reduction.  A warp takes heads of one token only: the token's cosines and
 // sines and the gains are converted once for all of them.  Arithmetic in fp32, one rounding at the end.
-// Measured (B200): forward 8192 x 72 heads of 128, bf16, 59.7 us (5.1 TB/s); forward and backward of 8191 x 40 heads, fp16, half rotated, 94.1 us
-// (4.5 TB/s of the five passes).  Issue slots are 0.70 and 0.58 busy and loads in flight bound the rest.
+// Measured (B200): forward 8192 x 72 heads of 128, bf16, 59.7 us (5.1 TB/s); forward and backward of 8191 x 40 heads, fp16, half
+// rotated, 94.1 us (4.5 TB/s of the five passes); fp32, 8192 x 40 heads 52.3 us (6.4 TB/s) and 135 (6.2).  Issue slots are 0.69 and
+// 0.62 busy and loads in flight bound the rest.  Heads that take two elements an access for four (R / 2 not a multiple of four)
+// cost 1.5 times the time.
 #include <algorithm>
 #include <type_traits>
 
@@ -627,7 +629,8 @@ static int qk_check(const QkArgs &a, int dtype, int64_t B) {
                "qk_norm_rope: the head size must lie in [1, %d] and the rotated part be even and no larger (got %d, %d)", kQkMaxD, a.D, a.R);
     PT_REQUIRE(a.T < (1ll << 31) && a.T * (a.heads[0] + (int64_t) a.heads[1]) < (1ll << 31), "qk_norm_rope: tokens x heads exceed 32-bit indices");
     PT_REQUIRE(a.pos_bytes == 0 || a.pos_bytes == 4 || a.pos_bytes == 8, "qk_norm_rope: positions must be int32 or int64");
-    PT_REQUIRE(a.T == 0 || (a.pos_bytes == 0) == (a.positions == nullptr), "qk_norm_rope: positions and their size go together");   // an empty tensor is a null pointer
+    // an empty tensor is a null pointer
+    PT_REQUIRE(a.T == 0 || (a.pos_bytes == 0) == (a.positions == nullptr), "qk_norm_rope: positions and their size go together");
     for (int r = 0; r < 2; ++r)
         PT_REQUIRE(a.T == 0 || a.heads[r] == 0 || (a.x[r] && a.out[r] && a.gamma[r]), "qk_norm_rope: null pointer");
     PT_REQUIRE(a.T == 0 || a.R == 0 || (a.cos && a.sin), "qk_norm_rope: null table");
@@ -657,7 +660,8 @@ int pt_qk_norm_rope_fwd(const void *q, const void *k, int dtype, const void *q_g
     qk_strides(q_strides, B, S, Hq, a.xb[0], a.xt[0], a.xh[0]);
     qk_strides(k_strides, B, S, Hk, a.xb[1], a.xt[1], a.xh[1]);
     a.heads[0] = Hq; a.heads[1] = Hk; a.cos = cos; a.sin = sin; a.positions = positions; a.pos_bytes = pos_bytes;
-    a.T = B * S; a.S = S; a.P = P; a.D = D; a.R = R; a.eps = eps; a.inv_d = 1.f / (float) std::max(D, 1); a.g0 = zero_centered ? 1.f : 0.f; a.status = status;
+    a.T = B * S; a.S = S; a.P = P; a.D = D; a.R = R; a.eps = eps; a.inv_d = 1.f / (float) std::max(D, 1); a.g0 = zero_centered ? 1.f : 0.f;
+    a.status = status;
     const int rc = qk_check(a, dtype, B);
     if (rc != PT_OK) return rc;
     if (a.T == 0 || Hq + Hk == 0) return PT_OK;
@@ -683,7 +687,8 @@ int pt_qk_norm_rope_bwd(const void *dq, const void *dk, const void *q, const voi
     qk_strides(dq_strides, B, S, Hq, a.gb[0], a.gt[0], a.gh[0]);
     qk_strides(dk_strides, B, S, Hk, a.gb[1], a.gt[1], a.gh[1]);
     a.heads[0] = Hq; a.heads[1] = Hk; a.cos = cos; a.sin = sin; a.positions = positions; a.pos_bytes = pos_bytes;
-    a.T = B * S; a.S = std::max<int64_t>(S, 1); a.P = P; a.D = D; a.R = R; a.eps = eps; a.inv_d = 1.f / (float) std::max(D, 1); a.g0 = zero_centered ? 1.f : 0.f; a.status = status;
+    a.T = B * S; a.S = std::max<int64_t>(S, 1); a.P = P; a.D = D; a.R = R; a.eps = eps; a.inv_d = 1.f / (float) std::max(D, 1);
+    a.g0 = zero_centered ? 1.f : 0.f; a.status = status;
     const int rc = qk_check(a, dtype, B);
     if (rc != PT_OK) return rc;
     for (int r = 0; r < 2; ++r) PT_REQUIRE(a.T == 0 || a.heads[r] == 0 || a.dy[r], "qk_norm_rope backward: null pointer");

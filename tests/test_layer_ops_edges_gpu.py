@@ -208,3 +208,44 @@ def test_moe_few_tokens_reads_the_routing_of_this_call(idt):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------------ host threads
+@pytest.mark.parametrize("shared_stream", [False, True])
+def test_same_bits_from_several_threads(shared_stream):
+    """Four host threads, each on a stream of its own or all on one, forward and backward: the bits of the same calls one after another."""
+    import threading
+    from primus_turbo.pytorch import ops
+    t = torch.ones(64, 32, device="cuda")
+    cases = []
+    for i in range(4):
+        x, w, b = _rand((3 + 40 * i, 256), i), _rand((264, 256), 10 + i, 0.06), _rand((264,), 20 + i)
+        q, g = _rand((5 + i, 6, 64), 30 + i), _rand((64,), 40 + i)
+        gu, dn, p = _rand((4, 96, 256), 50 + i, 0.06), _rand((4, 256, 48), 60 + i, 0.1), torch.rand(3, 2, device="cuda")
+        ids = (torch.arange(6, device="cuda").view(3, 2) + i) % 4
+
+        def run(x=x, w=w, b=b, q=q, g=g, gu=gu, dn=dn, p=p, ids=ids):
+            a, v, h = x.detach().requires_grad_(), w.detach().requires_grad_(), q.detach().requires_grad_()
+            y = ops.gemm_bias_act(a, v, bias=b, activation="gelu", trans_b=True)
+            z = ops.qk_norm_rope(h, h[:, :2], g, g, t, t)
+            return [y.detach(), *torch.autograd.grad(y, (a, v), y.detach()), z[0].detach(), *torch.autograd.grad(z, h, [z[0].detach(), z[1].detach()]),
+                    ops.moe_few_tokens(x[:3], gu, dn, ids, p)]
+        cases.append(run)
+    want = [run() for run in cases]
+    torch.cuda.synchronize()
+    common, wrong = torch.cuda.Stream(), []
+
+    def work(i):
+        stream = common if shared_stream else torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(25):
+                got = cases[i]()
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong

@@ -249,3 +249,44 @@ def test_same_bits_from_several_threads(shared_stream):
     for th in threads:
         th.join()
     assert not wrong
+
+
+# ------------------------------------------------------------------------------------------------ captured training steps
+@pytest.mark.parametrize("M,N,K", [(3, 264, 96), (300, 264, 96), (8200, 1028, 264)])
+@pytest.mark.parametrize("fused", [False, True])
+def test_captured_training_step_follows_new_inputs(M, N, K, fused):
+    """Forward and backward of a product and of the head norm in one graph, replayed on inputs that changed: the bits of eager calls on them,
+    also where the weight's gradient is added to main_grad."""
+    from primus_turbo.pytorch import ops
+    a, b, bias = (t.requires_grad_() for t in (_rand((M, K), 1), _rand((N, K), 2, 0.1), _rand((N,), 3)))
+    q, g, t = _rand((M, 3, 64), 4).requires_grad_(), _rand((64,), 5).requires_grad_(), torch.linspace(-1, 1, 16 * 32, device="cuda").view(16, 32)
+    pos, dy, dq = torch.arange(M, device="cuda") % 16, _rand((M, N), 6), _rand((M, 3, 64), 7)
+    if fused:
+        b.main_grad, b.grad_added_to_main_grad = torch.zeros(N, K, device="cuda"), False
+
+    def step():
+        y = ops.gemm_bias_act(a, b, bias=bias, activation="gelu", trans_b=True, fuse_bgrad_accum_pattern="megatron" if fused else None)
+        u, _ = ops.qk_norm_rope(q, q.detach()[:, :1], g, g.detach(), t, t, positions=pos)
+        grads = torch.autograd.grad([y, u], [a, b, bias, q, g], [dy, dq])
+        return [y.detach(), u.detach(), grads[0], b.main_grad if fused else grads[1], *grads[2:]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (11, 12):
+        with torch.no_grad():
+            for i, x in enumerate((a, b, bias, q, g, dy, dq)):
+                x.copy_(_rand(x.shape, seed * 10 + i))
+            pos.copy_(torch.randint(0, 16, (M,), generator=torch.Generator().manual_seed(seed)).cuda())
+        if fused:
+            b.main_grad.fill_(0.5)
+        want = [w.clone() for w in step()]
+        if fused:
+            b.main_grad.fill_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, w) for x, w in zip(held, want))
